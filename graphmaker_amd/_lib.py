@@ -23,8 +23,27 @@ EXPORTS = [
     "gm_layernorm_bwd_workspace_bytes", "gm_layernorm_bwd", "gm_spmm_mean_bwd", "gm_embedding_bwd_workspace_bytes", "gm_embedding_bwd",
     "gm_hadamard_gather_bwd", "gm_softmax_ce2_workspace_bytes", "gm_softmax_ce2", "gm_ce2_diff", "gm_head_diff_bwd",
     "gm_relu_bwd", "gm_dropout", "gm_embedding_fwd", "gm_denoise_match2", "gm_bitmap_lookup",
+    "gm_token_embedding_fwd", "gm_token_embedding_bwd_workspace_bytes", "gm_token_embedding_bwd", "gm_layer_norm_fwd",
+    "gm_layer_norm_bwd_workspace_bytes", "gm_layer_norm_bwd", "gm_class_log_prob_workspace_bytes", "gm_class_log_prob_fwd",
+    "gm_class_log_prob_bwd", "gm_sequence_loss_workspace_bytes", "gm_policy_loss_fwd", "gm_preference_loss_fwd",
+    "gm_sequence_loss_bwd",
     "gm_triangles_per_node", "gm_same_class_degree", "gm_bitmap_square", "gm_class_bitmaps", "gm_masked_degree",
 ]
+
+
+# Argument types of the entry points that take typed rows: with them ctypes converts plain Python numbers and addresses, so
+# a call names each argument once.  i = int64, d = int, f = float, p = device pointer (an address or None).
+_SIGNATURES = {
+    "gm_token_embedding_fwd": "iiipdpidfpip", "gm_token_embedding_bwd_workspace_bytes": "iii",
+    "gm_token_embedding_bwd": "iiipdipidfpipip", "gm_layer_norm_fwd": "iipidppdfpippp",
+    "gm_layer_norm_bwd_workspace_bytes": "ii", "gm_layer_norm_bwd": "iipipidpppdpipppip",
+    "gm_class_log_prob_workspace_bytes": "ii", "gm_class_log_prob_fwd": "iipidpdipppip",
+    "gm_class_log_prob_bwd": "iippidpdippip", "gm_sequence_loss_workspace_bytes": "ii",
+    "gm_policy_loss_fwd": "iippppppdfffdpppppip", "gm_preference_loss_fwd": "iippppdffdppppip",
+    "gm_sequence_loss_bwd": "iipppdpppp",
+}
+_CTYPES = {"i": C.c_int64, "d": C.c_int, "f": C.c_float, "p": C.c_void_p}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # GM_DTYPE_*
 
 
 class GraphMakerHipError(RuntimeError):
@@ -57,6 +76,10 @@ def load():
         for name in ("gm_tower_prep_floats", "gm_onehot_prep_floats", "gm_gemm_workspace_bytes", "gm_mlp2_hidden_grad_workspace_bytes", "gm_colsum_workspace_bytes", "gm_layernorm_bwd_workspace_bytes",
                      "gm_softmax_ce2_workspace_bytes", "gm_embedding_bwd_workspace_bytes"):
             getattr(lib, name).restype = C.c_int64
+        for name, kinds in _SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.argtypes = [_CTYPES[k] for k in kinds]
+            fn.restype = C.c_int64 if name.endswith("_bytes") else C.c_int
         _lib = lib
     return _lib
 
@@ -104,3 +127,15 @@ I32 = C.c_int
 U64 = C.c_uint64
 U32 = C.c_uint32
 F32 = C.c_float
+
+
+def launch(name, device, *args):
+    """One call of an entry point in _SIGNATURES on `device`'s current stream, whatever device is current."""
+    fn = getattr(load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        _check(rc, name)

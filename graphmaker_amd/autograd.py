@@ -11,10 +11,22 @@ Operators (each a torch.autograd.Function over contiguous float32 device tensors
     hadamard_gather(h, src, dst)     h[src] * h[dst]                           model/gnn.py:246
     softmax_ce2(logits, target)      F.cross_entropy, 2 classes, mean          model/diffusion.py:139,513
     dropout(x, p, seed, call)        nn.Dropout in training mode               model/gnn.py:31,37
+
+Operators for wider models, large vocabularies and fine-tuning on rewards or preferences (no counterpart in the reference;
+float32, bfloat16 or float16 rows, sums in float32 or float64):
+    token_embedding(weight, tokens, scale, padding_idx)            scaled lookup; gradient by sorted tokens
+    layer_norm(x, gamma, beta, eps)                                layer norm over rows of any width
+    class_log_prob(logits, classes, ignore_index)                  log-probability of one class a row
+    policy_loss(log_prob, old_log_prob, advantage, ...)            clipped policy loss with a KL term
+    preference_loss(log_prob, ref_log_prob, offsets, ...)          loss of preferred over rejected sequences
+They enqueue on the current stream of their tensors' device, keep their workspaces to one call, read nothing back to the
+host and can be captured in a HIP graph, forward and backward.  Capture a backward pass only when no graph recorded eagerly
+over the same leaf tensors is still alive: torch ties a leaf's gradient accumulation to the stream of the first such graph.
 """
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
@@ -177,6 +189,9 @@ class _Mlp2(torch.autograd.Function):
         return dx, dW1, db1, dW2, db2, None, None
 
 
+LAYERNORM_BWD_MAX = 1024        # gm_layernorm_bwd keeps a row's columns in registers; wider blocks use gm_layer_norm_bwd
+
+
 class _UpdateBlock(torch.autograd.Function):
     """Linear -> ReLU -> LayerNorm of GNNLayer / MLPLayer (model/gnn.py:27-38)."""
 
@@ -205,6 +220,11 @@ class _UpdateBlock(torch.autograd.Function):
         dev = a.device
         da = torch.empty_like(a)
         dgb = torch.empty((2, N), dtype=torch.float32, device=dev)
+        if N > LAYERNORM_BWD_MAX:
+            _layer_norm_bwd(g, a, mean, rstd, gamma, da, dgb[0], dgb[1])
+            L.call("gm_relu_bwd", I64(a.numel()), ptr(da), ptr(a), ptr(da), stream_ptr())
+            dx, dW, db = _linear_backward(x, W, da, (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]))
+            return dx, dW, db, dgb[0], dgb[1], None
         need = L.load().gm_layernorm_bwd_workspace_bytes(I64(M), I64(N))
         ws = _scratch(need, dev)
         L.call("gm_layernorm_bwd", I64(M), I64(N), ptr(g), I64(N), ptr(a), I64(N), ptr(mean), ptr(rstd), ptr(gamma), I32(1),
@@ -443,3 +463,397 @@ def dropout(x, p, state):
         return x
     seed, call = state.next()
     return _Dropout.apply(x, float(p), seed, call)
+
+
+# ------------------------------------------------------------------ wider models and fine-tuning
+def _on_gpu(t, what):
+    if not t.is_cuda:
+        raise L.GraphMakerHipError(f"{what}: graphmaker_amd runs on a ROCm device only (tensor is on {t.device})")
+
+
+def _same_device(t, what, device):
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    return t
+
+
+def _row_dtype(t, what):
+    code = L.DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rows(t, width):
+    """(tensor, leading dimension) of t as rows of `width` elements; a view where its strides allow one, else a copy."""
+    t = t.reshape(-1, width)
+    if t.shape[0] == 0 or (t.shape[0] == 1 and (width == 1 or t.stride(1) == 1)):
+        return t, width
+    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _index(t, what, device):
+    """(contiguous tensor, 1 if int64) of an index argument."""
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
+        raise TypeError(f"{what}: expected int32 or int64, got {t.dtype}")
+    return _c(_same_device(t, what, device)), int(t.dtype == torch.int64)
+
+
+def _records(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _token_embedding_fwd(weight, tokens, i64, scale):
+    C, w = weight.shape
+    table, ldw = _rows(weight, w)
+    out = torch.empty(tokens.shape + (w,), dtype=weight.dtype, device=weight.device)
+    L.launch("gm_token_embedding_fwd", weight.device, tokens.numel(), C, w, tokens.data_ptr(), i64, table.data_ptr(), ldw,
+             L.DTYPES[weight.dtype], scale, out.data_ptr(), w)
+    return out
+
+
+class _TokenEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, i64, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.args = (weight.shape, i64, scale, padding)
+        return _token_embedding_fwd(weight, tokens, i64, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (tokens,) = ctx.saved_tensors
+        (C, w), i64, scale, padding = ctx.args
+        n, dev = tokens.numel(), g.device
+        g2, ldg = _rows(g, w)
+        dW = torch.empty((C, w), dtype=g.dtype, device=dev)
+        need = L.load().gm_token_embedding_bwd_workspace_bytes(n, C, w)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        L.launch("gm_token_embedding_bwd", dev, n, C, w, tokens.data_ptr(), i64, padding, g2.data_ptr(), ldg, L.DTYPES[g.dtype], scale,
+                 dW.data_ptr(), w, ws.data_ptr(), need)
+        return dW, None, None, None, None
+
+
+def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
+    """scale * weight[tokens], shape tokens.shape + (w,), in weight's type (float32, bfloat16, float16).  tokens: int32 or int64
+    of any shape.  The gradient sums each row's tokens in ascending position (no atomics: the same bits on every run) and
+    leaves row padding_idx zero, as nn.Embedding does.  Tokens are not read on the host: one outside [0, C) gives a row of
+    NaN and adds to no gradient; ops.check_index_range(tokens, C, "tokens") is the check that raises."""
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"token_embedding: weight must be (C, w) with C, w > 0, got {tuple(weight.shape)}")
+    _row_dtype(weight, "weight")
+    tokens, i64 = _index(tokens, "tokens", weight.device)
+    C = weight.shape[0]
+    if padding_idx is None:
+        padding = -1
+    else:
+        if not -C <= padding_idx < C:
+            raise ValueError(f"token_embedding: padding_idx {padding_idx} is outside the {C} rows of weight")
+        padding = int(padding_idx) % C
+    _on_gpu(weight, "weight")
+    if _records(weight):
+        return _TokenEmbedding.apply(weight, tokens, i64, float(scale), padding)
+    return _token_embedding_fwd(weight, tokens, i64, float(scale))
+
+
+def _layer_norm_fwd(x, gamma, beta, eps, stats):
+    N, dev = x.shape[-1], x.device
+    x2, ldx = _rows(x, N)
+    M = x2.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    st = torch.empty((2, M), dtype=torch.float32, device=dev) if stats else None
+    at = st.data_ptr() if stats else None
+    wt = gamma if gamma is not None else beta
+    L.launch("gm_layer_norm_fwd", dev, M, N, x2.data_ptr(), ldx, L.DTYPES[x.dtype], gamma.data_ptr() if gamma is not None else None,
+             beta.data_ptr() if beta is not None else None, L.DTYPES[wt.dtype] if wt is not None else 0, eps, y.data_ptr(), N, at,
+             at + 4 * M if stats and M else None)
+    return y, x2, st
+
+
+def _layer_norm_bwd(g, x2, mean, rstd, gamma, dx, dgamma, dbeta):
+    """gm_layer_norm_bwd over rows x2 (M, N); dx, dgamma, dbeta: outputs or None."""
+    M, N = x2.shape
+    x2, ldx = _rows(x2, N)
+    g2, ldg = _rows(g, N)
+    wt = next((t for t in (gamma, dgamma, dbeta) if t is not None), None)
+    need = L.load().gm_layer_norm_bwd_workspace_bytes(M, N) if dgamma is not None or dbeta is not None else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
+
+    def at(t):
+        return t.data_ptr() if t is not None else None
+
+    L.launch("gm_layer_norm_bwd", x2.device, M, N, g2.data_ptr(), ldg, x2.data_ptr(), ldx, L.DTYPES[x2.dtype], at(mean), at(rstd), at(gamma),
+             L.DTYPES[wt.dtype] if wt is not None else 0, at(dx), N, at(dgamma), at(dbeta), at(ws), need)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps):
+        y, x2, st = _layer_norm_fwd(x, gamma, beta, eps, True)
+        ctx.save_for_backward(x2, st, gamma)
+        ctx.shape, ctx.beta_dtype = x.shape, beta.dtype if beta is not None else None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x2, st, gamma = ctx.saved_tensors
+        N, dev, need = x2.shape[1], x2.device, ctx.needs_input_grad
+        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need[0] else None
+        dgamma = torch.empty(N, dtype=gamma.dtype, device=dev) if need[1] else None
+        dbeta = torch.empty(N, dtype=ctx.beta_dtype, device=dev) if need[2] else None
+        _layer_norm_bwd(g, x2, st[0], st[1], gamma, dx, dgamma, dbeta)
+        return dx, dgamma, dbeta, None
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension, of any width, in x's type (float32, bfloat16,
+    float16).  gamma and beta (N,): x's type or float32, both the same; None: 1 and 0.  Statistics are float32 about the mean,
+    the variance that of the differences from it."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm: x must have a last dimension of at least 1, got {tuple(x.shape)}")
+    _row_dtype(x, "x")
+    for t, what in ((gamma, "gamma"), (beta, "beta")):
+        if t is None:
+            continue
+        if t.shape != x.shape[-1:]:
+            raise ValueError(f"layer_norm: {what} is {tuple(t.shape)}, x's rows have {x.shape[-1]} columns")
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise TypeError(f"layer_norm: {what} is {t.dtype}, expected {x.dtype} or float32")
+        _same_device(t, what, x.device)
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise TypeError(f"layer_norm: gamma is {gamma.dtype} and beta is {beta.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
+    _on_gpu(x, "x")
+    gamma, beta = (t if t is None else _c(t) for t in (gamma, beta))
+    if _records(x, gamma, beta):
+        return _LayerNorm.apply(x, gamma, beta, float(eps))
+    return _layer_norm_fwd(x, gamma, beta, float(eps), False)[0]
+
+
+def _class_log_prob_fwd(logits, classes, i64, ignore_index, stats):
+    V, dev = logits.shape[-1], logits.device
+    x2, ldx = _rows(logits, V)
+    M = x2.shape[0]
+    lp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    st = torch.empty((M, 2), dtype=torch.float32, device=dev) if stats else None
+    need = L.load().gm_class_log_prob_workspace_bytes(M, V)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    L.launch("gm_class_log_prob_fwd", dev, M, V, x2.data_ptr(), ldx, L.DTYPES[logits.dtype], classes.data_ptr(), i64, ignore_index,
+             lp.data_ptr(), st.data_ptr() if stats else None, ws.data_ptr() if need else None, need)
+    return lp, x2, st
+
+
+class _ClassLogProb(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, classes, i64, ignore_index):
+        lp, x2, st = _class_log_prob_fwd(logits, classes, i64, ignore_index, True)
+        ctx.save_for_backward(x2, classes, st)
+        ctx.args = (logits.shape, i64, ignore_index)
+        return lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x2, classes, st = ctx.saved_tensors
+        shape, i64, ignore_index = ctx.args
+        M, V = x2.shape
+        x2, ldx = _rows(x2, V)
+        g = _c(g)
+        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device)
+        L.launch("gm_class_log_prob_bwd", x2.device, M, V, g.data_ptr(), x2.data_ptr(), ldx, L.DTYPES[x2.dtype], classes.data_ptr(), i64,
+                 ignore_index, st.data_ptr(), dx.data_ptr(), V)
+        return dx, None, None, None
+
+
+def class_log_prob(logits, classes, ignore_index=-100):
+    """log softmax(logits)[classes] over the last dimension: float32 of shape classes.shape = logits.shape[:-1]; logits float32,
+    bfloat16 or float16, classes int32 or int64.  A row whose class is ignore_index has log-probability 0 and a zero gradient,
+    whatever its logits hold; any other class outside [0, V) gives NaN in both (classes are not read on the host).  A row
+    whose upstream gradient is exactly 0 gets a zero gradient too."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"class_log_prob: logits must have a last dimension of at least 1, got {tuple(logits.shape)}")
+    if classes.shape != logits.shape[:-1]:
+        raise ValueError(f"class_log_prob: classes is {tuple(classes.shape)}, logits is {tuple(logits.shape)}")
+    _row_dtype(logits, "logits")
+    classes, i64 = _index(classes, "classes", logits.device)
+    _on_gpu(logits, "logits")
+    if _records(logits):
+        return _ClassLogProb.apply(logits, classes, i64, int(ignore_index))
+    return _class_log_prob_fwd(logits, classes, i64, int(ignore_index), False)[0]
+
+
+def _items(t, what, like=None):
+    """A float32 per-item argument; with `like`, one of its shape and device that takes no gradient."""
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: expected float32, got {t.dtype}")
+    if like is not None:
+        if t.shape != like.shape:
+            raise ValueError(f"{what} is {tuple(t.shape)}, log_prob is {tuple(like.shape)}")
+        _constant(t, what)
+        _same_device(t, what, like.device)
+    return _c(t)
+
+
+def _constant(t, what):
+    if t.requires_grad:
+        raise ValueError(f"{what} is a constant of the loss and gets no gradient: pass {what}.detach()")
+
+
+def _mask(mask, like):
+    if mask is None:
+        return None
+    if mask.dtype != torch.bool and mask.dtype != torch.uint8:
+        raise TypeError(f"mask: expected bool or uint8, got {mask.dtype}")
+    if mask.shape != like.shape:
+        raise ValueError(f"mask is {tuple(mask.shape)}, log_prob is {tuple(like.shape)}")
+    return _c(_same_device(mask, "mask", like.device))
+
+
+def _offsets(offsets, device):
+    if offsets.dim() != 1 or offsets.numel() < 2:
+        raise ValueError(f"offsets: expected the S + 1 borders of S > 0 sequences, got {tuple(offsets.shape)}")
+    return _index(offsets, "offsets", device)
+
+
+def _sequence_loss_bwd(g, slope, mask, offsets, i64, weight, shape):
+    out = torch.empty(shape, dtype=torch.float32, device=g.device)
+    L.launch("gm_sequence_loss_bwd", g.device, out.numel(), weight.numel(), slope.data_ptr() if slope is not None else None,
+             mask.data_ptr() if mask is not None else None, offsets.data_ptr() if offsets is not None else None, i64, weight.data_ptr(),
+             g.data_ptr(), out.data_ptr())
+    return out
+
+
+def _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, clip_low, clip_high, kl_coef, by_sequence, grad):
+    dev, M = lp.device, lp.numel()
+    S = offsets.numel() - 1 if offsets is not None else 1
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty(4, dtype=torch.float32, device=dev)
+    slope = torch.empty(M, dtype=torch.float32, device=dev) if grad else None
+    weight = torch.empty(S, dtype=torch.float32, device=dev) if grad else None
+    need = L.load().gm_sequence_loss_workspace_bytes(M, S)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+
+    def at(t):
+        return t.data_ptr() if t is not None else None
+
+    L.launch("gm_policy_loss_fwd", dev, M, S, at(lp), at(old), at(adv), at(ref), at(mask), at(offsets), i64, clip_low, clip_high, kl_coef,
+             by_sequence, loss.data_ptr(), stats.data_ptr(), at(slope), at(weight), ws.data_ptr(), need)
+    return loss, stats, slope, weight
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lp, old, adv, ref, mask, offsets, i64, *args):
+        loss, stats, slope, weight = _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, *args, True)
+        ctx.save_for_backward(slope, mask, offsets, weight)
+        ctx.args = (i64, lp.shape)
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _stats):
+        slope, mask, offsets, weight = ctx.saved_tensors
+        i64, shape = ctx.args
+        return (_sequence_loss_bwd(g, slope, mask, offsets, i64, weight, shape),) + (None,) * 10
+
+
+def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, ref_log_prob=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, reduction="token"):
+    """Clipped policy loss of the items' log-probabilities (float32, any shape; see class_log_prob) against those under the
+    model that drew them:  r = exp(log_prob - old_log_prob),  -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+    + kl_coef * (exp(q) - q - 1),  q = ref_log_prob - log_prob.
+
+    offsets: S + 1 non-decreasing borders (int32 / int64) of consecutive sequences of items; `advantage` then has one value a
+    sequence, without offsets one an item.  mask: bool / uint8.  An item outside every sequence or masked off counts nowhere,
+    whatever its values, and gets a zero gradient.  reduction: "token" averages over the live items, "sequence" over each
+    sequence's and then over the sequences that have one; without any live item the loss is 0.  old_log_prob, advantage and
+    ref_log_prob are constants.
+
+    Returns (loss, stats), stats = [mean surrogate, mean KL, share of clipped items, live items] without a gradient."""
+    lp = _items(log_prob, "log_prob")
+    old = _items(old_log_prob, "old_log_prob", log_prob)
+    ref = _items(ref_log_prob, "ref_log_prob", log_prob) if ref_log_prob is not None else None
+    mask = _mask(mask, log_prob)
+    i64 = 0
+    if offsets is None:
+        adv = _items(advantage, "advantage", log_prob)
+    else:
+        offsets, i64 = _offsets(offsets, log_prob.device)
+        adv = _items(advantage, "advantage")
+        _same_device(adv, "advantage", log_prob.device)
+        _constant(advantage, "advantage")
+        if advantage.shape != (offsets.numel() - 1,):
+            raise ValueError(f"advantage is {tuple(advantage.shape)}, offsets border {offsets.numel() - 1} sequences")
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction: expected 'token' or 'sequence', got {reduction!r}")
+    if reduction == "sequence" and offsets is None:
+        raise ValueError("reduction 'sequence' needs offsets")
+    if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
+        raise ValueError(f"clip range: 0 <= clip_low <= 1 and 0 <= clip_high, got {clip_low}, {clip_high}")
+    if kl_coef != 0.0 and ref is None:
+        raise ValueError("kl_coef needs ref_log_prob")
+    if kl_coef - kl_coef != 0.0:
+        raise ValueError(f"kl_coef must be finite, got {kl_coef}")
+    _on_gpu(log_prob, "log_prob")
+    args = (float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
+    if _records(log_prob):
+        return _PolicyLoss.apply(lp, old, adv, ref, mask, offsets, i64, *args)
+    return _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, *args, False)[:2]
+
+
+def _preference_loss_fwd(lp, ref, mask, offsets, i64, beta, smoothing, average, grad):
+    dev, M, S = lp.device, lp.numel(), offsets.numel() - 1
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    rewards = torch.empty(S, dtype=torch.float32, device=dev)
+    weight = torch.empty(S, dtype=torch.float32, device=dev) if grad else None
+    need = L.load().gm_sequence_loss_workspace_bytes(M, S)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    L.launch("gm_preference_loss_fwd", dev, M, S // 2, lp.data_ptr(), ref.data_ptr(), mask.data_ptr() if mask is not None else None,
+             offsets.data_ptr(), i64, beta, smoothing, average, loss.data_ptr(), rewards.data_ptr(),
+             weight.data_ptr() if grad else None, ws.data_ptr(), need)
+    return loss, rewards, weight
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lp, ref, mask, offsets, i64, *args):
+        loss, rewards, weight = _preference_loss_fwd(lp, ref, mask, offsets, i64, *args, True)
+        ctx.save_for_backward(mask, offsets, weight)
+        ctx.args = (i64, lp.shape)
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _rewards):
+        mask, offsets, weight = ctx.saved_tensors
+        i64, shape = ctx.args
+        return (_sequence_loss_bwd(g, None, mask, offsets, i64, weight, shape),) + (None,) * 7
+
+
+def preference_loss(log_prob, ref_log_prob, offsets, *, mask=None, beta=0.1, label_smoothing=0.0, average=False):
+    """Loss of P pairs of sequences from the items' log-probabilities under the trained and a reference model (float32):
+    sequence 2p of the 2P that the 2P + 1 `offsets` border is preferred over sequence 2p + 1.  h = sum (average=True: mean) over
+    a sequence's live items of log_prob - ref_log_prob,  z = beta (h_2p - h_2p+1),
+    mean over pairs of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z).
+
+    mask, items outside every sequence: as in policy_loss.  A sequence without a live item has h = 0.
+    Returns (loss, rewards), rewards = beta h of the 2P sequences, without a gradient."""
+    lp = _items(log_prob, "log_prob")
+    ref = _items(ref_log_prob, "ref_log_prob", log_prob)
+    mask = _mask(mask, log_prob)
+    offsets, i64 = _offsets(offsets, log_prob.device)
+    if offsets.numel() % 2 == 0:
+        raise ValueError(f"offsets border {offsets.numel() - 1} sequences: an even number makes pairs")
+    if not 0.0 < beta < float("inf") or not 0.0 <= label_smoothing <= 0.5:
+        raise ValueError(f"0 < beta and 0 <= label_smoothing <= 0.5, got {beta}, {label_smoothing}")
+    _on_gpu(log_prob, "log_prob")
+    args = (float(beta), float(label_smoothing), int(bool(average)))
+    if _records(log_prob):
+        return _PreferenceLoss.apply(lp, ref, mask, offsets, i64, *args)
+    return _preference_loss_fwd(lp, ref, mask, offsets, i64, *args, False)[:2]

@@ -1,0 +1,362 @@
+// gm_policy.hip -- losses over the log-probabilities of a batch of ragged sequences (answers, or the draws of generated
+// graphs): the clipped policy loss with a KL term, and the preference loss of pairs.  Item i has log-probability l under
+// the trained model, `old` under the one that drew it and `ref` under a fixed reference; a sequence is a run of items
+// [offsets[s], offsets[s+1]).  An item is live if it is inside a sequence and its mask byte is set; the values of the
+// others are never used.
+//
+//   policy       r = exp(l - old),  t = -min(r A, clip(r, 1 - low, 1 + high) A) + k (exp(q) - q - 1),  q = ref - l
+//                loss = mean of t over the live items, or mean over sequences of each one's mean
+//                dt/dl = (0 where the clipped product is the smaller one, else -r A) + k (1 - exp(q))
+//   preference   h_s = sum (or mean) over the live items of l - ref,  z = beta (h_2p - h_2p+1)
+//                loss = mean over pairs of -(1 - e) log sig(z) - e log sig(-z),  dloss/dz = (sig(z) - (1 - e)) / P
+//
+// Both make one pass over the items and reduce per sequence: a workgroup takes `chunk` consecutive items, whatever the
+// sequences' lengths, and sums each sequence's piece in float64 (the losses are small differences of long sums).  A
+// sequence inside one chunk has its sum at once; one that crosses chunks has a piece per chunk, added in ascending order.
+// The order of every sum depends on (M, offsets) alone.  Offsets that decrease or leave [0, M] read and write no memory
+// out of range; the results are then unspecified.
+#include "gm_rows.h"
+
+namespace gm {
+
+constexpr int SEQ_FUSED = 64;        // sequences up to which one workgroup both gathers the pieces and forms the loss
+
+struct Sequences {
+    IndexArray offsets;              // p == NULL: all items are one sequence
+    int64_t S, M;
+    __device__ __forceinline__ int64_t lo(int64_t s) const {
+        if (!offsets.p) return 0;
+        const int64_t v = offsets.at(s);
+        return v < 0 ? 0 : v > M ? M : v;
+    }
+    __device__ __forceinline__ int64_t hi(int64_t s) const {
+        if (!offsets.p) return M;
+        const int64_t v = offsets.at(s + 1);
+        return v < 0 ? 0 : v > M ? M : v;
+    }
+    // the last sequence of [first, last] that starts at or before item i (first if none does)
+    __device__ __forceinline__ int64_t of(int64_t i, int64_t first, int64_t last) const {
+        if (!offsets.p) return 0;
+        while (first < last) {
+            const int64_t mid = (first + last + 1) >> 1;
+            if (offsets.at(mid) <= i) first = mid;
+            else last = mid - 1;
+        }
+        return first;
+    }
+};
+
+static inline int64_t chunk_items(int64_t M) { return M <= 2048 * 1024 ? 1024 : ((M + 2047) / 2048 + 1023) / 1024 * 1024; }
+
+template <int Q> struct alignas(8) Sums { double v[Q]; };
+
+// exp(x) - 1 - x: the series where the difference would cancel (its first left-out term is below 2^-24 of the sum)
+__device__ __forceinline__ float exp_minus_1_x(float x) {
+    if (!(__builtin_fabsf(x) < 1.0f)) return expf(x) - 1.0f - x;
+    float p = 2.75573192e-7f;                           // 1/10!
+    p = __builtin_fmaf(p, x, 2.75573192e-6f);
+    p = __builtin_fmaf(p, x, 2.48015873e-5f);
+    p = __builtin_fmaf(p, x, 1.98412698e-4f);
+    p = __builtin_fmaf(p, x, 1.38888889e-3f);
+    p = __builtin_fmaf(p, x, 8.33333333e-3f);
+    p = __builtin_fmaf(p, x, 4.16666667e-2f);
+    p = __builtin_fmaf(p, x, 1.66666667e-1f);
+    p = __builtin_fmaf(p, x, 0.5f);
+    return p * x * x;
+}
+
+struct PolicyTerm {                                      // sums: surrogate, KL, clipped items, live items
+    static constexpr int Q = 4;
+    const float *lp, *old, *adv, *ref;
+    const uint8_t* mask;
+    float low, high, kl;                                 // 1 - clip_low, 1 + clip_high, KL coefficient
+    int adv_per_sequence;
+    float* slope;
+    __device__ __forceinline__ void add(int64_t i, int64_t s, Sums<4>& a) const {
+        float d = 0.0f;
+        if (!mask || mask[i]) {
+            const float l = lp[i], A = adv[adv_per_sequence ? s : i];
+            const float r = expf(l - old[i]);
+            const bool cut = (A > 0.0f && r > high) || (A < 0.0f && r < low);
+            const float gain = A == 0.0f ? 0.0f : (cut ? (A > 0.0f ? high : low) : r) * A;
+            a.v[0] -= (double)gain;
+            a.v[2] += cut ? 1.0 : 0.0;
+            a.v[3] += 1.0;
+            d = cut ? 0.0f : -gain;
+            if (ref) {
+                const float q = ref[i] - l, k = exp_minus_1_x(q);
+                a.v[1] += (double)k;
+                if (kl != 0.0f) d = d - kl * (q + k);
+            }
+        }
+        if (slope) slope[i] = d;
+    }
+};
+
+struct PreferenceTerm {                                  // sums: log ratio, live items
+    static constexpr int Q = 2;
+    const float *lp, *ref;
+    const uint8_t* mask;
+    __device__ __forceinline__ void add(int64_t i, int64_t, Sums<2>& a) const {
+        if (!mask || mask[i]) {
+            a.v[0] += (double)lp[i] - (double)ref[i];
+            a.v[1] += 1.0;
+        }
+    }
+};
+
+// pieces of the sequences: `whole`[s] of one inside this chunk; `piece`[2k] of one that began before chunk k,
+// `piece`[2k+1] of one that begins in it and goes on
+template <class F>
+__global__ void __launch_bounds__(256)
+k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whole, Sums<F::Q>* __restrict__ piece) {
+    constexpr int Q = F::Q;
+    __shared__ Sums<Q> red[4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int64_t a = (int64_t)blockIdx.x * chunk, b = a + chunk < q.M ? a + chunk : q.M;
+    const int64_t s0 = q.of(a, 0, q.S - 1), s1 = q.of(b - 1, s0, q.S - 1);
+    const bool alone = s0 == s1;                         // one sequence: all four waves sum it together
+    for (int64_t s = s0 + (alone ? 0 : wv); s <= s1; s += 4) {
+        const int64_t lo = q.lo(s), hi = q.hi(s);
+        const int64_t i0 = lo > a ? lo : a, i1 = hi < b ? hi : b;
+        if (i0 >= i1) continue;                          // uniform over the workgroup if `alone`, over the wave if not
+        Sums<Q> acc = {};
+        const int64_t step = alone ? 256 : 64;
+#pragma unroll 4
+        for (int64_t i = i0 + (alone ? (int)threadIdx.x : lane); i < i1; i += step) f.add(i, s, acc);
+#pragma unroll
+        for (int c = 0; c < Q; ++c) acc.v[c] = wave_add(acc.v[c]);
+        if (alone) {
+            if (lane == 0) red[wv] = acc;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < Q; ++c) acc.v[c] = ((red[0].v[c] + red[1].v[c]) + red[2].v[c]) + red[3].v[c];
+        }
+        if (lane == 0 && (wv == 0 || !alone)) {
+            Sums<Q>* to = lo >= a && hi <= b ? whole + s : piece + 2 * (int64_t)blockIdx.x + (lo < a ? 0 : 1);
+            *to = acc;
+        }
+    }
+}
+
+// whole[s] of every sequence, by one wave
+template <int Q>
+__device__ __forceinline__ void gather_sequence(const Sequences& q, int64_t chunk, int64_t s, int lane, Sums<Q>* __restrict__ whole,
+                                                const Sums<Q>* __restrict__ piece) {
+    const int64_t lo = q.lo(s), hi = q.hi(s);
+    Sums<Q> acc = {};
+    if (lo < hi) {
+        const int64_t k0 = lo / chunk, k1 = (hi - 1) / chunk;
+        if (k0 == k1) return;
+        for (int64_t k = k0 + lane; k <= k1; k += 64)
+#pragma unroll
+            for (int c = 0; c < Q; ++c) acc.v[c] += piece[2 * k + (k == k0 ? 1 : 0)].v[c];
+#pragma unroll
+        for (int c = 0; c < Q; ++c) acc.v[c] = wave_add(acc.v[c]);
+    }
+    if (lane == 0) whole[s] = acc;
+}
+template <int Q>
+__global__ void __launch_bounds__(256)
+k_sequence_gather(Sequences q, int64_t chunk, Sums<Q>* __restrict__ whole, const Sums<Q>* __restrict__ piece) {
+    const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (s < q.S) gather_sequence<Q>(q, chunk, s, threadIdx.x & 63, whole, piece);
+}
+
+// sum over a workgroup of 1024 threads, in every thread
+__device__ __forceinline__ double block_add(double v, double* red) {
+    v = wave_add(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t = t + red[k];
+    return t;
+}
+
+__global__ void __launch_bounds__(1024)
+k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, Sums<4>* __restrict__ whole,
+                const Sums<4>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ weight) {
+    __shared__ double red[16];
+    if (gather) {
+        for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<4>(q, chunk, s, threadIdx.x & 63, whole, piece);
+        __syncthreads();
+    }
+    double tot[4] = {0.0, 0.0, 0.0, 0.0}, used = 0.0;
+    for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
+        const Sums<4> w = whole[s];
+        if (w.v[3] <= 0.0) continue;
+        const double unit = by_sequence ? 1.0 / w.v[3] : 1.0;
+        used += 1.0;
+#pragma unroll
+        for (int c = 0; c < 3; ++c) tot[c] += w.v[c] * unit;
+        tot[3] += w.v[3];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tot[c] = block_add(tot[c], red);
+    used = block_add(used, red);
+    const double over = by_sequence ? used : tot[3];
+    const double norm = over > 0.0 ? 1.0 / over : 0.0;    // no live item: the loss and every gradient are 0
+    for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
+        const double n = whole[s].v[3];
+        if (weight) weight[s] = n > 0.0 ? (float)(by_sequence ? norm / n : norm) : 0.0f;
+    }
+    if (threadIdx.x == 0) {
+        const double surrogate = tot[0] * norm, apart = tot[1] * norm;
+        loss[0] = (float)(kl != 0.0f ? surrogate + (double)kl * apart : surrogate);
+        stats[0] = (float)surrogate;
+        stats[1] = (float)apart;
+        stats[2] = (float)(tot[2] * norm);
+        stats[3] = (float)tot[3];
+    }
+}
+
+__global__ void __launch_bounds__(1024)
+k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double smoothing, int average, Sums<2>* __restrict__ whole,
+                    const Sums<2>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ weight) {
+    __shared__ double red[16];
+    if (gather) {
+        for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<2>(q, chunk, s, threadIdx.x & 63, whole, piece);
+        __syncthreads();
+    }
+    const int64_t P = q.S / 2;
+    double tot = 0.0;
+    for (int64_t p = threadIdx.x; p < P; p += 1024) {
+        double h[2], unit[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const Sums<2> w = whole[2 * p + k];
+            unit[k] = average && w.v[1] > 1.0 ? 1.0 / w.v[1] : 1.0;
+            h[k] = w.v[0] * unit[k];
+            rewards[2 * p + k] = (float)(beta * h[k]);
+        }
+        const double z = beta * (h[0] - h[1]), e = exp(-fabs(z));
+        const double up = (z < 0.0 ? -z : 0.0) + log1p(e);              // -log sig(z); z NaN: e is
+        tot += smoothing != 0.0 ? (1.0 - smoothing) * up + smoothing * (up + z) : up;
+        const double dz = (smoothing - (z >= 0.0 ? e : 1.0) / (1.0 + e)) / (double)P;    // sig(z) - 1 = -sig(-z)
+        if (weight) {
+            weight[2 * p] = (float)(beta * dz * unit[0]);
+            weight[2 * p + 1] = (float)(-beta * dz * unit[1]);
+        }
+    }
+    tot = block_add(tot, red);
+    if (threadIdx.x == 0) loss[0] = (float)(tot / (double)P);
+}
+
+// dl[i] = g weight[s] slope[i] for the live items of sequence s, 0 for every other item
+__global__ void __launch_bounds__(256)
+k_sequence_spread(Sequences q, int64_t chunk, const float* __restrict__ slope, const uint8_t* __restrict__ mask,
+                  const float* __restrict__ weight, const float* __restrict__ g, float* __restrict__ dl) {
+    const int64_t a = (int64_t)blockIdx.x * chunk, b = a + chunk < q.M ? a + chunk : q.M;
+    const int64_t s0 = q.of(a, 0, q.S - 1), s1 = q.of(b - 1, s0, q.S - 1);
+    const float up = g[0];
+    for (int64_t i = a + threadIdx.x; i < b; i += 256) {
+        const int64_t s = q.of(i, s0, s1);
+        const bool live = i >= q.lo(s) && i < q.hi(s) && (!mask || mask[i]);
+        float v = 0.0f;
+        if (live) {
+            v = weight[s] * up;
+            if (slope) v = v * slope[i];
+        }
+        dl[i] = v;
+    }
+}
+
+struct SequenceLayout { int64_t nchunk, whole, piece, bytes; };
+static inline SequenceLayout sequence_layout(int64_t M, int64_t S) {
+    SequenceLayout l;
+    const int64_t chunk = chunk_items(M);
+    l.nchunk = (M + chunk - 1) / chunk;
+    l.whole = 0;
+    l.piece = S * (int64_t)sizeof(Sums<4>);
+    l.bytes = l.piece + 2 * l.nchunk * (int64_t)sizeof(Sums<4>);
+    return l;
+}
+
+template <class F, class Finish>
+static int launch_sequence_loss(const Sequences& q, const F& f, void* workspace, int64_t workspace_bytes, hipStream_t s,
+                                Finish&& finish) {
+    constexpr int Q = F::Q;
+    const SequenceLayout l = sequence_layout(q.M, q.S);
+    GM_REQUIRE(workspace && workspace_bytes >= l.bytes && aligned(workspace, 16),
+               "needs %lld workspace bytes (gm_sequence_loss_workspace_bytes)", (long long)l.bytes);
+    Sums<Q>* whole = reinterpret_cast<Sums<Q>*>(static_cast<char*>(workspace) + l.whole);
+    Sums<Q>* piece = reinterpret_cast<Sums<Q>*>(static_cast<char*>(workspace) + l.piece);
+    const int64_t chunk = chunk_items(q.M);
+    if (l.nchunk > 0) {
+        hipLaunchKernelGGL((k_sequence_pieces<F>), dim3((unsigned)l.nchunk), dim3(256), 0, s, q, chunk, f, whole, piece);
+        GM_LAUNCH_CHECK();
+    }
+    const int fused = q.S <= SEQ_FUSED;
+    if (!fused) {
+        hipLaunchKernelGGL((k_sequence_gather<Q>), dim3((unsigned)((q.S + 3) / 4)), dim3(256), 0, s, q, chunk, whole, piece);
+        GM_LAUNCH_CHECK();
+    }
+    finish(chunk, fused, whole, piece);
+    GM_LAUNCH_CHECK();
+    return GM_OK;
+}
+
+}  // namespace gm
+
+using namespace gm;
+
+#define GM_SEQUENCE_CHECK()                                                                                               \
+    GM_REQUIRE(M >= 0 && S > 0 && (M == 0 || log_prob), "bad arguments");                                                 \
+    GM_REQUIRE(M < (1ll << 40) && S < (1ll << 31), "M or the number of sequences too large")
+
+extern "C" int64_t gm_sequence_loss_workspace_bytes(int64_t M, int64_t S) {
+    if (M < 0 || S <= 0 || M >= (1ll << 40) || S >= (1ll << 31)) return -1;
+    return sequence_layout(M, S).bytes;
+}
+
+extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, const float* old_log_prob, const float* advantage,
+                                  const float* ref_log_prob, const uint8_t* mask, const void* offsets, int offsets_i64,
+                                  float clip_low, float clip_high, float kl_coef, int by_sequence, float* loss, float* stats,
+                                  float* slope, float* weight, void* workspace, int64_t workspace_bytes, gm_stream_t stream) {
+    GM_SEQUENCE_CHECK();
+    GM_REQUIRE(loss && stats && (M == 0 || (advantage && old_log_prob)) && (offsets || S == 1), "bad arguments");
+    GM_REQUIRE(clip_low >= 0.0f && clip_low <= 1.0f && clip_high >= 0.0f && clip_high < INFINITY, "clip range: 0 <= clip_low <= 1, 0 <= clip_high");
+    GM_REQUIRE(kl_coef == 0.0f || ref_log_prob, "kl_coef without ref_log_prob");
+    GM_REQUIRE(kl_coef - kl_coef == 0.0f, "kl_coef is not finite");
+    hipStream_t s = as_stream(stream);
+    const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
+    const PolicyTerm f{log_prob, old_log_prob, advantage, ref_log_prob, mask, 1.0f - clip_low, 1.0f + clip_high, kl_coef,
+                       offsets != nullptr, slope};
+    return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece) {
+        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, loss, stats, weight);
+    });
+}
+
+extern "C" int gm_preference_loss_fwd(int64_t M, int64_t P, const float* log_prob, const float* ref_log_prob, const uint8_t* mask,
+                                      const void* offsets, int offsets_i64, float beta, float label_smoothing, int average,
+                                      float* loss, float* rewards, float* weight, void* workspace, int64_t workspace_bytes,
+                                      gm_stream_t stream) {
+    GM_REQUIRE(P > 0 && P < (1ll << 30), "no pair, or too many");
+    const int64_t S = 2 * P;
+    GM_SEQUENCE_CHECK();
+    GM_REQUIRE(loss && rewards && offsets && (M == 0 || ref_log_prob), "bad arguments");
+    GM_REQUIRE(beta > 0.0f && beta < INFINITY && label_smoothing >= 0.0f && label_smoothing <= 0.5f,
+               "0 < beta and 0 <= label_smoothing <= 0.5");
+    hipStream_t s = as_stream(stream);
+    const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
+    const PreferenceTerm f{log_prob, ref_log_prob, mask};
+    return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<2>* whole, Sums<2>* piece) {
+        hipLaunchKernelGGL(k_preference_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, (double)beta, (double)label_smoothing, average,
+                           whole, piece, loss, rewards, weight);
+    });
+}
+
+extern "C" int gm_sequence_loss_bwd(int64_t M, int64_t S, const float* slope, const uint8_t* mask, const void* offsets, int offsets_i64,
+                                    const float* weight, const float* g, float* dlog_prob, gm_stream_t stream) {
+    GM_REQUIRE(M >= 0 && S > 0 && M < (1ll << 40) && S < (1ll << 31) && (offsets || S == 1), "bad arguments");
+    if (M == 0) return GM_OK;
+    GM_REQUIRE(weight && g && dlog_prob, "bad arguments");
+    const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
+    const int64_t chunk = chunk_items(M);
+    hipLaunchKernelGGL(k_sequence_spread, dim3((unsigned)((M + chunk - 1) / chunk)), dim3(256), 0, as_stream(stream), q, chunk, slope,
+                       mask, weight, g, dlog_prob);
+    GM_LAUNCH_CHECK();
+    return GM_OK;
+}

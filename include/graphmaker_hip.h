@@ -339,6 +339,63 @@ int gm_denoise_match2(int64_t total, const float* logits, const uint8_t* z_t, co
 int gm_bitmap_lookup(int64_t n, int64_t wpr, const uint32_t* bits, int64_t B, const int64_t* i, const int64_t* j,
                      uint8_t* out, gm_stream_t stream);
 
+/* ---- wider training and fine-tuning operators: typed rows, large vocabularies, losses over sampled draws ----
+ * Not in the reference; each stands beside one that is: gm_embedding_*, gm_layernorm_*, gm_softmax_ce2.
+ * Element types of the rows: */
+enum { GM_DTYPE_F32 = 0, GM_DTYPE_BF16 = 1, GM_DTYPE_F16 = 2 };
+/* All sums are float32 or float64 in a fixed order; a store to a 16-bit type rounds once.  Sizes of 0 rows are allowed.
+ * Rows may be further apart than their width (ld*, in elements).  Index arrays are int32, or int64 where *_i64 is set. */
+
+/* out[i] = scale * weight[tokens[i]]; a token outside [0, C) reads nothing and gives a row of NaN */
+int gm_token_embedding_fwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, const void* weight, int64_t ldw,
+                           int dtype, float scale, void* out, int64_t ldo, gm_stream_t stream);
+/* dW (C, w) = scale * (sum of the rows G[i] with tokens[i] == c, ascending i); zero where there is none, for row padding_idx
+ * (negative: no such row) and from tokens outside [0, C).  The tokens are sorted in the workspace; n, C < 2^31. */
+int64_t gm_token_embedding_bwd_workspace_bytes(int64_t n, int64_t C, int64_t w);
+int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, int64_t padding_idx, const void* G,
+                           int64_t ldg, int dtype, float scale, void* dW, int64_t ldw, void* workspace, int64_t workspace_bytes,
+                           gm_stream_t stream);
+/* y = (x - mean) * rstd * gamma + beta over rows of any width N; gamma / beta may be NULL and have the rows' type or float32
+ * (weight_dtype); mean, rstd (M floats each, both or neither): what the backward needs */
+int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ldx, int dtype, const void* gamma, const void* beta,
+                      int weight_dtype, float eps, void* Y, int64_t ldy, float* mean, float* rstd, gm_stream_t stream);
+/* gradients of the above for dY = G; dX, dgamma, dbeta may each be NULL (workspace needed only for dgamma / dbeta) */
+int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N);
+int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ldg, const void* X, int64_t ldx, int dtype, const float* mean,
+                      const float* rstd, const void* gamma, int weight_dtype, void* dX, int64_t lddx, void* dgamma, void* dbeta,
+                      void* workspace, int64_t workspace_bytes, gm_stream_t stream);
+/* log_prob[i] = logits[i][classes[i]] - logsumexp(logits[i]); 0 where classes[i] == ignore_index (such a row is not read), NaN
+ * for another class outside [0, V).  stats (2 floats a row, may be NULL): what the backward needs. */
+int64_t gm_class_log_prob_workspace_bytes(int64_t M, int64_t V);
+int gm_class_log_prob_fwd(int64_t M, int64_t V, const void* logits, int64_t ldx, int dtype, const void* classes, int classes_i64,
+                          int64_t ignore_index, float* log_prob, float* stats, void* workspace, int64_t workspace_bytes,
+                          gm_stream_t stream);
+/* dlogits[i][j] = g[i] * ([j == classes[i]] - softmax(logits[i])[j]); a zero row where classes[i] == ignore_index or g[i] == 0 */
+int gm_class_log_prob_bwd(int64_t M, int64_t V, const float* g, const void* logits, int64_t ldx, int dtype, const void* classes,
+                          int classes_i64, int64_t ignore_index, const float* stats, void* dlogits, int64_t lddx,
+                          gm_stream_t stream);
+/* Losses over M log-probabilities in S sequences, items [offsets[s], offsets[s+1]) of a non-decreasing array of S + 1; items
+ * outside every sequence or with mask[i] == 0 count nowhere and get a zero gradient.
+ *   policy      r = exp(log_prob - old), q = ref - log_prob:
+ *               -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1), averaged over the live items, or
+ *               (by_sequence) per sequence and then over the sequences that have one.  A = advantage[s], or advantage[i] where
+ *               offsets is NULL (S = 1: all items).  stats (4 floats): mean surrogate, mean KL, clipped share, live items.
+ *               slope (M) and weight (S), may be NULL: what the backward needs.
+ *   preference  sequences 2p (chosen) and 2p + 1 (rejected) of P pairs: h = sum (average: mean) of log_prob - ref,
+ *               z = beta (h_chosen - h_rejected), mean over pairs of -(1 - e) log sigmoid(z) - e log sigmoid(-z),
+ *               e = label_smoothing.  rewards (2P) = beta h; weight (2P), may be NULL. */
+int64_t gm_sequence_loss_workspace_bytes(int64_t M, int64_t S);
+int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, const float* old_log_prob, const float* advantage,
+                       const float* ref_log_prob, const uint8_t* mask, const void* offsets, int offsets_i64, float clip_low,
+                       float clip_high, float kl_coef, int by_sequence, float* loss, float* stats, float* slope, float* weight,
+                       void* workspace, int64_t workspace_bytes, gm_stream_t stream);
+int gm_preference_loss_fwd(int64_t M, int64_t P, const float* log_prob, const float* ref_log_prob, const uint8_t* mask,
+                           const void* offsets, int offsets_i64, float beta, float label_smoothing, int average, float* loss,
+                           float* rewards, float* weight, void* workspace, int64_t workspace_bytes, gm_stream_t stream);
+/* gradient of either loss: dlog_prob[i] = g[0] * weight[s] * slope[i] (slope NULL: 1) for the live items of sequence s, else 0 */
+int gm_sequence_loss_bwd(int64_t M, int64_t S, const float* slope, const uint8_t* mask, const void* offsets, int offsets_i64,
+                         const float* weight, const float* g, float* dlog_prob, gm_stream_t stream);
+
 /* ---- integer statistics of a generated graph (eval_utils.py:19-74, 506-596) on bitmap + CSR; no self loops ----
  * tri2[v] = sum_{u in N(v)} |N(v) & N(u)| = 2 * (triangles through v): get_triangle_count (:19-21) = sum(tri2) / 6,
  * nx.clustering (:585) = tri2[v] / (deg(v) * (deg(v) - 1)) */
