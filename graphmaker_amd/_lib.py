@@ -129,13 +129,19 @@ U32 = C.c_uint32
 F32 = C.c_float
 
 
+_functions = {}
+
+
 def launch(name, device, *args):
     """One call of an entry point in _SIGNATURES on `device`'s current stream, whatever device is current."""
-    fn = getattr(load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         _check(rc, name)

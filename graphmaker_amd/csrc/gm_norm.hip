@@ -10,85 +10,317 @@
 
 namespace gm {
 
-template <class T, class W>
-__global__ void __launch_bounds__(256)
-k_layer_norm_fwd(int64_t M, int64_t N, const T* __restrict__ X, int64_t ldx, const W* __restrict__ gamma, const W* __restrict__ beta,
-                 float eps, T* __restrict__ Y, int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    const int lane = threadIdx.x & 63;
-    const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (m >= M) return;
-    const T* x = X + m * ldx;
-    float s = 0.0f, q = 0.0f;
-    for (int64_t c = lane; c < N; c += 64) s = s + to_f32(x[c]);
-    const float mean = wave_add(s) / (float)N;
-    for (int64_t c = lane; c < N; c += 64) {
-        const float t = to_f32(x[c]) - mean;
-        q = __builtin_fmaf(t, t, q);
+// gamma and beta as the caller has them
+struct Weights {
+    const void *gamma, *beta;
+    int f32;
+    template <class T, int V, bool TAIL> __device__ __forceinline__ void load(const void* p, int col, int N, float absent, float (&x)[V]) const {
+        if (!p) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = absent;
+        } else if (f32 && sizeof(T) != 4) {
+            constexpr int F = V < 4 ? V : 4;
+#pragma unroll
+            for (int i = 0; i < V; i += F) {
+                const Vec<float, F> t = load_vec<float, F, TAIL>(static_cast<const float*>(p), col + i, N);
+#pragma unroll
+                for (int j = 0; j < F; ++j) x[i + j] = t.v[j];
+            }
+        } else {
+            const Vec<T, V> t = load_vec<T, V, TAIL>(static_cast<const T*>(p), col, N);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = to_f32(t.v[i]);
+        }
     }
-    const float rstd = 1.0f / __builtin_sqrtf(wave_add(q) / (float)N + eps);
-    for (int64_t c = lane; c < N; c += 64) {
-        const float t = (to_f32(x[c]) - mean) * rstd;
-        Y[m * ldy + c] = from_f32<T>(__builtin_fmaf(t, gamma ? to_f32(gamma[c]) : 1.0f, beta ? to_f32(beta[c]) : 0.0f));
+    template <class T> __device__ __forceinline__ float at(const void* p, int64_t col, float absent) const {
+        return !p ? absent : f32 ? static_cast<const float*>(p)[col] : to_f32(static_cast<const T*>(p)[col]);
     }
-    if (lane == 0 && mean_out) {
-        mean_out[m] = mean;
-        rstd_out[m] = rstd;
+};
+
+// sum of v over the TPR threads of a row, in each of them.  `red` holds one float a wave and is a fresh one at every call
+// between two barriers of the workgroup.
+template <int TPR> __device__ __forceinline__ float row_add(float v, float* red) {
+    v = wave_add(v);
+    if (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int k = 1; k < TPR / 64; ++k) v = v + red[k];
+    }
+    return v;
+}
+
+// the same of two values behind one barrier
+template <int TPR> __device__ __forceinline__ void row_add(float& a, float& b, float (*red)[16]) {
+    a = wave_add(a);
+    b = wave_add(b);
+    if (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = a; red[1][threadIdx.x >> 6] = b; }
+        __syncthreads();
+        a = red[0][0];
+        b = red[1][0];
+#pragma unroll
+        for (int k = 1; k < TPR / 64; ++k) { a = a + red[0][k]; b = b + red[1][k]; }
     }
 }
 
-// dx, and the column sums of g xh and g over a workgroup's rows: part[workgroup][0][c], part[workgroup][1][c]
-template <class T, class W>
-__global__ void __launch_bounds__(256)
-k_layer_norm_bwd(int64_t M, int64_t N, const T* __restrict__ G, int64_t ldg, const T* __restrict__ X, int64_t ldx,
-                 const float* __restrict__ mean, const float* __restrict__ rstd, const W* __restrict__ gamma, T* __restrict__ dX,
-                 int64_t lddx, float* __restrict__ part) {
-    __shared__ float red[2][4];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    bool first = true;
+// A row stays in registers: TPR threads hold K x 16 bytes each, so HBM sees every element once.  A workgroup walks several
+// rows with gamma and beta in registers too, and loads the next row before it reduces the one it has: what a row waits for
+// is HBM alone.
+template <class T, int V, bool TAIL, int K, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+k_layer_norm_fwd(int64_t M, int N, const T* __restrict__ X, int64_t ldx, Weights w, float eps, T* __restrict__ Y, int64_t ldy,
+                 float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[2][16];
+    const int t = threadIdx.x & (TPR - 1);
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    if (m >= M) return;
+    Vec<T, V> r[K], next[K];
+    float ga[K][V], be[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
+        w.load<T, V, TAIL>(w.beta, (k * TPR + t) * V, N, 0.0f, be[k]);
+    }
+    for (; m < M; m += step) {
+        const int64_t ahead = m + step < M ? m + step : m;
+#pragma unroll
+        for (int k = 0; k < K; ++k) r[k] = next[k];
+#pragma unroll
+        for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s = s + to_f32(r[k].v[i]);
+        const float mean = row_add<TPR>(s, red[0]) / (float)N;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = to_f32(r[k].v[i]) - mean;
+                if ((k * TPR + t) * V + i < N) q = __builtin_fmaf(d, d, q);
+            }
+        const float rstd = 1.0f / __builtin_sqrtf(row_add<TPR>(q, red[1]) / (float)N + eps);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = __builtin_fmaf((to_f32(r[k].v[i]) - mean) * rstd, ga[k][i], be[k][i]);
+            store_vec<T, V, TAIL>(Y + m * ldy, (k * TPR + t) * V, N, y);
+        }
+        if (t == 0 && mean_out) {
+            mean_out[m] = mean;
+            rstd_out[m] = rstd;
+        }
+    }
+}
+
+// dx of a workgroup's rows, and the column sums of g xh and g over them, held in registers until the last row:
+// part[workgroup][0][c], part[workgroup][1][c]
+template <class T, int V, bool TAIL, int K, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+k_layer_norm_bwd(int64_t M, int N, const T* __restrict__ G, int64_t ldg, const T* __restrict__ X, int64_t ldx,
+                 const float* __restrict__ mean, const float* __restrict__ rstd, Weights w, T* __restrict__ dX, int64_t lddx,
+                 float* __restrict__ part) {
+    constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[2][2][16];
+    const int t = threadIdx.x & (TPR - 1);
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    float ga[K][V], dga[K][V], dbe[K][V];
+    Vec<T, V> xr[K], gr[K], xn[K], gn[K];
+    float mu_n = 0.0f, rs_n = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dga[k][i] = dbe[k][i] = 0.0f;
+    if (m < M) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            xn[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
+            gn[k] = load_vec<T, V, TAIL>(G + m * ldg, (k * TPR + t) * V, N);
+        }
+        mu_n = mean[m];
+        rs_n = rstd[m];
+#pragma unroll
+        for (int k = 0; k < K; ++k) w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
+    }
+    for (int turn = 0; m < M; m += step, turn ^= 1) {
+        const int64_t ahead = m + step < M ? m + step : m;
+        const float mu = mu_n, rs = rs_n;
+#pragma unroll
+        for (int k = 0; k < K; ++k) { xr[k] = xn[k]; gr[k] = gn[k]; }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            xn[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
+            gn[k] = load_vec<T, V, TAIL>(G + ahead * ldg, (k * TPR + t) * V, N);           // 0 behind the row: adds to no sum
+        }
+        mu_n = mean[ahead];
+        rs_n = rstd[ahead];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float g = to_f32(gr[k].v[i]), xh = (to_f32(xr[k].v[i]) - mu) * rs, gg = g * ga[k][i];
+                if ((k * TPR + t) * V + i < N) {                    // x is 0 there, xh is not, and may be infinite
+                    dga[k][i] = __builtin_fmaf(g, xh, dga[k][i]);
+                    s2 = __builtin_fmaf(gg, xh, s2);
+                    s1 = s1 + gg;
+                }
+                dbe[k][i] = dbe[k][i] + g;
+            }
+        row_add<TPR>(s1, s2, red[turn]);
+        s1 = s1 / (float)N;
+        s2 = s2 / (float)N;
+        if (dX)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float y[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float xh = (to_f32(xr[k].v[i]) - mu) * rs;
+                    y[i] = rs * ((to_f32(gr[k].v[i]) * ga[k][i] - s1) - xh * s2);
+                }
+                store_vec<T, V, TAIL>(dX + m * lddx, (k * TPR + t) * V, N, y);
+            }
+    }
+    if (!part) return;
+    float* out = part + (int64_t)blockIdx.x * 2 * N;
+    if (ROWS == 1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = (k * TPR + t) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (col + i < N) {
+                    out[col + i] = dga[k][i];
+                    out[N + col + i] = dbe[k][i];
+                }
+        }
+    } else {                                                        // the waves' sums, in order
+        __shared__ float sums[ROWS][TPR * V];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < V; ++i) sums[threadIdx.x / TPR][i * TPR + t] = which ? dbe[k][i] : dga[k][i];
+                __syncthreads();
+                for (int c = threadIdx.x; c < TPR * V; c += 256) {
+                    const int col = k * TPR * V + c;
+                    const int at = (c % V) * TPR + c / V;
+                    float v = sums[0][at];
+#pragma unroll
+                    for (int r = 1; r < ROWS; ++r) v = v + sums[r][at];
+                    if (col < N) out[which * N + col] = v;
+                }
+            }
+    }
+}
+
+// rows too wide for registers: the same, reading the row again for every sum
+template <class T>
+__global__ void __launch_bounds__(1024)
+k_layer_norm_fwd_long(int64_t M, int64_t N, const T* __restrict__ X, int64_t ldx, Weights w, float eps, T* __restrict__ Y, int64_t ldy,
+                      float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    __shared__ float red[2][16];
     for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
+        const T* x = X + m * ldx;
+        float s = 0.0f, q = 0.0f;
+        for (int64_t c = threadIdx.x; c < N; c += 1024) s = s + to_f32(x[c]);
+        const float mean = row_add<1024>(s, red[0]) / (float)N;
+        for (int64_t c = threadIdx.x; c < N; c += 1024) {
+            const float d = to_f32(x[c]) - mean;
+            q = __builtin_fmaf(d, d, q);
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(row_add<1024>(q, red[1]) / (float)N + eps);
+        for (int64_t c = threadIdx.x; c < N; c += 1024)
+            Y[m * ldy + c] = from_f32<T>(__builtin_fmaf((to_f32(x[c]) - mean) * rstd, w.at<T>(w.gamma, c, 1.0f), w.at<T>(w.beta, c, 0.0f)));
+        if (threadIdx.x == 0 && mean_out) {
+            mean_out[m] = mean;
+            rstd_out[m] = rstd;
+        }
+    }
+}
+// column sums go through the workgroup's own `part`, which each thread reads and writes at its own columns
+template <class T>
+__global__ void __launch_bounds__(1024)
+k_layer_norm_bwd_long(int64_t M, int64_t N, const T* __restrict__ G, int64_t ldg, const T* __restrict__ X, int64_t ldx,
+                      const float* __restrict__ mean, const float* __restrict__ rstd, Weights w, T* __restrict__ dX, int64_t lddx,
+                      float* __restrict__ part) {
+    __shared__ float red[2][2][16];
+    bool first = true;
+    int turn = 0;
+    for (int64_t m = blockIdx.x; m < M; m += gridDim.x, turn ^= 1) {
         const float mu = mean[m], rs = rstd[m];
         const T *x = X + m * ldx, *gr = G + m * ldg;
         float s1 = 0.0f, s2 = 0.0f;
-        for (int64_t c = threadIdx.x; c < N; c += 256) {
-            const float g = to_f32(gr[c]), xh = (to_f32(x[c]) - mu) * rs;
+        for (int64_t c = threadIdx.x; c < N; c += 1024) {
+            const float g = to_f32(gr[c]), xh = (to_f32(x[c]) - mu) * rs, gg = g * w.at<T>(w.gamma, c, 1.0f);
             if (part) {
                 float* p = part + (int64_t)blockIdx.x * 2 * N + c;
-                p[0] = (first ? 0.0f : p[0]) + g * xh;
+                p[0] = __builtin_fmaf(g, xh, first ? 0.0f : p[0]);
                 p[N] = (first ? 0.0f : p[N]) + g;
             }
-            const float gg = g * (gamma ? to_f32(gamma[c]) : 1.0f);
             s1 = s1 + gg;
             s2 = __builtin_fmaf(gg, xh, s2);
         }
         first = false;
-        s1 = wave_add(s1);
-        s2 = wave_add(s2);
-        __syncthreads();
-        if (lane == 0) { red[0][wv] = s1; red[1][wv] = s2; }
-        __syncthreads();
-        s1 = (red[0][0] + red[0][1] + red[0][2] + red[0][3]) / (float)N;
-        s2 = (red[1][0] + red[1][1] + red[1][2] + red[1][3]) / (float)N;
+        row_add<1024>(s1, s2, red[turn]);
+        s1 = s1 / (float)N;
+        s2 = s2 / (float)N;
         if (dX)
-            for (int64_t c = threadIdx.x; c < N; c += 256) {
+            for (int64_t c = threadIdx.x; c < N; c += 1024) {
                 const float xh = (to_f32(x[c]) - mu) * rs;
-                const float gg = to_f32(gr[c]) * (gamma ? to_f32(gamma[c]) : 1.0f);
-                dX[m * lddx + c] = from_f32<T>(rs * ((gg - s1) - xh * s2));
+                dX[m * lddx + c] = from_f32<T>(rs * ((to_f32(gr[c]) * w.at<T>(w.gamma, c, 1.0f) - s1) - xh * s2));
             }
     }
 }
 
-// dgamma[c], dbeta[c]: the workgroups' sums in ascending order
+// dgamma[c], dbeta[c]: 16 lanes of rows each add every 16th workgroup's sums, then the lanes are added in order
 template <class W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 k_layer_norm_cols(int64_t nblk, int64_t N, const float* __restrict__ part, W* __restrict__ dgamma, W* __restrict__ dbeta) {
-    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (g >= 2 * N) return;
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int64_t g = (int64_t)blockIdx.x * 64 + lane;
     float acc = 0.0f;
-    for (int64_t b = 0; b < nblk; ++b) acc = acc + part[b * 2 * N + g];
+    if (g < 2 * N)
+#pragma unroll 8
+        for (int64_t b = wv; b < nblk; b += 16) acc = acc + part[b * 2 * N + g];
+    red[wv][lane] = acc;
+    __syncthreads();
+    if (wv != 0 || g >= 2 * N) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) acc = acc + red[k][lane];
     W* out = g < N ? dgamma : dbeta;
     if (out) out[g < N ? g : g - N] = from_f32<W>(acc);
 }
 
+// Threads a row and 16-byte pieces a thread.  A wave a row while four pieces hold it (no barrier, four rows a workgroup); a
+// workgroup where they do not, or where the rows are fewer than the waves the chip wants.  tpr = 0: too wide.
+struct RowShape { int tpr, K; };
+static inline RowShape row_shape(int64_t M, int64_t N, int vec, int most) {
+    const int64_t v = (N + vec - 1) / vec;
+    const int tpr = v <= 64 || (v <= 256 && M >= 1024) ? 64 : v <= 1024 ? 256 : 1024;
+    int K = 1;
+    while ((int64_t)K * tpr < v) K *= 2;
+    return K > most ? RowShape{0, 0} : RowShape{tpr, K};
+}
+// workgroups of the forward: what the CUs hold at once
+static inline int64_t norm_blocks_fwd(int64_t M, int rows, int threads) {
+    const int64_t want = (M + rows - 1) / rows, most = 256 * (1024 / threads);
+    return want < most ? want : most;
+}
+// workgroups of the backward: two on every CU, each with as many rows as it takes
 static inline int64_t norm_blocks(int64_t M) { return M < 512 ? M : 512; }
 
 template <class Fn> static inline int with_weight_dtype(int dtype, int weight_dtype, Fn&& fn) {
@@ -106,26 +338,48 @@ using namespace gm;
     GM_REQUIRE(M >= 0 && N > 0, "bad arguments");                                                                         \
     GM_REQUIRE(dtype_ok(dtype) && (weight_dtype == dtype || weight_dtype == GM_DTYPE_F32),                                \
                "dtype %d with weight_dtype %d: the weights have the rows' type or are float32", dtype, weight_dtype);     \
-    GM_REQUIRE(M < (1ll << 31) && N < (1ll << 31), "M or N of 2^31 or more")
+    GM_REQUIRE(M < (1ll << 31) && N < (1ll << 30), "M of 2^31 or more, or N of 2^30 or more")
 
 extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ldx, int dtype, const void* gamma, const void* beta,
                                  int weight_dtype, float eps, void* Y, int64_t ldy, float* mean, float* rstd, gm_stream_t stream) {
     GM_NORM_CHECK();
     if (M == 0) return GM_OK;
     GM_REQUIRE(X && Y && ldx >= N && ldy >= N && !mean == !rstd, "bad arguments");
-    return with_weight_dtype(dtype, weight_dtype, [&](auto t, auto u) -> int {
+    const Weights w{gamma, beta, weight_dtype == GM_DTYPE_F32};
+    return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        using W = decltype(u);
-        hipLaunchKernelGGL((k_layer_norm_fwd<T, W>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, as_stream(stream), M, N,
-                           static_cast<const T*>(X), ldx, static_cast<const W*>(gamma), static_cast<const W*>(beta), eps,
-                           static_cast<T*>(Y), ldy, mean, rstd);
+        const RowShape r = row_shape(M, N, VEC<T>, 8);
+#define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)norm_blocks_fwd(M, ROWS, THREADS)), dim3(THREADS), 0, as_stream(stream), M, N, \
+                       static_cast<const T*>(X), ldx, w, eps, static_cast<T*>(Y), ldy, mean, rstd)
+        with_row_form<T>(N, [&](auto v, auto tail) {
+            constexpr int V = decltype(v)::value;
+            constexpr bool TAIL = decltype(tail)::value;
+            if constexpr (V == 1) {
+                GM_LAUNCH_NORM((k_layer_norm_fwd<T, 1, false, 1, 64>), 4, 256);
+            } else {
+                switch (r.tpr + r.K) {
+                    case 64 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 64>), 4, 256); break;
+                    case 64 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 64>), 4, 256); break;
+                    case 64 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 64>), 4, 256); break;
+                    case 256 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 256>), 1, 256); break;
+                    case 256 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 256>), 1, 256); break;
+                    case 256 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 256>), 1, 256); break;
+                    case 1024 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 1024>), 1, 1024); break;
+                    case 1024 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 1024>), 1, 1024); break;
+                    case 1024 + 8: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 8, 1024>), 1, 1024); break;
+                    default: GM_LAUNCH_NORM((k_layer_norm_fwd_long<T>), 1, 1024); break;
+                }
+            }
+        });
+#undef GM_LAUNCH_NORM
         GM_LAUNCH_CHECK();
         return GM_OK;
     });
 }
 
 extern "C" int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
-    if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 31)) return -1;
+    if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 30)) return -1;
     return norm_blocks(M) * 2 * N * 4;
 }
 
@@ -144,12 +398,35 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
         using T = decltype(t);
         using W = decltype(u);
         if (M > 0) {
-            hipLaunchKernelGGL((k_layer_norm_bwd<T, W>), dim3((unsigned)nblk), dim3(256), 0, s, M, N, static_cast<const T*>(G), ldg,
-                               static_cast<const T*>(X), ldx, mean, rstd, static_cast<const W*>(gamma), static_cast<T*>(dX), lddx, part);
+            const Weights w{gamma, nullptr, weight_dtype == GM_DTYPE_F32};
+            const RowShape r = row_shape(M, N, VEC<T>, 4);
+#define GM_LAUNCH_NORM(KERNEL, THREADS)                                                                                   \
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,            \
+                       static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part)
+            with_row_form<T>(N, [&](auto v, auto tail) {
+                constexpr int V = decltype(v)::value;
+                constexpr bool TAIL = decltype(tail)::value;
+                if constexpr (V == 1) {
+                    GM_LAUNCH_NORM((k_layer_norm_bwd<T, 1, false, 1, 64>), 256);
+                } else {
+                    switch (r.tpr + r.K) {
+                        case 64 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 64>), 256); break;
+                        case 64 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 64>), 256); break;
+                        case 64 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 64>), 256); break;
+                        case 256 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 256>), 256); break;
+                        case 256 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 256>), 256); break;
+                        case 256 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 256>), 256); break;
+                        case 1024 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 1024>), 1024); break;
+                        case 1024 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 1024>), 1024); break;
+                        default: GM_LAUNCH_NORM((k_layer_norm_bwd_long<T>), 1024); break;
+                    }
+                }
+            });
+#undef GM_LAUNCH_NORM
             GM_LAUNCH_CHECK();
         }
         if (cols) {
-            hipLaunchKernelGGL((k_layer_norm_cols<W>), dim3((unsigned)((2 * N + 255) / 256)), dim3(256), 0, s, nblk, N, part,
+            hipLaunchKernelGGL((k_layer_norm_cols<W>), dim3((unsigned)((2 * N + 63) / 64)), dim3(1024), 0, s, nblk, N, part,
                                static_cast<W*>(dgamma), static_cast<W*>(dbeta));
             GM_LAUNCH_CHECK();
         }

@@ -10,15 +10,39 @@
 
 namespace gm {
 
-template <class T>
+// A row is `tpr` threads wide (a power of two up to the workgroup), V elements a thread and step; a workgroup takes
+// FWD_ROWS rows per thread so that their loads are in flight together (the address of each waits for its token).
+constexpr int FWD_ROWS = 4;
+template <class T, int V, bool TAIL>
 __global__ void __launch_bounds__(256)
-k_token_embedding_fwd(int64_t n, int64_t C, int64_t w, IndexArray tok, const T* __restrict__ W, int64_t ldw, float scale,
+k_token_embedding_fwd(int64_t n, int64_t C, int w, int shift, IndexArray tok, const T* __restrict__ W, int64_t ldw, float scale,
                       T* __restrict__ out, int64_t ldo) {
-    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (g >= n * w) return;
-    const int64_t i = g / w, col = g - i * w;
-    const int64_t c = tok.at(i);
-    out[i * ldo + col] = c >= 0 && c < C ? from_f32<T>(to_f32(W[c * ldw + col]) * scale) : from_f32<T>(__builtin_nanf(""));
+    const int tpr = 1 << shift, rows = 256 >> shift;
+    const int t = threadIdx.x & (tpr - 1);
+    const int64_t step = (int64_t)gridDim.x * rows * FWD_ROWS;
+    for (int64_t i0 = (int64_t)blockIdx.x * rows * FWD_ROWS + (threadIdx.x >> shift); i0 < n; i0 += step) {
+        int64_t c[FWD_ROWS];
+#pragma unroll
+        for (int u = 0; u < FWD_ROWS; ++u) {
+            const int64_t i = i0 + u * rows;
+            c[u] = i < n ? tok.at(i) : -1;
+        }
+        for (int col = t * V; col < w; col += tpr * V) {
+            Vec<T, V> x[FWD_ROWS];
+#pragma unroll
+            for (int u = 0; u < FWD_ROWS; ++u)
+                x[u] = load_vec<T, V, TAIL>(W + (c[u] >= 0 && c[u] < C ? c[u] : 0) * ldw, col, w);
+#pragma unroll
+            for (int u = 0; u < FWD_ROWS; ++u) {
+                const int64_t i = i0 + u * rows;
+                if (i >= n) continue;
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = c[u] >= 0 && c[u] < C ? to_f32(x[u].v[v]) * scale : __builtin_nanf("");
+                store_vec<T, V, TAIL>(out + i * ldo, col, w, y);
+            }
+        }
+    }
 }
 
 // ---- stable radix sort of n keys in [0, C] (C: tokens that add to no row, sorted behind the others), RADIX_BITS at a time
@@ -27,6 +51,24 @@ constexpr int SORT_KEYS = 2048;                       // keys per workgroup: 4 w
 __device__ __forceinline__ uint32_t token_key(const IndexArray& tok, int64_t i, int64_t C, int64_t padding) {
     const int64_t c = tok.at(i);
     return c >= 0 && c < C && c != padding ? (uint32_t)c : (uint32_t)C;
+}
+
+// The place of a lane's key with digit d: the wave's next free place of the digit and the number of lower lanes with the same
+// one (found by a ballot per digit bit), so that equal digits keep their order.  Moves the digit's next free place on.
+__device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, bool in, int lane) {
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int bit = 0; bit < RADIX_BITS; ++bit) {
+        const uint64_t set = __ballot((d >> bit) & 1u);
+        same &= (d >> bit) & 1u ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1ull));
+    uint32_t at = 0;
+    if (in) at = next[d] + rank;
+    wave_fence();                                       // every lane has read its place before a leader moves it on
+    if (in && rank == 0) next[d] = at + (uint32_t)__popcll(same);
+    wave_fence();
+    return at;
 }
 
 // counts[digit][workgroup]
@@ -48,15 +90,23 @@ k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint3
     for (int b = threadIdx.x; b < RADIX_BINS; b += 256) counts[(int64_t)b * gridDim.x + blockIdx.x] = hist[b];
 }
 
-// exclusive prefix sum of m counts by one workgroup
+// exclusive prefix sum of m counts (a multiple of 4) by one workgroup, SCAN_EACH a thread and step
+constexpr int SCAN_EACH = 16;
 __global__ void __launch_bounds__(1024) k_radix_scan(int64_t m, uint32_t* __restrict__ counts) {
     __shared__ uint32_t tot[16];
     uint32_t carry = 0;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    for (int64_t b = 0; b < m; b += 1024) {
-        const int64_t i = b + threadIdx.x;
-        const uint32_t v = i < m ? counts[i] : 0;
-        uint32_t s = v;
+    for (int64_t b = 0; b < m; b += 1024 * SCAN_EACH) {
+        const int64_t i = b + threadIdx.x * SCAN_EACH;
+        uint32_t v[SCAN_EACH], sum = 0;
+#pragma unroll
+        for (int k = 0; k < SCAN_EACH; k += 4) {
+            const uint4 x = i + k < m ? *reinterpret_cast<const uint4*>(counts + i + k) : make_uint4(0, 0, 0, 0);
+            v[k] = x.x; v[k + 1] = x.y; v[k + 2] = x.z; v[k + 3] = x.w;
+        }
+#pragma unroll
+        for (int k = 0; k < SCAN_EACH; ++k) sum += v[k];
+        uint32_t s = sum;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const uint32_t t = __shfl_up(s, off);
@@ -64,20 +114,26 @@ __global__ void __launch_bounds__(1024) k_radix_scan(int64_t m, uint32_t* __rest
         }
         if (lane == 63) tot[wv] = s;
         __syncthreads();
-        uint32_t before = 0, all = 0;
+        uint32_t at = carry + s - sum;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            if (k < wv) before += tot[k];
-            all += tot[k];
+            if (k < wv) at += tot[k];
+            carry += tot[k];
         }
-        if (i < m) counts[i] = carry + before + s - v;
-        carry += all;
+#pragma unroll
+        for (int k = 0; k < SCAN_EACH; k += 4) {
+            uint4 x;
+            x.x = at; at += v[k];
+            x.y = at; at += v[k + 1];
+            x.z = at; at += v[k + 2];
+            x.w = at; at += v[k + 3];
+            if (i + k < m) *reinterpret_cast<uint4*>(counts + i + k) = x;
+        }
         __syncthreads();
     }
 }
 
-// Each wave owns SORT_KEYS/4 consecutive keys and keeps the next free place of every digit; the rank among the 64 keys of
-// a round is the number of lower lanes with the same digit (one ballot per digit bit), so equal digits keep their order.
+// Each wave owns SORT_KEYS/4 consecutive keys and keeps the next free place of every digit.
 __global__ void __launch_bounds__(256)
 k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys,
                 const uint32_t* __restrict__ pos, int shift, const uint32_t* __restrict__ starts, uint32_t* __restrict__ keys_out,
@@ -113,21 +169,83 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
         const int64_t i = base + r * 64 + lane;
         const bool in = i < n;
         const uint32_t d = (key[r] >> shift) & (RADIX_BINS - 1);
-        uint64_t same = __ballot(in);
-#pragma unroll
-        for (int bit = 0; bit < RADIX_BITS; ++bit) {
-            const uint64_t set = __ballot((d >> bit) & 1u);
-            same &= (d >> bit) & 1u ? set : ~set;
-        }
-        const int rank = __popcll(same & ((1ull << lane) - 1ull));
-        uint32_t at = 0;
-        if (in) at = next[wv][d] + rank;
-        wave_fence();                                   // every lane has read its place before a leader moves it on
-        if (in && rank == 0) next[wv][d] = at + (uint32_t)__popcll(same);
-        wave_fence();
+        const uint32_t at = take_place(next[wv], d, in, lane);
         if (in) {
             keys_out[at] = key[r];
             pos_out[at] = pos ? pos[i] : (uint32_t)i;
+        }
+    }
+}
+
+// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch.  Wave wv holds keys
+// [wv * 1024, wv * 1024 + 1024) of the current order in registers and exchanges them through LDS.
+constexpr int SMALL_WAVES = 8, SMALL_ROUNDS = 16, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64;
+__global__ void __launch_bounds__(SMALL_WAVES * 64)
+k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes, uint32_t* __restrict__ keys_out,
+                   uint32_t* __restrict__ pos_out) {
+    __shared__ uint32_t next[SMALL_WAVES][RADIX_BINS];
+    __shared__ uint32_t buf[SMALL_KEYS];
+    __shared__ uint32_t tot[SMALL_WAVES];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    uint32_t key[SMALL_ROUNDS], pos[SMALL_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < SMALL_ROUNDS; ++r) {
+        const int i = (wv * SMALL_ROUNDS + r) * 64 + lane;
+        pos[r] = (uint32_t)i;
+        key[r] = i < n ? token_key(tok, i, C, padding) : 0xFFFFFFFFu;         // behind every key in every digit: stays last
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * RADIX_BITS;
+        for (int b = threadIdx.x; b < SMALL_WAVES * RADIX_BINS; b += SMALL_WAVES * 64) (&next[0][0])[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < SMALL_ROUNDS; ++r) atomicAdd(&next[wv][(key[r] >> shift) & (RADIX_BINS - 1)], 1u);
+        __syncthreads();
+        // thread b owns digit b: starts of the digits by a scan over the workgroup, then of each wave's share of its digit
+        static_assert(RADIX_BINS == SMALL_WAVES * 64, "one thread a digit");
+        uint32_t sum = 0;
+#pragma unroll
+        for (int k = 0; k < SMALL_WAVES; ++k) sum += next[k][threadIdx.x];
+        uint32_t s = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t t = __shfl_up(s, off);
+            if (lane >= off) s += t;
+        }
+        if (lane == 63) tot[wv] = s;
+        __syncthreads();
+        uint32_t at = s - sum;
+        for (int k = 0; k < wv; ++k) at += tot[k];
+#pragma unroll
+        for (int k = 0; k < SMALL_WAVES; ++k) {
+            const uint32_t c = next[k][threadIdx.x];
+            next[k][threadIdx.x] = at;
+            at += c;
+        }
+        __syncthreads();
+        uint32_t place[SMALL_ROUNDS];
+#pragma unroll
+        for (int r = 0; r < SMALL_ROUNDS; ++r) {
+            const uint32_t d = (key[r] >> shift) & (RADIX_BINS - 1);
+            place[r] = take_place(next[wv], d, true, lane);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint32_t(&x)[SMALL_ROUNDS] = half ? pos : key;
+#pragma unroll
+            for (int r = 0; r < SMALL_ROUNDS; ++r) buf[place[r]] = x[r];
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < SMALL_ROUNDS; ++r) x[r] = buf[(wv * SMALL_ROUNDS + r) * 64 + lane];
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < SMALL_ROUNDS; ++r) {
+        const int i = (wv * SMALL_ROUNDS + r) * 64 + lane;
+        if (i < n) {
+            keys_out[i] = key[r];
+            pos_out[i] = pos[r];
         }
     }
 }
@@ -146,37 +264,182 @@ k_token_rowptr(int64_t n, int64_t C, const uint32_t* __restrict__ keys, uint32_t
     rowptr[c] = (uint32_t)lo;
 }
 
-// one wave per row of dW
+// ---- sums of gradient rows.  A wave covers K x 64 x V columns, or a narrow row with `lanes` lanes (a power of two) and
+// per = 64 / lanes rows side by side, joined at the end.  The lanes fetch 64 positions at once; the rows of up to 8 rounds
+// are then in flight together (walked one by one, each row waits for its position and then for itself).
+template <class T, int V, bool TAIL, int K>
+struct RowSum {
+    float acc[K][V];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[k][v] = 0.0f;
+    }
+    // R rounds from round r; an entry behind the last one loads from the last one's row and sees zeros
+    template <int R>
+    __device__ __forceinline__ void rounds(int r, int count, int sub, int per, uint32_t p, const T* __restrict__ G, int64_t ldg, int w, int col) {
+        Vec<T, V> x[R][K];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int e = (r + u) * per + sub;
+            const T* row = G + (int64_t)__shfl(p, e & 63) * ldg;
+#pragma unroll
+            for (int k = 0; k < K; ++k) x[u][k] = load_vec<T, V, TAIL>(row, e < count ? col + k * 64 * V : w, w);
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[k][v] = acc[k][v] + to_f32(x[u][k].v[v]);
+    }
+    // rows at the sorted positions [a, b)
+    __device__ __forceinline__ void add(const uint32_t* __restrict__ pos, uint32_t a, uint32_t b, const T* __restrict__ G, int64_t ldg, int w,
+                                        int col0, int lanes) {
+        const int lane = threadIdx.x & 63, sub = lane / lanes, per = 64 / lanes;
+        const int col = col0 + (lane & (lanes - 1)) * V;
+        for (uint32_t i = a; i < b; i += 64) {
+            const int count = b - i < 64 ? (int)(b - i) : 64, all = (count + per - 1) / per;
+            const uint32_t p = pos[i + (lane < count ? lane : count - 1)];
+            for (int r = 0; r < all; r += 8) {
+                if (all - r > 4) rounds<8>(r, count, sub, per, p, G, ldg, w, col);
+                else if (all - r > 1) rounds<4>(r, count, sub, per, p, G, ldg, w, col);
+                else rounds<1>(r, count, sub, per, p, G, ldg, w, col);
+            }
+        }
+    }
+    __device__ __forceinline__ void join(int lanes) {
+        for (int off = 32; off >= lanes; off >>= 1)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[k][v] = acc[k][v] + __shfl_xor(acc[k][v], off);
+    }
+};
+
+// A row of more than `cut` tokens is summed in pieces, one for each chunk of `cut` sorted positions that it meets:
+// part[2k] of the row that chunk k begins with, part[2k+1] of the row that it ends with and did not begin with.  Such a row
+// meets at least two chunks, so a chunk holds pieces of at most two of them.
+template <class T, int V, bool TAIL, int K>
+__global__ void __launch_bounds__(64)
+k_token_pieces(int64_t n, int64_t C, int w, int lanes, uint32_t cut, const uint32_t* __restrict__ keys,
+               const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G, int64_t ldg,
+               float* __restrict__ part, int64_t ldp) {
+    const int lane = threadIdx.x, col0 = blockIdx.y * 64 * V * K;
+    const uint32_t a = blockIdx.x * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
+    const uint32_t first = keys[a], last = keys[b - 1];
+#pragma unroll 1
+    for (int end = 0; end < 2; ++end) {
+        const uint32_t c = end ? last : first;
+        if (c >= C || (end && last == first)) continue;
+        const uint32_t r0 = rowptr[c], r1 = rowptr[c + 1];
+        if (r1 - r0 <= cut) continue;
+        RowSum<T, V, TAIL, K> sum;
+        sum.clear();
+        sum.add(pos, r0 > a ? r0 : a, r1 < b ? r1 : b, G, ldg, w, col0, lanes);
+        sum.join(lanes);
+        float* to = part + (2 * (int64_t)blockIdx.x + end) * ldp;
+        if (lane < lanes)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int col = col0 + (lane + k * 64) * V;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (col + v < w) to[col + v] = sum.acc[k][v];
+            }
+    }
+}
+
+// The row that begins in chunk blockIdx.x and goes on behind it, if it is one of more than `cut` tokens.  `wide` threads (a
+// power of two) take four columns each, 1024 / wide lanes of them every so-manieth piece; the lanes are added as a tree.
 template <class T>
-__global__ void __launch_bounds__(256)
-k_token_grad(int64_t C, int64_t w, const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos,
-             const T* __restrict__ G, int64_t ldg, float scale, T* __restrict__ dW, int64_t ldw) {
-    const int lane = threadIdx.x & 63;
-    const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ void __launch_bounds__(1024)
+k_token_join(int64_t n, int64_t C, int w, int64_t ldp, int wide, uint32_t cut, const uint32_t* __restrict__ keys,
+             const uint32_t* __restrict__ rowptr, const float* __restrict__ part, float scale, T* __restrict__ dW, int64_t ldw) {
+    __shared__ float4 red[1024];
+    const uint32_t a = blockIdx.x * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
+    const uint32_t c = keys[b - 1];
     if (c >= C) return;
-    const uint32_t a = rowptr[c], b = rowptr[c + 1];
-    for (int64_t col = lane; col < w; col += 64) {
-        float acc = 0.0f;
-        for (uint32_t k = a; k < b; ++k) acc = acc + to_f32(G[(int64_t)pos[k] * ldg + col]);
-        dW[c * ldw + col] = from_f32<T>(acc * scale);
+    const uint32_t r0 = rowptr[c], r1 = rowptr[c + 1];
+    if (r1 - r0 <= cut || r0 < a) return;
+    const uint32_t k1 = (r1 - 1) / cut;
+    const int lanes = 1024 / wide, lane = threadIdx.x / wide, t = threadIdx.x & (wide - 1);
+    for (int col0 = 0; col0 < w; col0 += 4 * wide) {
+        const int col = col0 + 4 * t;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (col < w)
+#pragma unroll 4
+            for (uint32_t q = blockIdx.x + lane; q <= k1; q += lanes) {
+                const int64_t at = (2 * (int64_t)q + (q == blockIdx.x && r0 != a ? 1 : 0)) * ldp + col;
+                const float4 x = *reinterpret_cast<const float4*>(part + at);
+                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+            }
+        __syncthreads();
+        red[threadIdx.x] = acc;
+        for (int half = lanes / 2; half >= 1; half /= 2) {
+            __syncthreads();
+            if (lane < half) {
+                const float4 x = red[threadIdx.x + half * wide];
+                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+                red[threadIdx.x] = acc;
+            }
+        }
+        if (lane == 0) {
+            const float y[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (col + v < w) dW[c * ldw + col + v] = from_f32<T>(y[v] * scale);
+        }
+    }
+}
+
+// every other row of dW, one wave per row and 64 V K columns
+template <class T, int V, bool TAIL, int K>
+__global__ void __launch_bounds__(256)
+k_token_grad(int64_t C, int w, int lanes, uint32_t cut, const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos,
+             const T* __restrict__ G, int64_t ldg, float scale, T* __restrict__ dW, int64_t ldw) {
+    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V * K;
+    for (int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); c < C; c += (int64_t)gridDim.x * 4) {
+        const uint32_t a = rowptr[c], b = rowptr[c + 1];
+        if (b - a > cut) continue;
+        RowSum<T, V, TAIL, K> sum;
+        sum.clear();
+        if (a < b) {
+            sum.add(pos, a, b, G, ldg, w, col0, lanes);
+            sum.join(lanes);
+        }
+        if (lane < lanes)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int col = col0 + (lane + k * 64) * V;
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = sum.acc[k][v] * scale;
+                store_vec<T, V, TAIL>(dW + c * ldw, col, w, y);
+            }
     }
 }
 
 struct TokenLayout {
-    int64_t nblk, keys[2], pos[2], counts, rowptr, bytes;
+    int64_t nblk, keys[2], pos[2], counts, rowptr, part, bytes;
+    uint32_t cut;
     int passes;
 };
-static inline TokenLayout token_layout(int64_t n, int64_t C) {
+static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
     TokenLayout l;
     int bits = 1;
     while ((C >> bits) != 0) ++bits;                   // keys are 0..C
     l.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
     l.nblk = (n + SORT_KEYS - 1) / SORT_KEYS;
+    l.cut = 64;
+    while ((int64_t)l.cut * 4096 < n) l.cut *= 2;      // at most 4096 pieces of one row
     int64_t at = 0;
     auto take = [&at](int64_t words) { const int64_t p = at; at += (words * 4 + 255) / 256 * 256; return p; };
     for (int k = 0; k < 2; ++k) { l.keys[k] = take(n); l.pos[k] = take(n); }
-    l.counts = take(l.nblk * RADIX_BINS);
+    l.counts = take(n > SMALL_KEYS ? l.nblk * RADIX_BINS : 0);
     l.rowptr = take(C + 1);
+    l.part = take(n > l.cut ? 2 * ((n + l.cut - 1) / l.cut) * ((w + 3) / 4 * 4) : 0);
     l.bytes = at;
     return l;
 }
@@ -188,26 +451,32 @@ using namespace gm;
 #define GM_TOKEN_CHECK(ptr_)                                                                                              \
     GM_REQUIRE(n >= 0 && C > 0 && w > 0 && (n == 0 || (tokens && ptr_)), "bad arguments");                                \
     GM_REQUIRE(dtype_ok(dtype), "dtype %d is none of GM_DTYPE_*", dtype);                                                 \
-    GM_REQUIRE(C < (1ll << 31) && n < (1ll << 31) && w < (1ll << 31), "n, C or w of 2^31 or more")
+    GM_REQUIRE(C < (1ll << 31) && n < (1ll << 31) && w < (1ll << 30), "n or C of 2^31 or more, or w of 2^30 or more")
 
 extern "C" int gm_token_embedding_fwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, const void* weight,
                                       int64_t ldw, int dtype, float scale, void* out, int64_t ldo, gm_stream_t stream) {
     GM_TOKEN_CHECK(out);
     GM_REQUIRE(weight && ldw >= w && ldo >= w, "weight missing or leading dimension too small");
     if (n == 0) return GM_OK;
-    GM_REQUIRE((n * w + 255) / 256 < (1ll << 31), "n * w too large");
+    const int vec = w < 16 / dtype_size(dtype) ? 1 : 16 / dtype_size(dtype);        // with_row_form
+    int shift = 0;
+    while (shift < 8 && ((int64_t)vec << shift) < w) ++shift;
+    const int64_t rows = (int64_t)(256 >> shift) * FWD_ROWS;
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        hipLaunchKernelGGL((k_token_embedding_fwd<T>), dim3((unsigned)((n * w + 255) / 256)), dim3(256), 0, as_stream(stream), n, C,
-                           w, IndexArray{tokens, tokens_i64}, static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out), ldo);
+        with_row_form<T>(w, [&](auto v, auto tail) {
+            hipLaunchKernelGGL((k_token_embedding_fwd<T, decltype(v)::value, decltype(tail)::value>), dim3(grid_for((n + rows - 1) / rows, 256)),
+                               dim3(256), 0, as_stream(stream), n, C, (int)w, shift, IndexArray{tokens, tokens_i64},
+                               static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out), ldo);
+        });
         GM_LAUNCH_CHECK();
         return GM_OK;
     });
 }
 
 extern "C" int64_t gm_token_embedding_bwd_workspace_bytes(int64_t n, int64_t C, int64_t w) {
-    if (n < 0 || C <= 0 || w <= 0 || n >= (1ll << 31) || C >= (1ll << 31)) return -1;
-    return token_layout(n, C).bytes;
+    if (n < 0 || C <= 0 || w <= 0 || n >= (1ll << 31) || C >= (1ll << 31) || w >= (1ll << 30)) return -1;
+    return token_layout(n, C, w).bytes;
 }
 
 extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, int64_t padding_idx,
@@ -216,7 +485,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     GM_TOKEN_CHECK(G);
     GM_REQUIRE(dW && ldg >= w && ldw >= w, "dW missing or leading dimension too small");
     GM_REQUIRE(padding_idx < C, "padding_idx %lld is not below C = %lld", (long long)padding_idx, (long long)C);
-    const TokenLayout l = token_layout(n, C);
+    const TokenLayout l = token_layout(n, C, w);
     GM_REQUIRE(workspace && workspace_bytes >= l.bytes && aligned(workspace, 16),
                "gm_token_embedding_bwd needs %lld workspace bytes (gm_token_embedding_bwd_workspace_bytes)", (long long)l.bytes);
     hipStream_t s = as_stream(stream);
@@ -224,26 +493,67 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     auto u32 = [ws](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
     const IndexArray tok{tokens, tokens_i64};
     uint32_t *counts = u32(l.counts), *rowptr = u32(l.rowptr);
-    const uint32_t *keys = nullptr, *pos = nullptr;
-    for (int p = 0; p < l.passes && n > 0; ++p) {
+    const uint32_t *keys = u32(l.keys[0]), *pos = u32(l.pos[0]);
+    float* part = reinterpret_cast<float*>(ws + l.part);
+    if (n > 0 && n <= SMALL_KEYS) {
+        hipLaunchKernelGGL(k_token_sort_small, dim3(1), dim3(SMALL_WAVES * 64), 0, s, (int)n, C, padding_idx, tok, l.passes,
+                           u32(l.keys[0]), u32(l.pos[0]));
+        GM_LAUNCH_CHECK();
+    }
+    for (int p = 0; p < l.passes && n > SMALL_KEYS; ++p) {
         uint32_t *ko = u32(l.keys[p & 1]), *po = u32(l.pos[p & 1]);
-        hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, keys, p * RADIX_BITS, counts);
+        hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
+                           p * RADIX_BITS, counts);
         GM_LAUNCH_CHECK();
         hipLaunchKernelGGL(k_radix_scan, dim3(1), dim3(1024), 0, s, l.nblk * RADIX_BINS, counts);
         GM_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_radix_scatter, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, keys, pos, p * RADIX_BITS,
-                           counts, ko, po);
+        hipLaunchKernelGGL(k_radix_scatter, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
+                           p ? pos : nullptr, p * RADIX_BITS, counts, ko, po);
         GM_LAUNCH_CHECK();
         keys = ko;
         pos = po;
     }
     hipLaunchKernelGGL(k_token_rowptr, dim3((unsigned)((C + 1 + 255) / 256)), dim3(256), 0, s, n, C, keys, rowptr);
     GM_LAUNCH_CHECK();
+    const int vec = w < 16 / dtype_size(dtype) ? 1 : 16 / dtype_size(dtype);        // with_row_form
+    const int64_t vecs = (w + vec - 1) / vec;
+    int lanes = 64;
+    while (lanes > 1 && lanes / 2 >= vecs) lanes /= 2;
+    const int K = vecs > 64 ? 2 : 1;                    // a wave's two accesses to each row of a wide table
+    const unsigned tiles = (unsigned)((vecs + 64 * K - 1) / (64 * K));
+    const unsigned chunks = (unsigned)((n + l.cut - 1) / l.cut);
+    GM_REQUIRE(tiles < 65536u, "w too large");
+    const int64_t ldp = (w + 3) / 4 * 4;
+    int wide = 1;
+    while (wide < 256 && wide * 4 < w) wide *= 2;
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        hipLaunchKernelGGL((k_token_grad<T>), dim3((unsigned)((C + 3) / 4)), dim3(256), 0, s, C, w, rowptr, pos,
-                           static_cast<const T*>(G), ldg, scale, static_cast<T*>(dW), ldw);
-        GM_LAUNCH_CHECK();
+        int rc = GM_OK;
+        with_row_form<T>(w, [&](auto v, auto tail) {
+            constexpr int V = decltype(v)::value;
+            constexpr bool TAIL = decltype(tail)::value;
+            rc = [&]() -> int {
+#define GM_LAUNCH_GRAD(K_)                                                                                                \
+    do {                                                                                                                  \
+        if (n > l.cut) {                                                                                                  \
+            hipLaunchKernelGGL((k_token_pieces<T, V, TAIL, K_>), dim3(chunks, tiles), dim3(64), 0, s, n, C, (int)w, lanes, l.cut, keys, rowptr, pos, \
+                               static_cast<const T*>(G), ldg, part, ldp);                                                 \
+            GM_LAUNCH_CHECK();                                                                                            \
+            hipLaunchKernelGGL((k_token_join<T>), dim3(chunks), dim3(1024), 0, s, n, C, (int)w, ldp, wide, l.cut, keys, rowptr, part, scale, \
+                               static_cast<T*>(dW), ldw);                                                                 \
+            GM_LAUNCH_CHECK();                                                                                            \
+        }                                                                                                                 \
+        hipLaunchKernelGGL((k_token_grad<T, V, TAIL, K_>), dim3(grid_for((C + 3) / 4, 256), tiles), dim3(256), 0, s, C, (int)w, lanes,       \
+                           l.cut, rowptr, pos, static_cast<const T*>(G), ldg, scale, static_cast<T*>(dW), ldw);           \
+    } while (0)
+                if (K == 2) GM_LAUNCH_GRAD(2);
+                else GM_LAUNCH_GRAD(1);
+#undef GM_LAUNCH_GRAD
+                GM_LAUNCH_CHECK();
+                return GM_OK;
+            }();
+        });
+        if (rc != GM_OK) return rc;
         return GM_OK;
     });
 }
