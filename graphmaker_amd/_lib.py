@@ -24,7 +24,7 @@ EXPORTS = [
     "gm_hadamard_gather_bwd", "gm_softmax_ce2_workspace_bytes", "gm_softmax_ce2", "gm_ce2_diff", "gm_head_diff_bwd",
     "gm_relu_bwd", "gm_dropout", "gm_embedding_fwd", "gm_denoise_match2", "gm_bitmap_lookup",
     "gm_token_embedding_fwd", "gm_token_embedding_bwd_workspace_bytes", "gm_token_embedding_bwd", "gm_layer_norm_fwd",
-    "gm_layer_norm_bwd_workspace_bytes", "gm_layer_norm_bwd", "gm_class_log_prob_workspace_bytes", "gm_class_log_prob_fwd",
+    "gm_layer_norm_bwd_workspace_bytes", "gm_layer_norm_bwd", "gm_class_log_prob_stats_floats", "gm_class_log_prob_workspace_bytes", "gm_class_log_prob_fwd",
     "gm_class_log_prob_bwd", "gm_sequence_loss_workspace_bytes", "gm_policy_loss_fwd", "gm_preference_loss_fwd",
     "gm_sequence_loss_bwd",
     "gm_triangles_per_node", "gm_same_class_degree", "gm_bitmap_square", "gm_class_bitmaps", "gm_masked_degree",
@@ -37,7 +37,7 @@ _SIGNATURES = {
     "gm_token_embedding_fwd": "iiipdpidfpip", "gm_token_embedding_bwd_workspace_bytes": "iii",
     "gm_token_embedding_bwd": "iiipdipidfpipip", "gm_layer_norm_fwd": "iipidppdfpippp",
     "gm_layer_norm_bwd_workspace_bytes": "ii", "gm_layer_norm_bwd": "iipipidpppdpipppip",
-    "gm_class_log_prob_workspace_bytes": "ii", "gm_class_log_prob_fwd": "iipidpdipppip",
+    "gm_class_log_prob_stats_floats": "iid", "gm_class_log_prob_workspace_bytes": "iid", "gm_class_log_prob_fwd": "iipidpdipppip",
     "gm_class_log_prob_bwd": "iippidpdippip", "gm_sequence_loss_workspace_bytes": "ii",
     "gm_policy_loss_fwd": "iippppppdfffdpppppip", "gm_preference_loss_fwd": "iippppdffdppppip",
     "gm_sequence_loss_bwd": "iipppdpppp",
@@ -79,7 +79,7 @@ def load():
         for name, kinds in _SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = [_CTYPES[k] for k in kinds]
-            fn.restype = C.c_int64 if name.endswith("_bytes") else C.c_int
+            fn.restype = C.c_int64 if name.endswith(("_bytes", "_floats")) else C.c_int
         _lib = lib
     return _lib
 

@@ -639,11 +639,15 @@ def _class_log_prob_fwd(logits, classes, i64, ignore_index, stats):
     x2, ldx = _rows(logits, V)
     M = x2.shape[0]
     lp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    st = torch.empty((M, 2), dtype=torch.float32, device=dev) if stats else None
-    need = L.load().gm_class_log_prob_workspace_bytes(M, V)
+    code = L.DTYPES[logits.dtype]
+    st = None
+    if stats:
+        floats = L.load().gm_class_log_prob_stats_floats(M, V, code)
+        st = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    need = L.load().gm_class_log_prob_workspace_bytes(M, V, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    L.launch("gm_class_log_prob_fwd", dev, M, V, x2.data_ptr(), ldx, L.DTYPES[logits.dtype], classes.data_ptr(), i64, ignore_index,
-             lp.data_ptr(), st.data_ptr() if stats else None, ws.data_ptr() if need else None, need)
+    L.launch("gm_class_log_prob_fwd", dev, M, V, x2.data_ptr(), ldx, code, classes.data_ptr(), i64, ignore_index,
+             lp.data_ptr(), st.data_ptr() if st is not None else None, ws.data_ptr() if need else None, need)
     return lp, x2, st
 
 
@@ -665,7 +669,7 @@ class _ClassLogProb(torch.autograd.Function):
         g = _c(g)
         dx = torch.empty(shape, dtype=x2.dtype, device=x2.device)
         L.launch("gm_class_log_prob_bwd", x2.device, M, V, g.data_ptr(), x2.data_ptr(), ldx, L.DTYPES[x2.dtype], classes.data_ptr(), i64,
-                 ignore_index, st.data_ptr(), dx.data_ptr(), V)
+                 ignore_index, st.data_ptr() if st is not None else None, dx.data_ptr(), V)
         return dx, None, None, None
 
 
