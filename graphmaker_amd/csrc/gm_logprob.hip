@@ -15,16 +15,7 @@
 
 namespace gm {
 
-// exp(x), x <= 0, within about a unit in the last place: 2^(x log2 e) with the product's rounding error put back as a factor.
-// exp(-inf) = 0, NaN stays NaN.
-__device__ __forceinline__ float exp_nonpos(float x) {
-    x = x < -120.0f ? -120.0f : x;                       // 2^-173: below every float
-    const float t = x * 1.44269502f;
-    const float lo = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e * lo, 0.693147182f, e);
-}
-// the same without the correction, off by 1.2 |x| 2^-24 relative: for the sums of long rows, where |x| weighted by exp(x) is
+// exp(x), x <= 0, without exp_any's correction, off by 1.2 |x| 2^-24 relative: for the sums of long rows, where |x| weighted by exp(x) is
 // small against the number of additions
 __device__ __forceinline__ float exp_quick(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
@@ -66,7 +57,7 @@ k_log_prob_narrow(int64_t M, const float* __restrict__ g, const T* __restrict__ 
             float e[E];
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                e[j] = exp_nonpos(x[j] - mx);
+                e[j] = exp_any(x[j] - mx);
                 s = s + e[j];
             }
             if constexpr (!GRAD) {
@@ -110,7 +101,7 @@ k_log_prob_held(int64_t M, int N, const T* __restrict__ X, int64_t ldx, IndexArr
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s = s + exp_nonpos(or_neg_inf(to_f32(r[k].v[i]), (k * LANES + t) * V + i < N) - mx);
+            for (int i = 0; i < V; ++i) s = s + exp_any(or_neg_inf(to_f32(r[k].v[i]), (k * LANES + t) * V + i < N) - mx);
 #pragma unroll
         for (int off = LANES / 2; off >= 1; off >>= 1) s = s + __shfl_xor(s, off);
         if (t == 0) {
@@ -140,7 +131,7 @@ k_log_prob_held_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
             float y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float v = -gu * exp_nonpos((to_f32(r[k].v[i]) - st.x) - st.y);
+                const float v = -gu * exp_any((to_f32(r[k].v[i]) - st.x) - st.y);
                 y[i] = gu == 0.0f ? 0.0f : (col + i == c ? gu + v : v) + bad;
             }
             store_vec<T, V, TAIL>(dX + m * lddx, col, N, y);

@@ -44,6 +44,19 @@ struct Sequences {
         }
         return first;
     }
+    // the same for a whole wave and one i: 64 starts are tried at once, so that the search waits once per factor of 64
+    __device__ __forceinline__ int64_t of_wave(int64_t i, int64_t first, int64_t last) const {
+        if (!offsets.p) return 0;
+        while (first < last) {
+            const int64_t step = (last - first + 63) / 64;           // tries first + step, first + 2 step, ... up to last
+            const int64_t at = first + step * ((threadIdx.x & 63) + 1);
+            const int n = __popcll(__ballot(at <= last && offsets.at(at <= last ? at : last) <= i));
+            const int64_t next = first + step * (n + 1) - 1;
+            first += step * n;
+            last = next < last ? next : last;
+        }
+        return first;
+    }
 };
 
 static inline int64_t chunk_items(int64_t M) { return M <= 2048 * 1024 ? 1024 : ((M + 2047) / 2048 + 1023) / 1024 * 1024; }
@@ -52,7 +65,6 @@ template <int Q> struct alignas(8) Sums { double v[Q]; };
 
 // exp(x) - 1 - x: the series where the difference would cancel (its first left-out term is below 2^-24 of the sum)
 __device__ __forceinline__ float exp_minus_1_x(float x) {
-    if (!(__builtin_fabsf(x) < 1.0f)) return expf(x) - 1.0f - x;
     float p = 2.75573192e-7f;                           // 1/10!
     p = __builtin_fmaf(p, x, 2.75573192e-6f);
     p = __builtin_fmaf(p, x, 2.48015873e-5f);
@@ -62,47 +74,68 @@ __device__ __forceinline__ float exp_minus_1_x(float x) {
     p = __builtin_fmaf(p, x, 4.16666667e-2f);
     p = __builtin_fmaf(p, x, 1.66666667e-1f);
     p = __builtin_fmaf(p, x, 0.5f);
-    return p * x * x;
+    return __builtin_fabsf(x) < 1.0f ? p * x * x : exp_any(x) - 1.0f - x;
 }
 
-struct PolicyTerm {                                      // sums: surrogate, KL, clipped items, live items
-    static constexpr int Q = 4;
+// What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.
+template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
+    static constexpr int Q = 4;                          // sums: surrogate, KL, clipped items, live items
+    struct Acc { double surrogate = 0.0, kl = 0.0; int cut = 0, live = 0; };
     const float *lp, *old, *adv, *ref;
     const uint8_t* mask;
     float low, high, kl;                                 // 1 - clip_low, 1 + clip_high, KL coefficient
-    int adv_per_sequence;
     float* slope;
-    __device__ __forceinline__ void add(int64_t i, int64_t s, Sums<4>& a) const {
-        float d = 0.0f;
-        if (!mask || mask[i]) {
-            const float l = lp[i], A = adv[adv_per_sequence ? s : i];
-            const float r = expf(l - old[i]);
-            const bool cut = (A > 0.0f && r > high) || (A < 0.0f && r < low);
-            const float gain = A == 0.0f ? 0.0f : (cut ? (A > 0.0f ? high : low) : r) * A;
-            a.v[0] -= (double)gain;
-            a.v[2] += cut ? 1.0 : 0.0;
-            a.v[3] += 1.0;
-            d = cut ? 0.0f : -gain;
-            if (ref) {
-                const float q = ref[i] - l, k = exp_minus_1_x(q);
-                a.v[1] += (double)k;
-                if (kl != 0.0f) d = d - kl * (q + k);
+    __device__ __forceinline__ float of_sequence(int64_t s) const { return ITEM_ADV ? 0.0f : adv[s]; }
+    template <int W> __device__ __forceinline__ void add(int64_t i, float of_seq, Acc& a) const {
+        using F = Vec<float, W>;
+        const F l = *reinterpret_cast<const F*>(lp + i), o = *reinterpret_cast<const F*>(old + i);
+        F A, q, d;
+        Vec<uint8_t, W> on;
+        if constexpr (ITEM_ADV) A = *reinterpret_cast<const F*>(adv + i);
+        if constexpr (REF) q = *reinterpret_cast<const F*>(ref + i);
+        if constexpr (MASK) on = *reinterpret_cast<const Vec<uint8_t, W>*>(mask + i);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const bool live = !MASK || on.v[k] != 0;
+            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, r = exp_any(l.v[k] - o.v[k]);
+            const bool cut = (adv_k > 0.0f && r > high) || (adv_k < 0.0f && r < low);
+            const float gain = adv_k == 0.0f ? 0.0f : (cut ? (adv_k > 0.0f ? high : low) : r) * adv_k;
+            float slope_k = cut ? 0.0f : -gain, apart = 0.0f;
+            if constexpr (REF) {
+                const float x = q.v[k] - l.v[k];
+                apart = exp_minus_1_x(x);
+                if (kl != 0.0f) slope_k = slope_k - kl * (x + apart);
             }
+            a.surrogate -= live ? (double)gain : 0.0;
+            if constexpr (REF) a.kl += live ? (double)apart : 0.0;
+            a.cut += live && cut ? 1 : 0;
+            a.live += live ? 1 : 0;
+            d.v[k] = live ? slope_k : 0.0f;
         }
-        if (slope) slope[i] = d;
+        if (slope) *reinterpret_cast<F*>(slope + i) = d;
     }
+    __device__ __forceinline__ static Sums<4> sums(const Acc& a) { return {{a.surrogate, a.kl, (double)a.cut, (double)a.live}}; }
 };
 
-struct PreferenceTerm {                                  // sums: log ratio, live items
-    static constexpr int Q = 2;
+template <bool MASK> struct PreferenceTerm {
+    static constexpr int Q = 2;                          // sums: log ratio, live items
+    struct Acc { double ratio = 0.0; int live = 0; };
     const float *lp, *ref;
     const uint8_t* mask;
-    __device__ __forceinline__ void add(int64_t i, int64_t, Sums<2>& a) const {
-        if (!mask || mask[i]) {
-            a.v[0] += (double)lp[i] - (double)ref[i];
-            a.v[1] += 1.0;
+    __device__ __forceinline__ float of_sequence(int64_t) const { return 0.0f; }
+    template <int W> __device__ __forceinline__ void add(int64_t i, float, Acc& a) const {
+        using F = Vec<float, W>;
+        const F l = *reinterpret_cast<const F*>(lp + i), o = *reinterpret_cast<const F*>(ref + i);
+        Vec<uint8_t, W> on;
+        if constexpr (MASK) on = *reinterpret_cast<const Vec<uint8_t, W>*>(mask + i);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const bool live = !MASK || on.v[k] != 0;
+            a.ratio += live ? (double)l.v[k] - (double)o.v[k] : 0.0;
+            a.live += live ? 1 : 0;
         }
     }
+    __device__ __forceinline__ static Sums<2> sums(const Acc& a) { return {{a.ratio, (double)a.live}}; }
 };
 
 // pieces of the sequences: `whole`[s] of one inside this chunk; `piece`[2k] of one that began before chunk k,
@@ -114,27 +147,30 @@ k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whol
     __shared__ Sums<Q> red[4];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int64_t a = (int64_t)blockIdx.x * chunk, b = a + chunk < q.M ? a + chunk : q.M;
-    const int64_t s0 = q.of(a, 0, q.S - 1), s1 = q.of(b - 1, s0, q.S - 1);
-    const bool alone = s0 == s1;                         // one sequence: all four waves sum it together
+    const int64_t s0 = q.of_wave(a, 0, q.S - 1), s1 = q.of_wave(b - 1, s0, q.S - 1);
+    const bool alone = s0 == s1;                         // one sequence: all four waves sum it together, else one wave each
+    const int t = alone ? (int)threadIdx.x : lane, threads = alone ? 256 : 64;
     for (int64_t s = s0 + (alone ? 0 : wv); s <= s1; s += 4) {
         const int64_t lo = q.lo(s), hi = q.hi(s);
         const int64_t i0 = lo > a ? lo : a, i1 = hi < b ? hi : b;
         if (i0 >= i1) continue;                          // uniform over the workgroup if `alone`, over the wave if not
-        Sums<Q> acc = {};
-        const int64_t step = alone ? 256 : 64;
-#pragma unroll 4
-        for (int64_t i = i0 + (alone ? (int)threadIdx.x : lane); i < i1; i += step) f.add(i, s, acc);
+        const float of_seq = f.of_sequence(s);
+        typename F::Acc acc;
+        for (int64_t i = i0 + 4 * t; i + 4 <= i1; i += 4 * threads) f.template add<4>(i, of_seq, acc);
+        const int64_t rest = i0 + (i1 - i0) / 4 * 4 + t;
+        if (rest < i1) f.template add<1>(rest, of_seq, acc);
+        Sums<Q> sum = F::sums(acc);
 #pragma unroll
-        for (int c = 0; c < Q; ++c) acc.v[c] = wave_add(acc.v[c]);
+        for (int c = 0; c < Q; ++c) sum.v[c] = wave_add(sum.v[c]);
         if (alone) {
-            if (lane == 0) red[wv] = acc;
+            if (lane == 0) red[wv] = sum;
             __syncthreads();
 #pragma unroll
-            for (int c = 0; c < Q; ++c) acc.v[c] = ((red[0].v[c] + red[1].v[c]) + red[2].v[c]) + red[3].v[c];
+            for (int c = 0; c < Q; ++c) sum.v[c] = ((red[0].v[c] + red[1].v[c]) + red[2].v[c]) + red[3].v[c];
         }
         if (lane == 0 && (wv == 0 || !alone)) {
             Sums<Q>* to = lo >= a && hi <= b ? whole + s : piece + 2 * (int64_t)blockIdx.x + (lo < a ? 0 : 1);
-            *to = acc;
+            *to = sum;
         }
     }
 }
@@ -163,40 +199,42 @@ k_sequence_gather(Sequences q, int64_t chunk, Sums<Q>* __restrict__ whole, const
     if (s < q.S) gather_sequence<Q>(q, chunk, s, threadIdx.x & 63, whole, piece);
 }
 
-// sum over a workgroup of 1024 threads, in every thread
-__device__ __forceinline__ double block_add(double v, double* red) {
-    v = wave_add(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double t = 0.0;
+// sums over a workgroup of 1024 threads, in every thread
+template <int N> __device__ __forceinline__ void block_add(double (&v)[N], double (*red)[N]) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) t = t + red[k];
-    return t;
+    for (int c = 0; c < N; ++c) v[c] = wave_add(v[c]);
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int c = 0; c < N; ++c) red[threadIdx.x >> 6][c] = v[c];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        v[c] = 0.0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[c] = v[c] + red[k][c];
+    }
 }
 
 __global__ void __launch_bounds__(1024)
 k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, Sums<4>* __restrict__ whole,
                 const Sums<4>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ weight) {
-    __shared__ double red[16];
+    __shared__ double red[16][5];
     if (gather) {
         for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<4>(q, chunk, s, threadIdx.x & 63, whole, piece);
         __syncthreads();
     }
-    double tot[4] = {0.0, 0.0, 0.0, 0.0}, used = 0.0;
+    double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};           // the sums, live items, sequences that have one
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
         const Sums<4> w = whole[s];
         if (w.v[3] <= 0.0) continue;
         const double unit = by_sequence ? 1.0 / w.v[3] : 1.0;
-        used += 1.0;
+        tot[4] += 1.0;
 #pragma unroll
         for (int c = 0; c < 3; ++c) tot[c] += w.v[c] * unit;
         tot[3] += w.v[3];
     }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tot[c] = block_add(tot[c], red);
-    used = block_add(used, red);
-    const double over = by_sequence ? used : tot[3];
+    block_add(tot, red);
+    const double over = by_sequence ? tot[4] : tot[3];
     const double norm = over > 0.0 ? 1.0 / over : 0.0;    // no live item: the loss and every gradient are 0
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
         const double n = whole[s].v[3];
@@ -215,13 +253,13 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
 __global__ void __launch_bounds__(1024)
 k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double smoothing, int average, Sums<2>* __restrict__ whole,
                     const Sums<2>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ weight) {
-    __shared__ double red[16];
+    __shared__ double red[16][1];
     if (gather) {
         for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<2>(q, chunk, s, threadIdx.x & 63, whole, piece);
         __syncthreads();
     }
     const int64_t P = q.S / 2;
-    double tot = 0.0;
+    double tot[1] = {0.0};
     for (int64_t p = threadIdx.x; p < P; p += 1024) {
         double h[2], unit[2];
 #pragma unroll
@@ -233,33 +271,50 @@ k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double 
         }
         const double z = beta * (h[0] - h[1]), e = exp(-fabs(z));
         const double up = (z < 0.0 ? -z : 0.0) + log1p(e);              // -log sig(z); z NaN: e is
-        tot += smoothing != 0.0 ? (1.0 - smoothing) * up + smoothing * (up + z) : up;
+        tot[0] += smoothing != 0.0 ? (1.0 - smoothing) * up + smoothing * (up + z) : up;
         const double dz = (smoothing - (z >= 0.0 ? e : 1.0) / (1.0 + e)) / (double)P;    // sig(z) - 1 = -sig(-z)
         if (weight) {
             weight[2 * p] = (float)(beta * dz * unit[0]);
             weight[2 * p + 1] = (float)(-beta * dz * unit[1]);
         }
     }
-    tot = block_add(tot, red);
-    if (threadIdx.x == 0) loss[0] = (float)(tot / (double)P);
+    block_add(tot, red);
+    if (threadIdx.x == 0) loss[0] = (float)(tot[0] / (double)P);
 }
 
 // dl[i] = g weight[s] slope[i] for the live items of sequence s, 0 for every other item
+template <bool SLOPE, bool MASK>
 __global__ void __launch_bounds__(256)
 k_sequence_spread(Sequences q, int64_t chunk, const float* __restrict__ slope, const uint8_t* __restrict__ mask,
                   const float* __restrict__ weight, const float* __restrict__ g, float* __restrict__ dl) {
     const int64_t a = (int64_t)blockIdx.x * chunk, b = a + chunk < q.M ? a + chunk : q.M;
-    const int64_t s0 = q.of(a, 0, q.S - 1), s1 = q.of(b - 1, s0, q.S - 1);
+    const int64_t s0 = q.of_wave(a, 0, q.S - 1), s1 = q.of_wave(b - 1, s0, q.S - 1);
     const float up = g[0];
-    for (int64_t i = a + threadIdx.x; i < b; i += 256) {
-        const int64_t s = q.of(i, s0, s1);
-        const bool live = i >= q.lo(s) && i < q.hi(s) && (!mask || mask[i]);
-        float v = 0.0f;
-        if (live) {
-            v = weight[s] * up;
-            if (slope) v = v * slope[i];
+    auto put = [&](int64_t i, auto width, float w0, int64_t lo, int64_t hi) {       // width items of one sequence [lo, hi)
+        constexpr int W = decltype(width)::value;
+        Vec<float, W> x, y;
+        Vec<uint8_t, W> on;
+        if constexpr (SLOPE) x = *reinterpret_cast<const Vec<float, W>*>(slope + i);
+        if constexpr (MASK) on = *reinterpret_cast<const Vec<uint8_t, W>*>(mask + i);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const bool live = i + k >= lo && i + k < hi && (!MASK || on.v[k]);
+            y.v[k] = live ? (SLOPE ? w0 * x.v[k] : w0) : 0.0f;
         }
-        dl[i] = v;
+        *reinterpret_cast<Vec<float, W>*>(dl + i) = y;
+    };
+    if (s0 == s1) {
+        const float w0 = weight[s0] * up;
+        const int64_t lo = q.lo(s0), hi = q.hi(s0);
+        for (int64_t i = a + 4 * (int)threadIdx.x; i < b; i += 1024) {
+            if (i + 4 <= b) put(i, std::integral_constant<int, 4>{}, w0, lo, hi);
+            else for (int64_t k = i; k < b; ++k) put(k, std::integral_constant<int, 1>{}, w0, lo, hi);
+        }
+    } else {
+        for (int64_t i = a + threadIdx.x; i < b; i += 256) {
+            const int64_t s = q.of(i, s0, s1);
+            put(i, std::integral_constant<int, 1>{}, weight[s] * up, q.lo(s), q.hi(s));
+        }
     }
 }
 
@@ -298,6 +353,15 @@ static int launch_sequence_loss(const Sequences& q, const F& f, void* workspace,
     return GM_OK;
 }
 
+// fn(b0, b1, ...) with each flag as an integral constant
+template <class Fn> static inline int with_flags(bool a, Fn&& fn) { return a ? fn(std::true_type{}) : fn(std::false_type{}); }
+template <class Fn> static inline int with_flags(bool a, bool b, Fn&& fn) {
+    return with_flags(b, [&](auto y) { return a ? fn(std::true_type{}, y) : fn(std::false_type{}, y); });
+}
+template <class Fn> static inline int with_flags(bool a, bool b, bool c, Fn&& fn) {
+    return with_flags(b, c, [&](auto y, auto z) { return a ? fn(std::true_type{}, y, z) : fn(std::false_type{}, y, z); });
+}
+
 }  // namespace gm
 
 using namespace gm;
@@ -322,10 +386,12 @@ extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, c
     GM_REQUIRE(kl_coef - kl_coef == 0.0f, "kl_coef is not finite");
     hipStream_t s = as_stream(stream);
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
-    const PolicyTerm f{log_prob, old_log_prob, advantage, ref_log_prob, mask, 1.0f - clip_low, 1.0f + clip_high, kl_coef,
-                       offsets != nullptr, slope};
-    return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece) {
-        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, loss, stats, weight);
+    return with_flags(mask != nullptr, ref_log_prob != nullptr, offsets == nullptr, [&](auto m, auto r, auto item) {
+        const PolicyTerm<decltype(m)::value, decltype(r)::value, decltype(item)::value> f{
+            log_prob, old_log_prob, advantage, ref_log_prob, mask, 1.0f - clip_low, 1.0f + clip_high, kl_coef, slope};
+        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece) {
+            hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, loss, stats, weight);
+        });
     });
 }
 
@@ -341,10 +407,12 @@ extern "C" int gm_preference_loss_fwd(int64_t M, int64_t P, const float* log_pro
                "0 < beta and 0 <= label_smoothing <= 0.5");
     hipStream_t s = as_stream(stream);
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
-    const PreferenceTerm f{log_prob, ref_log_prob, mask};
-    return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<2>* whole, Sums<2>* piece) {
-        hipLaunchKernelGGL(k_preference_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, (double)beta, (double)label_smoothing, average,
-                           whole, piece, loss, rewards, weight);
+    return with_flags(mask != nullptr, [&](auto m) {
+        const PreferenceTerm<decltype(m)::value> f{log_prob, ref_log_prob, mask};
+        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<2>* whole, Sums<2>* piece) {
+            hipLaunchKernelGGL(k_preference_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, (double)beta, (double)label_smoothing, average,
+                               whole, piece, loss, rewards, weight);
+        });
     });
 }
 
@@ -355,8 +423,10 @@ extern "C" int gm_sequence_loss_bwd(int64_t M, int64_t S, const float* slope, co
     GM_REQUIRE(weight && g && dlog_prob, "bad arguments");
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
     const int64_t chunk = chunk_items(M);
-    hipLaunchKernelGGL(k_sequence_spread, dim3((unsigned)((M + chunk - 1) / chunk)), dim3(256), 0, as_stream(stream), q, chunk, slope,
-                       mask, weight, g, dlog_prob);
-    GM_LAUNCH_CHECK();
-    return GM_OK;
+    return with_flags(slope != nullptr, mask != nullptr, [&](auto sl, auto m) -> int {
+        hipLaunchKernelGGL((k_sequence_spread<decltype(sl)::value, decltype(m)::value>), dim3((unsigned)((M + chunk - 1) / chunk)), dim3(256), 0,
+                           as_stream(stream), q, chunk, slope, mask, weight, g, dlog_prob);
+        GM_LAUNCH_CHECK();
+        return GM_OK;
+    });
 }

@@ -80,6 +80,15 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// exp(x) within about two units in the last place: 2^(x log2 e), with the product's rounding error (|x| 2^-24 relative, were it
+// left) put back as a factor.  exp(-inf) = 0, overflow gives infinity, NaN stays NaN.
+__device__ __forceinline__ float exp_any(float x) {
+    x = x < -120.0f ? -120.0f : x > 100.0f ? 100.0f : x;       // 2^-173 and 2^144: what lies beyond is 0 or infinite anyway
+    const float t = x * 1.44269502f;
+    const float lo = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
+    return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(lo, 0.693147182f, 1.0f);
+}
+
 // orders one wave's LDS accesses among its lanes: nothing moves across it (the hardware keeps a wave's LDS order)
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
