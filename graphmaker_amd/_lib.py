@@ -132,11 +132,17 @@ F32 = C.c_float
 _functions = {}
 
 
-def launch(name, device, *args):
-    """One call of an entry point in _SIGNATURES on `device`'s current stream, whatever device is current."""
+def function(name):
+    """An entry point in _SIGNATURES, as a callable of plain numbers and addresses."""
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(load(), name)
+    return fn
+
+
+def launch(name, device, *args):
+    """One call of an entry point in _SIGNATURES on `device`'s current stream, whatever device is current."""
+    fn = function(name)
     index = device.index
     if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))

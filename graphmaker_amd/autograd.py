@@ -221,7 +221,7 @@ class _UpdateBlock(torch.autograd.Function):
         da = torch.empty_like(a)
         dgb = torch.empty((2, N), dtype=torch.float32, device=dev)
         if N > LAYERNORM_BWD_MAX:
-            _layer_norm_bwd(g, a, mean, rstd, gamma, da, dgb[0], dgb[1])
+            _layer_norm_bwd(g, a, M, N, 0, mean.data_ptr(), rstd.data_ptr(), gamma, 0, da, dgb[0], dgb[1])
             L.call("gm_relu_bwd", I64(a.numel()), ptr(da), ptr(a), ptr(da), stream_ptr())
             dx, dW, db = _linear_backward(x, W, da, (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]))
             return dx, dW, db, dgb[0], dgb[1], None
@@ -466,6 +466,19 @@ def dropout(x, p, state):
 
 
 # ------------------------------------------------------------------ wider models and fine-tuning
+# A small call costs what its Python costs (the kernels of a short sequence take a few microseconds, the autograd engine's
+# round trip some 30): contiguous tensors are used as they are, without a view, and backward passes get their sizes as numbers.
+def _gradient(fn):
+    """A backward pass without a second derivative: an error for who differentiates the gradient (create_graph), and no wrapper
+    around the call otherwise."""
+    checked = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
+
+
 def _on_gpu(t, what):
     if not t.is_cuda:
         raise L.GraphMakerHipError(f"{what}: graphmaker_amd runs on a ROCm device only (tensor is on {t.device})")
@@ -485,7 +498,9 @@ def _row_dtype(t, what):
 
 
 def _rows(t, width):
-    """(tensor, leading dimension) of t as rows of `width` elements; a view where its strides allow one, else a copy."""
+    """(tensor, leading dimension) of t as rows of `width` elements at its address; a copy only where its strides need one."""
+    if t.is_contiguous():
+        return t, width
     t = t.reshape(-1, width)
     if t.shape[0] == 0 or (t.shape[0] == 1 and (width == 1 or t.stride(1) == 1)):
         return t, width
@@ -496,44 +511,42 @@ def _rows(t, width):
 
 def _index(t, what, device):
     """(contiguous tensor, 1 if int64) of an index argument."""
-    if t.dtype != torch.int64 and t.dtype != torch.int32:
+    i64 = t.dtype == torch.int64
+    if not i64 and t.dtype != torch.int32:
         raise TypeError(f"{what}: expected int32 or int64, got {t.dtype}")
-    return _c(_same_device(t, what, device)), int(t.dtype == torch.int64)
+    return _c(_same_device(t, what, device)), int(i64)
 
 
-def _records(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _at(t):
+    return t.data_ptr() if t is not None else None
 
 
-def _token_embedding_fwd(weight, tokens, i64, scale):
-    C, w = weight.shape
+def _token_embedding_fwd(weight, tokens, args):
+    n, C, w, i64, code, scale, _, _ = args
     table, ldw = _rows(weight, w)
-    out = torch.empty(tokens.shape + (w,), dtype=weight.dtype, device=weight.device)
-    L.launch("gm_token_embedding_fwd", weight.device, tokens.numel(), C, w, tokens.data_ptr(), i64, table.data_ptr(), ldw,
-             L.DTYPES[weight.dtype], scale, out.data_ptr(), w)
+    out = torch.empty((*tokens.shape, w), dtype=weight.dtype, device=weight.device)
+    L.launch("gm_token_embedding_fwd", weight.device, n, C, w, tokens.data_ptr(), i64, table.data_ptr(), ldw, code, scale, out.data_ptr(), w)
     return out
 
 
 class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, tokens, i64, scale, padding):
+    def forward(ctx, weight, tokens, args):
         ctx.save_for_backward(tokens)
-        ctx.args = (weight.shape, i64, scale, padding)
-        return _token_embedding_fwd(weight, tokens, i64, scale)
+        ctx.args = args
+        return _token_embedding_fwd(weight, tokens, args)
 
-    @staticmethod
-    @once_differentiable
+    @_gradient
     def backward(ctx, g):
         (tokens,) = ctx.saved_tensors
-        (C, w), i64, scale, padding = ctx.args
-        n, dev = tokens.numel(), g.device
-        g2, ldg = _rows(g, w)
+        n, C, w, i64, code, scale, padding, need = ctx.args
+        dev = g.device
+        g, ldg = _rows(g, w)
         dW = torch.empty((C, w), dtype=g.dtype, device=dev)
-        need = L.load().gm_token_embedding_bwd_workspace_bytes(n, C, w)
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        L.launch("gm_token_embedding_bwd", dev, n, C, w, tokens.data_ptr(), i64, padding, g2.data_ptr(), ldg, L.DTYPES[g.dtype], scale,
-                 dW.data_ptr(), w, ws.data_ptr(), need)
-        return dW, None, None, None, None
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        L.launch("gm_token_embedding_bwd", dev, n, C, w, tokens.data_ptr(), i64, padding, g.data_ptr(), ldg, code, scale, dW.data_ptr(), w,
+                 ws.data_ptr(), need)
+        return dW, None, None
 
 
 def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
@@ -541,11 +554,11 @@ def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
     of any shape.  The gradient sums each row's tokens in ascending position (no atomics: the same bits on every run) and
     leaves row padding_idx zero, as nn.Embedding does.  Tokens are not read on the host: one outside [0, C) gives a row of
     NaN and adds to no gradient; ops.check_index_range(tokens, C, "tokens") is the check that raises."""
-    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+    if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"token_embedding: weight must be (C, w) with C, w > 0, got {tuple(weight.shape)}")
-    _row_dtype(weight, "weight")
+    code = _row_dtype(weight, "weight")
     tokens, i64 = _index(tokens, "tokens", weight.device)
-    C = weight.shape[0]
+    C, w = weight.shape
     if padding_idx is None:
         padding = -1
     else:
@@ -553,58 +566,56 @@ def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
             raise ValueError(f"token_embedding: padding_idx {padding_idx} is outside the {C} rows of weight")
         padding = int(padding_idx) % C
     _on_gpu(weight, "weight")
-    if _records(weight):
-        return _TokenEmbedding.apply(weight, tokens, i64, float(scale), padding)
-    return _token_embedding_fwd(weight, tokens, i64, float(scale))
+    n = tokens.numel()
+    if weight.requires_grad and torch.is_grad_enabled():
+        need = L.function("gm_token_embedding_bwd_workspace_bytes")(n, C, w)
+        return _TokenEmbedding.apply(weight, tokens, (n, C, w, i64, code, float(scale), padding, need))
+    return _token_embedding_fwd(weight, tokens, (n, C, w, i64, code, float(scale), padding, 0))
 
 
-def _layer_norm_fwd(x, gamma, beta, eps, stats):
-    N, dev = x.shape[-1], x.device
-    x2, ldx = _rows(x, N)
-    M = x2.shape[0]
+def _layer_norm_fwd(x, gamma, beta, args, stats):
+    M, N, code, wcode, eps = args
+    dev = x.device
+    rows, ldx = _rows(x, N)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    st = torch.empty((2, M), dtype=torch.float32, device=dev) if stats else None
-    at = st.data_ptr() if stats else None
-    wt = gamma if gamma is not None else beta
-    L.launch("gm_layer_norm_fwd", dev, M, N, x2.data_ptr(), ldx, L.DTYPES[x.dtype], gamma.data_ptr() if gamma is not None else None,
-             beta.data_ptr() if beta is not None else None, L.DTYPES[wt.dtype] if wt is not None else 0, eps, y.data_ptr(), N, at,
-             at + 4 * M if stats and M else None)
-    return y, x2, st
+    st = torch.empty(2 * M, dtype=torch.float32, device=dev) if stats else None
+    at = _at(st)
+    L.launch("gm_layer_norm_fwd", dev, M, N, rows.data_ptr(), ldx, code, _at(gamma), _at(beta), wcode, eps, y.data_ptr(), N, at,
+             at + 4 * M if at else at)
+    return y, rows, st
 
 
-def _layer_norm_bwd(g, x2, mean, rstd, gamma, dx, dgamma, dbeta):
-    """gm_layer_norm_bwd over rows x2 (M, N); dx, dgamma, dbeta: outputs or None."""
-    M, N = x2.shape
-    x2, ldx = _rows(x2, N)
-    g2, ldg = _rows(g, N)
-    wt = next((t for t in (gamma, dgamma, dbeta) if t is not None), None)
-    need = L.load().gm_layer_norm_bwd_workspace_bytes(M, N) if dgamma is not None or dbeta is not None else 0
-    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
-
-    def at(t):
-        return t.data_ptr() if t is not None else None
-
-    L.launch("gm_layer_norm_bwd", x2.device, M, N, g2.data_ptr(), ldg, x2.data_ptr(), ldx, L.DTYPES[x2.dtype], at(mean), at(rstd), at(gamma),
-             L.DTYPES[wt.dtype] if wt is not None else 0, at(dx), N, at(dgamma), at(dbeta), at(ws), need)
+def _layer_norm_bwd(g, rows, M, N, code, mean, rstd, gamma, wcode, dx, dgamma, dbeta):
+    """gm_layer_norm_bwd over the M rows of N of x; mean, rstd: addresses; dx, dgamma, dbeta: outputs or None."""
+    dev = rows.device
+    rows, ldx = _rows(rows, N)
+    g, ldg = _rows(g, N)
+    need = L.function("gm_layer_norm_bwd_workspace_bytes")(M, N) if dgamma is not None or dbeta is not None else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    L.launch("gm_layer_norm_bwd", dev, M, N, g.data_ptr(), ldg, rows.data_ptr(), ldx, code, mean, rstd, _at(gamma), wcode, _at(dx), N,
+             _at(dgamma), _at(dbeta), _at(ws), need)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, eps):
-        y, x2, st = _layer_norm_fwd(x, gamma, beta, eps, True)
-        ctx.save_for_backward(x2, st, gamma)
-        ctx.shape, ctx.beta_dtype = x.shape, beta.dtype if beta is not None else None
+    def forward(ctx, x, gamma, beta, args):
+        y, rows, st = _layer_norm_fwd(x, gamma, beta, args, True)
+        ctx.save_for_backward(rows, st, gamma)
+        ctx.args = args
+        ctx.shape = x.shape
+        ctx.weight_dtypes = (gamma.dtype if gamma is not None else None, beta.dtype if beta is not None else None)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_gradient
     def backward(ctx, g):
-        x2, st, gamma = ctx.saved_tensors
-        N, dev, need = x2.shape[1], x2.device, ctx.needs_input_grad
-        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need[0] else None
-        dgamma = torch.empty(N, dtype=gamma.dtype, device=dev) if need[1] else None
-        dbeta = torch.empty(N, dtype=ctx.beta_dtype, device=dev) if need[2] else None
-        _layer_norm_bwd(g, x2, st[0], st[1], gamma, dx, dgamma, dbeta)
+        rows, st, gamma = ctx.saved_tensors
+        M, N, code, wcode, _ = ctx.args
+        dev, need, types = g.device, ctx.needs_input_grad, ctx.weight_dtypes
+        dx = torch.empty(ctx.shape, dtype=g.dtype, device=dev) if need[0] else None
+        dgamma = torch.empty(N, dtype=types[0], device=dev) if need[1] else None
+        dbeta = torch.empty(N, dtype=types[1], device=dev) if need[2] else None
+        at = st.data_ptr()
+        _layer_norm_bwd(g, rows, M, N, code, at, at + 4 * M, gamma, wcode, dx, dgamma, dbeta)
         return dx, dgamma, dbeta, None
 
 
@@ -612,65 +623,65 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension, of any width, in x's type (float32, bfloat16,
     float16).  gamma and beta (N,): x's type or float32, both the same; None: 1 and 0.  Statistics are float32 about the mean,
     the variance that of the differences from it."""
-    if x.dim() == 0 or x.shape[-1] == 0:
+    N = x.shape[-1] if x.dim() else 0
+    if N == 0:
         raise ValueError(f"layer_norm: x must have a last dimension of at least 1, got {tuple(x.shape)}")
-    _row_dtype(x, "x")
+    code = _row_dtype(x, "x")
+    wcode, records = code, x.requires_grad
     for t, what in ((gamma, "gamma"), (beta, "beta")):
         if t is None:
             continue
-        if t.shape != x.shape[-1:]:
-            raise ValueError(f"layer_norm: {what} is {tuple(t.shape)}, x's rows have {x.shape[-1]} columns")
+        if t.dim() != 1 or t.numel() != N:
+            raise ValueError(f"layer_norm: {what} is {tuple(t.shape)}, x's rows have {N} columns")
         if t.dtype != x.dtype and t.dtype != torch.float32:
             raise TypeError(f"layer_norm: {what} is {t.dtype}, expected {x.dtype} or float32")
         _same_device(t, what, x.device)
+        wcode = L.DTYPES[t.dtype]
+        records = records or t.requires_grad
     if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
         raise TypeError(f"layer_norm: gamma is {gamma.dtype} and beta is {beta.dtype}")
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
     _on_gpu(x, "x")
     gamma, beta = (t if t is None else _c(t) for t in (gamma, beta))
-    if _records(x, gamma, beta):
-        return _LayerNorm.apply(x, gamma, beta, float(eps))
-    return _layer_norm_fwd(x, gamma, beta, float(eps), False)[0]
+    args = (x.numel() // N, N, code, wcode, float(eps))
+    if records and torch.is_grad_enabled():
+        return _LayerNorm.apply(x, gamma, beta, args)
+    return _layer_norm_fwd(x, gamma, beta, args, False)[0]
 
 
-def _class_log_prob_fwd(logits, classes, i64, ignore_index, stats):
-    V, dev = logits.shape[-1], logits.device
-    x2, ldx = _rows(logits, V)
-    M = x2.shape[0]
-    lp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    code = L.DTYPES[logits.dtype]
-    st = None
-    if stats:
-        floats = L.load().gm_class_log_prob_stats_floats(M, V, code)
-        st = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-    need = L.load().gm_class_log_prob_workspace_bytes(M, V, code)
+def _class_log_prob_fwd(logits, classes, args, stats):
+    M, V, code, i64, ignore_index = args
+    dev = logits.device
+    rows, ldx = _rows(logits, V)
+    lp = torch.empty(classes.shape, dtype=torch.float32, device=dev)
+    floats = L.function("gm_class_log_prob_stats_floats")(M, V, code) if stats else 0
+    st = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    need = L.function("gm_class_log_prob_workspace_bytes")(M, V, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    L.launch("gm_class_log_prob_fwd", dev, M, V, x2.data_ptr(), ldx, code, classes.data_ptr(), i64, ignore_index,
-             lp.data_ptr(), st.data_ptr() if st is not None else None, ws.data_ptr() if need else None, need)
-    return lp, x2, st
+    L.launch("gm_class_log_prob_fwd", dev, M, V, rows.data_ptr(), ldx, code, classes.data_ptr(), i64, ignore_index, lp.data_ptr(), _at(st),
+             _at(ws), need)
+    return lp, rows, ldx, st
 
 
 class _ClassLogProb(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, classes, i64, ignore_index):
-        lp, x2, st = _class_log_prob_fwd(logits, classes, i64, ignore_index, True)
-        ctx.save_for_backward(x2, classes, st)
-        ctx.args = (logits.shape, i64, ignore_index)
+    def forward(ctx, logits, classes, args):
+        lp, rows, ctx.ldx, st = _class_log_prob_fwd(logits, classes, args, True)
+        ctx.save_for_backward(rows, classes, st)
+        ctx.args = args
+        ctx.shape = logits.shape
         return lp
 
-    @staticmethod
-    @once_differentiable
+    @_gradient
     def backward(ctx, g):
-        x2, classes, st = ctx.saved_tensors
-        shape, i64, ignore_index = ctx.args
-        M, V = x2.shape
-        x2, ldx = _rows(x2, V)
+        rows, classes, st = ctx.saved_tensors
+        M, V, code, i64, ignore_index = ctx.args
         g = _c(g)
-        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device)
-        L.launch("gm_class_log_prob_bwd", x2.device, M, V, g.data_ptr(), x2.data_ptr(), ldx, L.DTYPES[x2.dtype], classes.data_ptr(), i64,
-                 ignore_index, st.data_ptr() if st is not None else None, dx.data_ptr(), V)
-        return dx, None, None, None
+        dx = torch.empty(ctx.shape, dtype=rows.dtype, device=g.device)
+        L.launch("gm_class_log_prob_bwd", g.device, M, V, g.data_ptr(), rows.data_ptr(), ctx.ldx, code, classes.data_ptr(), i64, ignore_index,
+                 _at(st), dx.data_ptr(), V)
+        return dx, None, None
 
 
 def class_log_prob(logits, classes, ignore_index=-100):
@@ -678,16 +689,18 @@ def class_log_prob(logits, classes, ignore_index=-100):
     bfloat16 or float16, classes int32 or int64.  A row whose class is ignore_index has log-probability 0 and a zero gradient,
     whatever its logits hold; any other class outside [0, V) gives NaN in both (classes are not read on the host).  A row
     whose upstream gradient is exactly 0 gets a zero gradient too."""
-    if logits.dim() == 0 or logits.shape[-1] == 0:
+    V = logits.shape[-1] if logits.dim() else 0
+    if V == 0:
         raise ValueError(f"class_log_prob: logits must have a last dimension of at least 1, got {tuple(logits.shape)}")
     if classes.shape != logits.shape[:-1]:
         raise ValueError(f"class_log_prob: classes is {tuple(classes.shape)}, logits is {tuple(logits.shape)}")
-    _row_dtype(logits, "logits")
+    code = _row_dtype(logits, "logits")
     classes, i64 = _index(classes, "classes", logits.device)
     _on_gpu(logits, "logits")
-    if _records(logits):
-        return _ClassLogProb.apply(logits, classes, i64, int(ignore_index))
-    return _class_log_prob_fwd(logits, classes, i64, int(ignore_index), False)[0]
+    args = (classes.numel(), V, code, i64, int(ignore_index))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _ClassLogProb.apply(logits, classes, args)
+    return _class_log_prob_fwd(logits, classes, args, False)[0]
 
 
 def _items(t, what, like=None):
@@ -723,47 +736,53 @@ def _offsets(offsets, device):
     return _index(offsets, "offsets", device)
 
 
-def _sequence_loss_bwd(g, slope, mask, offsets, i64, weight, shape):
+def _sequence_buffer(M, S, slopes, dev):
+    """(buffer, addresses of the S weights, `slopes` slopes and the workspace in it, workspace bytes).  What a loss keeps for its
+    backward pass and what it works in share one allocation."""
+    need = L.function("gm_sequence_loss_workspace_bytes")(M, S)
+    head = (4 * (S + slopes) + 15) // 16 * 16
+    buf = torch.empty(head + need, dtype=torch.uint8, device=dev)
+    at = buf.data_ptr()
+    return buf, at, at + 4 * S if slopes else None, at + head, need
+
+
+def _sequence_loss_bwd(g, buf, M, S, has_slope, mask, offsets, i64, shape):
     out = torch.empty(shape, dtype=torch.float32, device=g.device)
-    L.launch("gm_sequence_loss_bwd", g.device, out.numel(), weight.numel(), slope.data_ptr() if slope is not None else None,
-             mask.data_ptr() if mask is not None else None, offsets.data_ptr() if offsets is not None else None, i64, weight.data_ptr(),
-             g.data_ptr(), out.data_ptr())
+    at = buf.data_ptr()
+    L.launch("gm_sequence_loss_bwd", g.device, M, S, at + 4 * S if has_slope else None, _at(mask), _at(offsets), i64, at, g.data_ptr(),
+             out.data_ptr())
     return out
 
 
-def _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, clip_low, clip_high, kl_coef, by_sequence, grad):
-    dev, M = lp.device, lp.numel()
-    S = offsets.numel() - 1 if offsets is not None else 1
+def _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, grad):
+    M, S, i64, clip_low, clip_high, kl_coef, by_sequence = args
+    dev = lp.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
     stats = torch.empty(4, dtype=torch.float32, device=dev)
-    slope = torch.empty(M, dtype=torch.float32, device=dev) if grad else None
-    weight = torch.empty(S, dtype=torch.float32, device=dev) if grad else None
-    need = L.load().gm_sequence_loss_workspace_bytes(M, S)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-
-    def at(t):
-        return t.data_ptr() if t is not None else None
-
-    L.launch("gm_policy_loss_fwd", dev, M, S, at(lp), at(old), at(adv), at(ref), at(mask), at(offsets), i64, clip_low, clip_high, kl_coef,
-             by_sequence, loss.data_ptr(), stats.data_ptr(), at(slope), at(weight), ws.data_ptr(), need)
-    return loss, stats, slope, weight
+    buf, weight, slope, ws, need = _sequence_buffer(M, S, M if grad else 0, dev)
+    L.launch("gm_policy_loss_fwd", dev, M, S, lp.data_ptr(), old.data_ptr(), adv.data_ptr(), _at(ref), _at(mask), _at(offsets), i64, clip_low,
+             clip_high, kl_coef, by_sequence, loss.data_ptr(), stats.data_ptr(), slope, weight, ws, need)
+    return loss, stats, buf
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, lp, old, adv, ref, mask, offsets, i64, *args):
-        loss, stats, slope, weight = _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, *args, True)
-        ctx.save_for_backward(slope, mask, offsets, weight)
-        ctx.args = (i64, lp.shape)
+    def forward(ctx, lp, old, adv, ref, mask, offsets, args):
+        loss, stats, buf = _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, True)
+        ctx.save_for_backward(buf, mask, offsets)
+        ctx.args = args
+        ctx.shape = lp.shape
         ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
         return loss, stats
 
-    @staticmethod
-    @once_differentiable
+    @_gradient
     def backward(ctx, g, _stats):
-        slope, mask, offsets, weight = ctx.saved_tensors
-        i64, shape = ctx.args
-        return (_sequence_loss_bwd(g, slope, mask, offsets, i64, weight, shape),) + (None,) * 10
+        if g is None:
+            return (None,) * 7
+        buf, mask, offsets = ctx.saved_tensors
+        M, S, i64 = ctx.args[:3]
+        return _sequence_loss_bwd(g, buf, M, S, M > 0, mask, offsets, i64, ctx.shape), None, None, None, None, None, None
 
 
 def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, ref_log_prob=None, clip_low=0.2, clip_high=0.2,
@@ -783,16 +802,17 @@ def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, r
     old = _items(old_log_prob, "old_log_prob", log_prob)
     ref = _items(ref_log_prob, "ref_log_prob", log_prob) if ref_log_prob is not None else None
     mask = _mask(mask, log_prob)
-    i64 = 0
+    i64, S = 0, 1
     if offsets is None:
         adv = _items(advantage, "advantage", log_prob)
     else:
         offsets, i64 = _offsets(offsets, log_prob.device)
+        S = offsets.numel() - 1
         adv = _items(advantage, "advantage")
         _same_device(adv, "advantage", log_prob.device)
         _constant(advantage, "advantage")
-        if advantage.shape != (offsets.numel() - 1,):
-            raise ValueError(f"advantage is {tuple(advantage.shape)}, offsets border {offsets.numel() - 1} sequences")
+        if advantage.dim() != 1 or advantage.numel() != S:
+            raise ValueError(f"advantage is {tuple(advantage.shape)}, offsets border {S} sequences")
     if reduction not in ("token", "sequence"):
         raise ValueError(f"reduction: expected 'token' or 'sequence', got {reduction!r}")
     if reduction == "sequence" and offsets is None:
@@ -804,40 +824,41 @@ def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, r
     if kl_coef - kl_coef != 0.0:
         raise ValueError(f"kl_coef must be finite, got {kl_coef}")
     _on_gpu(log_prob, "log_prob")
-    args = (float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
-    if _records(log_prob):
-        return _PolicyLoss.apply(lp, old, adv, ref, mask, offsets, i64, *args)
-    return _policy_loss_fwd(lp, old, adv, ref, mask, offsets, i64, *args, False)[:2]
+    args = (lp.numel(), S, i64, float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
+    if log_prob.requires_grad and torch.is_grad_enabled():
+        return _PolicyLoss.apply(lp, old, adv, ref, mask, offsets, args)
+    return _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, False)[:2]
 
 
-def _preference_loss_fwd(lp, ref, mask, offsets, i64, beta, smoothing, average, grad):
-    dev, M, S = lp.device, lp.numel(), offsets.numel() - 1
+def _preference_loss_fwd(lp, ref, mask, offsets, args):
+    M, S, i64, beta, smoothing, average = args
+    dev = lp.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
     rewards = torch.empty(S, dtype=torch.float32, device=dev)
-    weight = torch.empty(S, dtype=torch.float32, device=dev) if grad else None
-    need = L.load().gm_sequence_loss_workspace_bytes(M, S)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    L.launch("gm_preference_loss_fwd", dev, M, S // 2, lp.data_ptr(), ref.data_ptr(), mask.data_ptr() if mask is not None else None,
-             offsets.data_ptr(), i64, beta, smoothing, average, loss.data_ptr(), rewards.data_ptr(),
-             weight.data_ptr() if grad else None, ws.data_ptr(), need)
-    return loss, rewards, weight
+    buf, weight, _, ws, need = _sequence_buffer(M, S, 0, dev)
+    L.launch("gm_preference_loss_fwd", dev, M, S // 2, lp.data_ptr(), ref.data_ptr(), _at(mask), offsets.data_ptr(), i64, beta, smoothing, average,
+             loss.data_ptr(), rewards.data_ptr(), weight, ws, need)
+    return loss, rewards, buf
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, lp, ref, mask, offsets, i64, *args):
-        loss, rewards, weight = _preference_loss_fwd(lp, ref, mask, offsets, i64, *args, True)
-        ctx.save_for_backward(mask, offsets, weight)
-        ctx.args = (i64, lp.shape)
+    def forward(ctx, lp, ref, mask, offsets, args):
+        loss, rewards, buf = _preference_loss_fwd(lp, ref, mask, offsets, args)
+        ctx.save_for_backward(buf, mask, offsets)
+        ctx.args = args
+        ctx.shape = lp.shape
         ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
         return loss, rewards
 
-    @staticmethod
-    @once_differentiable
+    @_gradient
     def backward(ctx, g, _rewards):
-        mask, offsets, weight = ctx.saved_tensors
-        i64, shape = ctx.args
-        return (_sequence_loss_bwd(g, None, mask, offsets, i64, weight, shape),) + (None,) * 7
+        if g is None:
+            return (None,) * 5
+        buf, mask, offsets = ctx.saved_tensors
+        M, S, i64 = ctx.args[:3]
+        return _sequence_loss_bwd(g, buf, M, S, False, mask, offsets, i64, ctx.shape), None, None, None, None
 
 
 def preference_loss(log_prob, ref_log_prob, offsets, *, mask=None, beta=0.1, label_smoothing=0.0, average=False):
@@ -852,12 +873,13 @@ def preference_loss(log_prob, ref_log_prob, offsets, *, mask=None, beta=0.1, lab
     ref = _items(ref_log_prob, "ref_log_prob", log_prob)
     mask = _mask(mask, log_prob)
     offsets, i64 = _offsets(offsets, log_prob.device)
-    if offsets.numel() % 2 == 0:
-        raise ValueError(f"offsets border {offsets.numel() - 1} sequences: an even number makes pairs")
+    S = offsets.numel() - 1
+    if S % 2:
+        raise ValueError(f"offsets border {S} sequences: an even number makes pairs")
     if not 0.0 < beta < float("inf") or not 0.0 <= label_smoothing <= 0.5:
         raise ValueError(f"0 < beta and 0 <= label_smoothing <= 0.5, got {beta}, {label_smoothing}")
     _on_gpu(log_prob, "log_prob")
-    args = (float(beta), float(label_smoothing), int(bool(average)))
-    if _records(log_prob):
-        return _PreferenceLoss.apply(lp, ref, mask, offsets, i64, *args)
-    return _preference_loss_fwd(lp, ref, mask, offsets, i64, *args, False)[:2]
+    args = (lp.numel(), S, i64, float(beta), float(label_smoothing), int(bool(average)))
+    if log_prob.requires_grad and torch.is_grad_enabled():
+        return _PreferenceLoss.apply(lp, ref, mask, offsets, args)
+    return _preference_loss_fwd(lp, ref, mask, offsets, args)[:2]
