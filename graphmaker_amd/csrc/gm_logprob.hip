@@ -140,7 +140,14 @@ k_log_prob_held_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
 }
 
 // ---- long
-constexpr int LONG_PIECES = 4;                           // pieces of 16 bytes a thread has in flight
+constexpr int READ_PIECES = 2;                           // pieces of 16 bytes a thread works on while it loads as many
+constexpr int LONG_PIECES = 4;                           // pieces of the gradient a thread has in flight
+// Elements of a row in front of its first 16-byte boundary.  The gradient of a long row is written from there: 4095 odd rows
+// of 50,021 bf16 took 184 us in pieces that straddle boundaries and take 150 us so.  The forward's pieces count from the
+// row's start instead: which elements a thread adds, and so the bits of the sum, must not depend on where a row lies.
+template <class T> __device__ __forceinline__ int head_of(const T* row) {
+    return (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+}
 constexpr float LOWEST = -3.40282347e+38f;
 
 // running maximum and sum of exp(x - maximum)
@@ -182,26 +189,31 @@ k_log_prob_long(int64_t M, int N, int span, const T* __restrict__ X, int64_t ldx
         int j = blockIdx.y * span;
         const int end = N - j < span ? N : j + span;
         Running run;
-        for (; j + LONG_PIECES * STEP <= end; j += LONG_PIECES * STEP) {
-            Vec<T, V> r[LONG_PIECES];
+        if (j + READ_PIECES * STEP <= end) {
+            Vec<T, V> next[READ_PIECES];
 #pragma unroll
-            for (int u = 0; u < LONG_PIECES; ++u) r[u] = *reinterpret_cast<const Vec<T, V>*>(row + j + u * STEP + threadIdx.x * V);
-            float x[LONG_PIECES * V];
+            for (int u = 0; u < READ_PIECES; ++u) next[u] = *reinterpret_cast<const Vec<T, V>*>(row + j + u * STEP + threadIdx.x * V);
+            for (; j + READ_PIECES * STEP <= end; j += READ_PIECES * STEP) {
+                Vec<T, V> now[READ_PIECES];
 #pragma unroll
-            for (int u = 0; u < LONG_PIECES; ++u)
+                for (int u = 0; u < READ_PIECES; ++u) now[u] = settled(next[u]);
+                const int ahead = j + 2 * READ_PIECES * STEP <= end ? j + READ_PIECES * STEP : j;
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[u * V + i] = to_f32(r[u].v[i]);
-            run.add(x);
+                for (int u = 0; u < READ_PIECES; ++u) next[u] = *reinterpret_cast<const Vec<T, V>*>(row + ahead + u * STEP + threadIdx.x * V);
+                __builtin_amdgcn_sched_barrier(0);
+                float x[READ_PIECES * V];
+#pragma unroll
+                for (int u = 0; u < READ_PIECES; ++u)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[u * V + i] = to_f32(now[u].v[i]);
+                run.add(x);
+            }
         }
-        if (j < end) {                                   // the rest, less than LONG_PIECES steps: loads where the row has any
-            Vec<T, V> r[LONG_PIECES];
+        for (; j < end; j += STEP) {                     // the rest: fewer steps than READ_PIECES, and one that ends inside
+            const Vec<T, V> r = load_vec<T, V, true>(row, j + threadIdx.x * V, end);
+            float x[V];
 #pragma unroll
-            for (int u = 0; u < LONG_PIECES; ++u) r[u] = load_vec<T, V, true>(row, j + u * STEP + threadIdx.x * V, end);
-            float x[LONG_PIECES * V];
-#pragma unroll
-            for (int u = 0; u < LONG_PIECES; ++u)
-#pragma unroll
-                for (int i = 0; i < V; ++i) x[u * V + i] = or_neg_inf(to_f32(r[u].v[i]), j + u * STEP + (int)threadIdx.x * V + i < end);
+            for (int i = 0; i < V; ++i) x[i] = or_neg_inf(to_f32(r.v[i]), j + (int)threadIdx.x * V + i < end);
             run.add(x);
         }
 #pragma unroll
@@ -246,7 +258,7 @@ k_log_prob_join(int N, int parts, const float2* __restrict__ part, const T* __re
     }
 }
 
-// columns [blockIdx.y * span, + span) of a row
+// columns head + [blockIdx.y * span, + span) of a row, span = LONG_PIECES steps, the head with the first
 template <class T>
 __global__ void __launch_bounds__(256)
 k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore,
@@ -259,21 +271,27 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
         const float scale = c >= 0 && c < N ? -gu : __builtin_nanf("");
         const T* row = X + m * ldx;
         T* out = dX + m * lddx;
-        const int j = blockIdx.y * (LONG_PIECES * STEP) + threadIdx.x * V;
-        Vec<T, V> r[LONG_PIECES];
-        const bool whole = (int)(blockIdx.y + 1) * (LONG_PIECES * STEP) <= N;          // uniform
+        const int head = head_of(out), j = head + blockIdx.y * (LONG_PIECES * STEP) + threadIdx.x * V;
+        const bool first = blockIdx.y == 0 && (int)threadIdx.x < head;
         if (gu == 0.0f) {                                // uniform: the row is written without being read
             const float zero[V] = {};
 #pragma unroll
             for (int u = 0; u < LONG_PIECES; ++u) store_vec<T, V, true>(out, j + u * STEP, N, zero);
+            if (first) out[threadIdx.x] = from_f32<T>(0.0f);
             continue;
         }
+        Vec<T, V> r[LONG_PIECES];
+        const bool whole = head + (int)(blockIdx.y + 1) * (LONG_PIECES * STEP) <= N;          // uniform
         if (whole) {
 #pragma unroll
             for (int u = 0; u < LONG_PIECES; ++u) r[u] = *reinterpret_cast<const Vec<T, V>*>(row + j + u * STEP);
         } else {
 #pragma unroll
             for (int u = 0; u < LONG_PIECES; ++u) r[u] = load_vec<T, V, true>(row, j + u * STEP, N);
+        }
+        if (first) {
+            const float p = scale * exp_quick((to_f32(row[threadIdx.x]) - st.x) - st.y);
+            out[threadIdx.x] = from_f32<T>((int)threadIdx.x == c ? p + gu : p);
         }
 #pragma unroll
         for (int u = 0; u < LONG_PIECES; ++u) {

@@ -59,7 +59,11 @@ struct Sequences {
     }
 };
 
-static inline int64_t chunk_items(int64_t M) { return M <= 2048 * 1024 ? 1024 : ((M + 2047) / 2048 + 1023) / 1024 * 1024; }
+// items a workgroup sums: as few as make 2048 chunks (one round of the chip, and the most pieces that one sequence can have)
+static inline int64_t chunk_items(int64_t M) { return M <= 2048 * 256 ? 256 : ((M + 2047) / 2048 + 255) / 256 * 256; }
+// items a workgroup of the gradient writes: it joins nothing, so its chunks stay short (10.5 million items: 30 us in chunks
+// of 6144, whose workgroups all look for their sequence at once and then all write, 18 us in chunks of 2048)
+static inline int64_t spread_items(int64_t M) { return M <= 1024 * 512 ? 512 : 2048; }
 
 template <int Q> struct alignas(8) Sums { double v[Q]; };
 
@@ -156,8 +160,8 @@ k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whol
         if (i0 >= i1) continue;                          // uniform over the workgroup if `alone`, over the wave if not
         const float of_seq = f.of_sequence(s);
         typename F::Acc acc;
-        for (int64_t i = i0 + 4 * t; i + 4 <= i1; i += 4 * threads) f.template add<4>(i, of_seq, acc);
-        const int64_t rest = i0 + (i1 - i0) / 4 * 4 + t;
+        for (int64_t i = i0 + 8 * t; i + 8 <= i1; i += 8 * threads) f.template add<8>(i, of_seq, acc);
+        const int64_t rest = i0 + (i1 - i0) / 8 * 8 + t;
         if (rest < i1) f.template add<1>(rest, of_seq, acc);
         Sums<Q> sum = F::sums(acc);
 #pragma unroll
@@ -175,28 +179,51 @@ k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whol
     }
 }
 
-// whole[s] of every sequence, by one wave
-template <int Q>
-__device__ __forceinline__ void gather_sequence(const Sequences& q, int64_t chunk, int64_t s, int lane, Sums<Q>* __restrict__ whole,
-                                                const Sums<Q>* __restrict__ piece) {
+// sums of sequence s by LANES lanes, the first of which gets them
+template <int Q, int LANES>
+__device__ __forceinline__ Sums<Q> gather_sequence(const Sequences& q, int64_t chunk, int64_t s, int lane, const Sums<Q>* __restrict__ whole,
+                                                   const Sums<Q>* __restrict__ piece) {
     const int64_t lo = q.lo(s), hi = q.hi(s);
     Sums<Q> acc = {};
     if (lo < hi) {
         const int64_t k0 = lo / chunk, k1 = (hi - 1) / chunk;
-        if (k0 == k1) return;
-        for (int64_t k = k0 + lane; k <= k1; k += 64)
+        if (k0 == k1) return whole[s];
+#pragma unroll 4
+        for (int64_t k = k0 + lane; k <= k1; k += LANES)
 #pragma unroll
             for (int c = 0; c < Q; ++c) acc.v[c] += piece[2 * k + (k == k0 ? 1 : 0)].v[c];
 #pragma unroll
-        for (int c = 0; c < Q; ++c) acc.v[c] = wave_add(acc.v[c]);
+        for (int c = 0; c < Q; ++c)
+#pragma unroll
+            for (int off = LANES / 2; off >= 1; off >>= 1) acc.v[c] = acc.v[c] + __shfl_xor(acc.v[c], off);
     }
-    if (lane == 0) whole[s] = acc;
+    return acc;
 }
 template <int Q>
 __global__ void __launch_bounds__(256)
 k_sequence_gather(Sequences q, int64_t chunk, Sums<Q>* __restrict__ whole, const Sums<Q>* __restrict__ piece) {
     const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (s < q.S) gather_sequence<Q>(q, chunk, s, threadIdx.x & 63, whole, piece);
+    if (s >= q.S) return;
+    const Sums<Q> sum = gather_sequence<Q, 64>(q, chunk, s, threadIdx.x & 63, whole, piece);
+    if ((threadIdx.x & 63) == 0) whole[s] = sum;
+}
+// the same into LDS by a workgroup of 1024 threads, for up to SEQ_FUSED sequences: all of them at once
+template <int Q, int LANES>
+__device__ __forceinline__ void gather_all(const Sequences& q, int64_t chunk, const Sums<Q>* __restrict__ whole,
+                                           const Sums<Q>* __restrict__ piece, Sums<Q>* held) {
+    const int64_t s = threadIdx.x / LANES;
+    const int lane = threadIdx.x & (LANES - 1);
+    if (s < q.S) {
+        const Sums<Q> sum = gather_sequence<Q, LANES>(q, chunk, s, lane, whole, piece);
+        if (lane == 0) held[s] = sum;
+    }
+    __syncthreads();
+}
+template <int Q>
+__device__ __forceinline__ void gather_all(const Sequences& q, int64_t chunk, const Sums<Q>* __restrict__ whole,
+                                           const Sums<Q>* __restrict__ piece, Sums<Q>* held) {
+    if (q.S <= 16) gather_all<Q, 64>(q, chunk, whole, piece, held);
+    else gather_all<Q, 1024 / SEQ_FUSED>(q, chunk, whole, piece, held);
 }
 
 // sums over a workgroup of 1024 threads, in every thread
@@ -216,16 +243,14 @@ template <int N> __device__ __forceinline__ void block_add(double (&v)[N], doubl
 }
 
 __global__ void __launch_bounds__(1024)
-k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, Sums<4>* __restrict__ whole,
+k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, const Sums<4>* __restrict__ whole,
                 const Sums<4>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ weight) {
     __shared__ double red[16][5];
-    if (gather) {
-        for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<4>(q, chunk, s, threadIdx.x & 63, whole, piece);
-        __syncthreads();
-    }
+    __shared__ Sums<4> held[SEQ_FUSED];
+    if (gather) gather_all<4>(q, chunk, whole, piece, held);
     double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};           // the sums, live items, sequences that have one
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
-        const Sums<4> w = whole[s];
+        const Sums<4> w = gather ? held[s] : whole[s];
         if (w.v[3] <= 0.0) continue;
         const double unit = by_sequence ? 1.0 / w.v[3] : 1.0;
         tot[4] += 1.0;
@@ -237,7 +262,7 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
     const double over = by_sequence ? tot[4] : tot[3];
     const double norm = over > 0.0 ? 1.0 / over : 0.0;    // no live item: the loss and every gradient are 0
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
-        const double n = whole[s].v[3];
+        const double n = gather ? held[s].v[3] : whole[s].v[3];
         if (weight) weight[s] = n > 0.0 ? (float)(by_sequence ? norm / n : norm) : 0.0f;
     }
     if (threadIdx.x == 0) {
@@ -251,20 +276,18 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
 }
 
 __global__ void __launch_bounds__(1024)
-k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double smoothing, int average, Sums<2>* __restrict__ whole,
+k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double smoothing, int average, const Sums<2>* __restrict__ whole,
                     const Sums<2>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ weight) {
     __shared__ double red[16][1];
-    if (gather) {
-        for (int64_t s = threadIdx.x >> 6; s < q.S; s += 16) gather_sequence<2>(q, chunk, s, threadIdx.x & 63, whole, piece);
-        __syncthreads();
-    }
+    __shared__ Sums<2> held[SEQ_FUSED];
+    if (gather) gather_all<2>(q, chunk, whole, piece, held);
     const int64_t P = q.S / 2;
     double tot[1] = {0.0};
     for (int64_t p = threadIdx.x; p < P; p += 1024) {
         double h[2], unit[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const Sums<2> w = whole[2 * p + k];
+            const Sums<2> w = gather ? held[2 * p + k] : whole[2 * p + k];
             unit[k] = average && w.v[1] > 1.0 ? 1.0 / w.v[1] : 1.0;
             h[k] = w.v[0] * unit[k];
             rewards[2 * p + k] = (float)(beta * h[k]);
@@ -306,14 +329,25 @@ k_sequence_spread(Sequences q, int64_t chunk, const float* __restrict__ slope, c
     if (s0 == s1) {
         const float w0 = weight[s0] * up;
         const int64_t lo = q.lo(s0), hi = q.hi(s0);
-        for (int64_t i = a + 4 * (int)threadIdx.x; i < b; i += 1024) {
-            if (i + 4 <= b) put(i, std::integral_constant<int, 4>{}, w0, lo, hi);
+        for (int64_t i = a + 8 * (int)threadIdx.x; i < b; i += 2048) {
+            if (i + 8 <= b) put(i, std::integral_constant<int, 8>{}, w0, lo, hi);
             else for (int64_t k = i; k < b; ++k) put(k, std::integral_constant<int, 1>{}, w0, lo, hi);
         }
     } else {
-        for (int64_t i = a + threadIdx.x; i < b; i += 256) {
-            const int64_t s = q.of(i, s0, s1);
-            put(i, std::integral_constant<int, 1>{}, weight[s] * up, q.lo(s), q.hi(s));
+        for (int64_t i = a + 8 * (int)threadIdx.x; i < b; i += 2048) {
+            int64_t s = q.of(i, s0, s1), lo = q.lo(s), hi = q.hi(s);
+            if (i >= lo && i + 8 <= hi && i + 8 <= b) {
+                put(i, std::integral_constant<int, 8>{}, weight[s] * up, lo, hi);
+                continue;
+            }
+            for (int64_t k = i; k < i + 8 && k < b; ++k) {
+                if (k >= hi && s < s1) {                  // on to the sequence that holds item k
+                    s = q.of(k, s, s1);
+                    lo = q.lo(s);
+                    hi = q.hi(s);
+                }
+                put(k, std::integral_constant<int, 1>{}, weight[s] * up, lo, hi);
+            }
         }
     }
 }
@@ -422,7 +456,7 @@ extern "C" int gm_sequence_loss_bwd(int64_t M, int64_t S, const float* slope, co
     if (M == 0) return GM_OK;
     GM_REQUIRE(weight && g && dlog_prob, "bad arguments");
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
-    const int64_t chunk = chunk_items(M);
+    const int64_t chunk = spread_items(M);
     return with_flags(slope != nullptr, mask != nullptr, [&](auto sl, auto m) -> int {
         hipLaunchKernelGGL((k_sequence_spread<decltype(sl)::value, decltype(m)::value>), dim3((unsigned)((M + chunk - 1) / chunk)), dim3(256), 0,
                            as_stream(stream), q, chunk, slope, mask, weight, g, dlog_prob);

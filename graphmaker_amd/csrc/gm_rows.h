@@ -49,6 +49,16 @@ template <class T, int V, bool TAIL> __device__ __forceinline__ Vec<T, V> load_v
     }
     return x;
 }
+// the piece itself, as a value that has arrived: keeps the loads of the piece behind it from being moved into its place
+template <class T, int V> __device__ __forceinline__ Vec<T, V> settled(Vec<T, V> x) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    static_assert(sizeof(x) == sizeof(words), "a piece of 16 bytes");
+    words w;
+    __builtin_memcpy(&w, &x, 16);
+    asm volatile("" : "+v"(w));
+    __builtin_memcpy(&x, &w, 16);
+    return x;
+}
 template <class T, int V, bool TAIL> __device__ __forceinline__ void store_vec(T* __restrict__ row, int col, int N, const float (&x)[V]) {
     if (!TAIL ? col < N : col + V <= N) {
         Vec<T, V> t;
