@@ -4,6 +4,7 @@ The library is the product: there is no CPU or eager-PyTorch fallback.  If the s
 fails, this module raises -- it never routes around the HIP path.
 """
 import ctypes as C
+import importlib.util
 import os
 
 import torch
@@ -31,8 +32,8 @@ EXPORTS = [
 ]
 
 
-# Argument types of the entry points that take typed rows: with them ctypes converts plain Python numbers and addresses, so
-# a call names each argument once.  i = int64, d = int, f = float, p = device pointer (an address or None).
+# Argument types of the entry points that take typed rows: with them ctypes converts plain Python numbers and addresses.
+# i = int64, d = int, f = float, p = device pointer (an address or None).
 _SIGNATURES = {
     "gm_token_embedding_fwd": "iiipdpidfpip", "gm_token_embedding_bwd_workspace_bytes": "iii",
     "gm_token_embedding_bwd": "iiipdipidfpipip", "gm_layer_norm_fwd": "iipidppdfpippp",
@@ -43,7 +44,6 @@ _SIGNATURES = {
     "gm_sequence_loss_bwd": "iipppdpppp",
 }
 _CTYPES = {"i": C.c_int64, "d": C.c_int, "f": C.c_float, "p": C.c_void_p}
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # GM_DTYPE_*
 
 
 class GraphMakerHipError(RuntimeError):
@@ -129,25 +129,21 @@ U32 = C.c_uint32
 F32 = C.c_float
 
 
-_functions = {}
+TAPE_PATH = os.path.join(_HERE, "lib", "gm_tape.so")
+_tape = None
 
 
-def function(name):
-    """An entry point in _SIGNATURES, as a callable of plain numbers and addresses."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = getattr(load(), name)
-    return fn
-
-
-def launch(name, device, *args):
-    """One call of an entry point in _SIGNATURES on `device`'s current stream, whatever device is current."""
-    fn = function(name)
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != 0:
-        _check(rc, name)
+def tape():
+    """The module of tape nodes over torch's C++ autograd (csrc/gm_tape.cpp), loaded once.  Raises if it has not been built."""
+    global _tape
+    if _tape is None:
+        if not os.path.exists(TAPE_PATH):
+            raise GraphMakerHipError(f"{TAPE_PATH} is missing: build it with `make -C graphmaker_amd/csrc`. "
+                                     "graphmaker_amd has no fallback path.")
+        load()
+        spec = importlib.util.spec_from_file_location("gm_tape", TAPE_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.set_error_class(GraphMakerHipError)
+        _tape = module
+    return _tape

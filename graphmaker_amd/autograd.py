@@ -26,7 +26,6 @@ over the same leaf tensors is still alive: torch ties a leaf's gradient accumula
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
@@ -221,7 +220,10 @@ class _UpdateBlock(torch.autograd.Function):
         da = torch.empty_like(a)
         dgb = torch.empty((2, N), dtype=torch.float32, device=dev)
         if N > LAYERNORM_BWD_MAX:
-            _layer_norm_bwd(g, a, M, N, 0, mean.data_ptr(), rstd.data_ptr(), gamma, 0, da, dgb[0], dgb[1])
+            need = L.load().gm_layer_norm_bwd_workspace_bytes(M, N)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            L.call("gm_layer_norm_bwd", M, N, ptr(g), N, ptr(a), N, 0, ptr(mean), ptr(rstd), ptr(gamma), 0, ptr(da), N, ptr(dgb),
+                   C_void(dgb, N), ptr(ws), need, stream_ptr())
             L.call("gm_relu_bwd", I64(a.numel()), ptr(da), ptr(a), ptr(da), stream_ptr())
             dx, dW, db = _linear_backward(x, W, da, (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]))
             return dx, dW, db, dgb[0], dgb[1], None
@@ -466,222 +468,20 @@ def dropout(x, p, state):
 
 
 # ------------------------------------------------------------------ wider models and fine-tuning
-# A small call costs what its Python costs (the kernels of a short sequence take a few microseconds, the autograd engine's
-# round trip some 30): contiguous tensors are used as they are, without a view, and backward passes get their sizes as numbers.
-def _gradient(fn):
-    """A backward pass without a second derivative: an error for who differentiates the gradient (create_graph), and no wrapper
-    around the call otherwise."""
-    checked = once_differentiable(fn)
-
-    def backward(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
-
-    return staticmethod(backward)
-
-
-def _on_gpu(t, what):
-    if not t.is_cuda:
-        raise L.GraphMakerHipError(f"{what}: graphmaker_amd runs on a ROCm device only (tensor is on {t.device})")
-
-
-def _same_device(t, what, device):
-    if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, expected {device}")
-    return t
-
-
-def _row_dtype(t, what):
-    code = L.DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
-    return code
-
-
-def _rows(t, width):
-    """(tensor, leading dimension) of t as rows of `width` elements at its address; a copy only where its strides need one."""
-    if t.is_contiguous():
-        return t, width
-    t = t.reshape(-1, width)
-    if t.shape[0] == 0 or (t.shape[0] == 1 and (width == 1 or t.stride(1) == 1)):
-        return t, width
-    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-def _index(t, what, device):
-    """(contiguous tensor, 1 if int64) of an index argument."""
-    i64 = t.dtype == torch.int64
-    if not i64 and t.dtype != torch.int32:
-        raise TypeError(f"{what}: expected int32 or int64, got {t.dtype}")
-    return _c(_same_device(t, what, device)), int(i64)
-
-
-def _at(t):
-    return t.data_ptr() if t is not None else None
-
-
-def _token_embedding_fwd(weight, tokens, args):
-    n, C, w, i64, code, scale, _, _ = args
-    table, ldw = _rows(weight, w)
-    out = torch.empty((*tokens.shape, w), dtype=weight.dtype, device=weight.device)
-    L.launch("gm_token_embedding_fwd", weight.device, n, C, w, tokens.data_ptr(), i64, table.data_ptr(), ldw, code, scale, out.data_ptr(), w)
-    return out
-
-
-class _TokenEmbedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, tokens, args):
-        ctx.save_for_backward(tokens)
-        ctx.args = args
-        return _token_embedding_fwd(weight, tokens, args)
-
-    @_gradient
-    def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        n, C, w, i64, code, scale, padding, need = ctx.args
-        dev = g.device
-        g, ldg = _rows(g, w)
-        dW = torch.empty((C, w), dtype=g.dtype, device=dev)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        L.launch("gm_token_embedding_bwd", dev, n, C, w, tokens.data_ptr(), i64, padding, g.data_ptr(), ldg, code, scale, dW.data_ptr(), w,
-                 ws.data_ptr(), need)
-        return dW, None, None
-
-
+# The nodes of these operators are C++ (csrc/gm_tape.cpp), which checks the arguments too.
 def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
     """scale * weight[tokens], shape tokens.shape + (w,), in weight's type (float32, bfloat16, float16).  tokens: int32 or int64
     of any shape.  The gradient sums each row's tokens in ascending position (no atomics: the same bits on every run) and
     leaves row padding_idx zero, as nn.Embedding does.  Tokens are not read on the host: one outside [0, C) gives a row of
     NaN and adds to no gradient; ops.check_index_range(tokens, C, "tokens") is the check that raises."""
-    if weight.dim() != 2 or weight.numel() == 0:
-        raise ValueError(f"token_embedding: weight must be (C, w) with C, w > 0, got {tuple(weight.shape)}")
-    code = _row_dtype(weight, "weight")
-    tokens, i64 = _index(tokens, "tokens", weight.device)
-    C, w = weight.shape
-    if padding_idx is None:
-        padding = -1
-    else:
-        if not -C <= padding_idx < C:
-            raise ValueError(f"token_embedding: padding_idx {padding_idx} is outside the {C} rows of weight")
-        padding = int(padding_idx) % C
-    _on_gpu(weight, "weight")
-    n = tokens.numel()
-    if weight.requires_grad and torch.is_grad_enabled():
-        need = L.function("gm_token_embedding_bwd_workspace_bytes")(n, C, w)
-        return _TokenEmbedding.apply(weight, tokens, (n, C, w, i64, code, float(scale), padding, need))
-    return _token_embedding_fwd(weight, tokens, (n, C, w, i64, code, float(scale), padding, 0))
-
-
-def _layer_norm_fwd(x, gamma, beta, args, stats):
-    M, N, code, wcode, eps = args
-    dev = x.device
-    rows, ldx = _rows(x, N)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    st = torch.empty(2 * M, dtype=torch.float32, device=dev) if stats else None
-    at = _at(st)
-    L.launch("gm_layer_norm_fwd", dev, M, N, rows.data_ptr(), ldx, code, _at(gamma), _at(beta), wcode, eps, y.data_ptr(), N, at,
-             at + 4 * M if at else at)
-    return y, rows, st
-
-
-def _layer_norm_bwd(g, rows, M, N, code, mean, rstd, gamma, wcode, dx, dgamma, dbeta):
-    """gm_layer_norm_bwd over the M rows of N of x; mean, rstd: addresses; dx, dgamma, dbeta: outputs or None."""
-    dev = rows.device
-    rows, ldx = _rows(rows, N)
-    g, ldg = _rows(g, N)
-    need = L.function("gm_layer_norm_bwd_workspace_bytes")(M, N) if dgamma is not None or dbeta is not None else 0
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    L.launch("gm_layer_norm_bwd", dev, M, N, g.data_ptr(), ldg, rows.data_ptr(), ldx, code, mean, rstd, _at(gamma), wcode, _at(dx), N,
-             _at(dgamma), _at(dbeta), _at(ws), need)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, args):
-        y, rows, st = _layer_norm_fwd(x, gamma, beta, args, True)
-        ctx.save_for_backward(rows, st, gamma)
-        ctx.args = args
-        ctx.shape = x.shape
-        ctx.weight_dtypes = (gamma.dtype if gamma is not None else None, beta.dtype if beta is not None else None)
-        return y
-
-    @_gradient
-    def backward(ctx, g):
-        rows, st, gamma = ctx.saved_tensors
-        M, N, code, wcode, _ = ctx.args
-        dev, need, types = g.device, ctx.needs_input_grad, ctx.weight_dtypes
-        dx = torch.empty(ctx.shape, dtype=g.dtype, device=dev) if need[0] else None
-        dgamma = torch.empty(N, dtype=types[0], device=dev) if need[1] else None
-        dbeta = torch.empty(N, dtype=types[1], device=dev) if need[2] else None
-        at = st.data_ptr()
-        _layer_norm_bwd(g, rows, M, N, code, at, at + 4 * M, gamma, wcode, dx, dgamma, dbeta)
-        return dx, dgamma, dbeta, None
+    return L.tape().token_embedding(weight, tokens, scale, padding_idx)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension, of any width, in x's type (float32, bfloat16,
     float16).  gamma and beta (N,): x's type or float32, both the same; None: 1 and 0.  Statistics are float32 about the mean,
     the variance that of the differences from it."""
-    N = x.shape[-1] if x.dim() else 0
-    if N == 0:
-        raise ValueError(f"layer_norm: x must have a last dimension of at least 1, got {tuple(x.shape)}")
-    code = _row_dtype(x, "x")
-    wcode, records = code, x.requires_grad
-    for t, what in ((gamma, "gamma"), (beta, "beta")):
-        if t is None:
-            continue
-        if t.dim() != 1 or t.numel() != N:
-            raise ValueError(f"layer_norm: {what} is {tuple(t.shape)}, x's rows have {N} columns")
-        if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise TypeError(f"layer_norm: {what} is {t.dtype}, expected {x.dtype} or float32")
-        _same_device(t, what, x.device)
-        wcode = L.DTYPES[t.dtype]
-        records = records or t.requires_grad
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise TypeError(f"layer_norm: gamma is {gamma.dtype} and beta is {beta.dtype}")
-    if not eps >= 0.0:
-        raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
-    _on_gpu(x, "x")
-    gamma, beta = (t if t is None else _c(t) for t in (gamma, beta))
-    args = (x.numel() // N, N, code, wcode, float(eps))
-    if records and torch.is_grad_enabled():
-        return _LayerNorm.apply(x, gamma, beta, args)
-    return _layer_norm_fwd(x, gamma, beta, args, False)[0]
-
-
-def _class_log_prob_fwd(logits, classes, args, stats):
-    M, V, code, i64, ignore_index = args
-    dev = logits.device
-    rows, ldx = _rows(logits, V)
-    lp = torch.empty(classes.shape, dtype=torch.float32, device=dev)
-    floats = L.function("gm_class_log_prob_stats_floats")(M, V, code) if stats else 0
-    st = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-    need = L.function("gm_class_log_prob_workspace_bytes")(M, V, code)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    L.launch("gm_class_log_prob_fwd", dev, M, V, rows.data_ptr(), ldx, code, classes.data_ptr(), i64, ignore_index, lp.data_ptr(), _at(st),
-             _at(ws), need)
-    return lp, rows, ldx, st
-
-
-class _ClassLogProb(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, classes, args):
-        lp, rows, ctx.ldx, st = _class_log_prob_fwd(logits, classes, args, True)
-        ctx.save_for_backward(rows, classes, st)
-        ctx.args = args
-        ctx.shape = logits.shape
-        return lp
-
-    @_gradient
-    def backward(ctx, g):
-        rows, classes, st = ctx.saved_tensors
-        M, V, code, i64, ignore_index = ctx.args
-        g = _c(g)
-        dx = torch.empty(ctx.shape, dtype=rows.dtype, device=g.device)
-        L.launch("gm_class_log_prob_bwd", g.device, M, V, g.data_ptr(), rows.data_ptr(), ctx.ldx, code, classes.data_ptr(), i64, ignore_index,
-                 _at(st), dx.data_ptr(), V)
-        return dx, None, None
+    return L.tape().layer_norm(x, gamma, beta, eps)
 
 
 def class_log_prob(logits, classes, ignore_index=-100):
@@ -689,100 +489,7 @@ def class_log_prob(logits, classes, ignore_index=-100):
     bfloat16 or float16, classes int32 or int64.  A row whose class is ignore_index has log-probability 0 and a zero gradient,
     whatever its logits hold; any other class outside [0, V) gives NaN in both (classes are not read on the host).  A row
     whose upstream gradient is exactly 0 gets a zero gradient too."""
-    V = logits.shape[-1] if logits.dim() else 0
-    if V == 0:
-        raise ValueError(f"class_log_prob: logits must have a last dimension of at least 1, got {tuple(logits.shape)}")
-    if classes.shape != logits.shape[:-1]:
-        raise ValueError(f"class_log_prob: classes is {tuple(classes.shape)}, logits is {tuple(logits.shape)}")
-    code = _row_dtype(logits, "logits")
-    classes, i64 = _index(classes, "classes", logits.device)
-    _on_gpu(logits, "logits")
-    args = (classes.numel(), V, code, i64, int(ignore_index))
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _ClassLogProb.apply(logits, classes, args)
-    return _class_log_prob_fwd(logits, classes, args, False)[0]
-
-
-def _items(t, what, like=None):
-    """A float32 per-item argument; with `like`, one of its shape and device that takes no gradient."""
-    if t.dtype != torch.float32:
-        raise TypeError(f"{what}: expected float32, got {t.dtype}")
-    if like is not None:
-        if t.shape != like.shape:
-            raise ValueError(f"{what} is {tuple(t.shape)}, log_prob is {tuple(like.shape)}")
-        _constant(t, what)
-        _same_device(t, what, like.device)
-    return _c(t)
-
-
-def _constant(t, what):
-    if t.requires_grad:
-        raise ValueError(f"{what} is a constant of the loss and gets no gradient: pass {what}.detach()")
-
-
-def _mask(mask, like):
-    if mask is None:
-        return None
-    if mask.dtype != torch.bool and mask.dtype != torch.uint8:
-        raise TypeError(f"mask: expected bool or uint8, got {mask.dtype}")
-    if mask.shape != like.shape:
-        raise ValueError(f"mask is {tuple(mask.shape)}, log_prob is {tuple(like.shape)}")
-    return _c(_same_device(mask, "mask", like.device))
-
-
-def _offsets(offsets, device):
-    if offsets.dim() != 1 or offsets.numel() < 2:
-        raise ValueError(f"offsets: expected the S + 1 borders of S > 0 sequences, got {tuple(offsets.shape)}")
-    return _index(offsets, "offsets", device)
-
-
-def _sequence_buffer(M, S, slopes, dev):
-    """(buffer, addresses of the S weights, `slopes` slopes and the workspace in it, workspace bytes).  What a loss keeps for its
-    backward pass and what it works in share one allocation."""
-    need = L.function("gm_sequence_loss_workspace_bytes")(M, S)
-    head = (4 * (S + slopes) + 15) // 16 * 16
-    buf = torch.empty(head + need, dtype=torch.uint8, device=dev)
-    at = buf.data_ptr()
-    return buf, at, at + 4 * S if slopes else None, at + head, need
-
-
-def _sequence_loss_bwd(g, buf, M, S, has_slope, mask, offsets, i64, shape):
-    out = torch.empty(shape, dtype=torch.float32, device=g.device)
-    at = buf.data_ptr()
-    L.launch("gm_sequence_loss_bwd", g.device, M, S, at + 4 * S if has_slope else None, _at(mask), _at(offsets), i64, at, g.data_ptr(),
-             out.data_ptr())
-    return out
-
-
-def _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, grad):
-    M, S, i64, clip_low, clip_high, kl_coef, by_sequence = args
-    dev = lp.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    stats = torch.empty(4, dtype=torch.float32, device=dev)
-    buf, weight, slope, ws, need = _sequence_buffer(M, S, M if grad else 0, dev)
-    L.launch("gm_policy_loss_fwd", dev, M, S, lp.data_ptr(), old.data_ptr(), adv.data_ptr(), _at(ref), _at(mask), _at(offsets), i64, clip_low,
-             clip_high, kl_coef, by_sequence, loss.data_ptr(), stats.data_ptr(), slope, weight, ws, need)
-    return loss, stats, buf
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, lp, old, adv, ref, mask, offsets, args):
-        loss, stats, buf = _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, True)
-        ctx.save_for_backward(buf, mask, offsets)
-        ctx.args = args
-        ctx.shape = lp.shape
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
-
-    @_gradient
-    def backward(ctx, g, _stats):
-        if g is None:
-            return (None,) * 7
-        buf, mask, offsets = ctx.saved_tensors
-        M, S, i64 = ctx.args[:3]
-        return _sequence_loss_bwd(g, buf, M, S, M > 0, mask, offsets, i64, ctx.shape), None, None, None, None, None, None
+    return L.tape().class_log_prob(logits, classes, ignore_index)
 
 
 def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, ref_log_prob=None, clip_low=0.2, clip_high=0.2,
@@ -798,67 +505,7 @@ def policy_loss(log_prob, old_log_prob, advantage, *, offsets=None, mask=None, r
     ref_log_prob are constants.
 
     Returns (loss, stats), stats = [mean surrogate, mean KL, share of clipped items, live items] without a gradient."""
-    lp = _items(log_prob, "log_prob")
-    old = _items(old_log_prob, "old_log_prob", log_prob)
-    ref = _items(ref_log_prob, "ref_log_prob", log_prob) if ref_log_prob is not None else None
-    mask = _mask(mask, log_prob)
-    i64, S = 0, 1
-    if offsets is None:
-        adv = _items(advantage, "advantage", log_prob)
-    else:
-        offsets, i64 = _offsets(offsets, log_prob.device)
-        S = offsets.numel() - 1
-        adv = _items(advantage, "advantage")
-        _same_device(adv, "advantage", log_prob.device)
-        _constant(advantage, "advantage")
-        if advantage.dim() != 1 or advantage.numel() != S:
-            raise ValueError(f"advantage is {tuple(advantage.shape)}, offsets border {S} sequences")
-    if reduction not in ("token", "sequence"):
-        raise ValueError(f"reduction: expected 'token' or 'sequence', got {reduction!r}")
-    if reduction == "sequence" and offsets is None:
-        raise ValueError("reduction 'sequence' needs offsets")
-    if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
-        raise ValueError(f"clip range: 0 <= clip_low <= 1 and 0 <= clip_high, got {clip_low}, {clip_high}")
-    if kl_coef != 0.0 and ref is None:
-        raise ValueError("kl_coef needs ref_log_prob")
-    if kl_coef - kl_coef != 0.0:
-        raise ValueError(f"kl_coef must be finite, got {kl_coef}")
-    _on_gpu(log_prob, "log_prob")
-    args = (lp.numel(), S, i64, float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
-    if log_prob.requires_grad and torch.is_grad_enabled():
-        return _PolicyLoss.apply(lp, old, adv, ref, mask, offsets, args)
-    return _policy_loss_fwd(lp, old, adv, ref, mask, offsets, args, False)[:2]
-
-
-def _preference_loss_fwd(lp, ref, mask, offsets, args):
-    M, S, i64, beta, smoothing, average = args
-    dev = lp.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    rewards = torch.empty(S, dtype=torch.float32, device=dev)
-    buf, weight, _, ws, need = _sequence_buffer(M, S, 0, dev)
-    L.launch("gm_preference_loss_fwd", dev, M, S // 2, lp.data_ptr(), ref.data_ptr(), _at(mask), offsets.data_ptr(), i64, beta, smoothing, average,
-             loss.data_ptr(), rewards.data_ptr(), weight, ws, need)
-    return loss, rewards, buf
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, lp, ref, mask, offsets, args):
-        loss, rewards, buf = _preference_loss_fwd(lp, ref, mask, offsets, args)
-        ctx.save_for_backward(buf, mask, offsets)
-        ctx.args = args
-        ctx.shape = lp.shape
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @_gradient
-    def backward(ctx, g, _rewards):
-        if g is None:
-            return (None,) * 5
-        buf, mask, offsets = ctx.saved_tensors
-        M, S, i64 = ctx.args[:3]
-        return _sequence_loss_bwd(g, buf, M, S, False, mask, offsets, i64, ctx.shape), None, None, None, None
+    return L.tape().policy_loss(log_prob, old_log_prob, advantage, offsets, mask, ref_log_prob, clip_low, clip_high, kl_coef, reduction)
 
 
 def preference_loss(log_prob, ref_log_prob, offsets, *, mask=None, beta=0.1, label_smoothing=0.0, average=False):
@@ -869,17 +516,4 @@ def preference_loss(log_prob, ref_log_prob, offsets, *, mask=None, beta=0.1, lab
 
     mask, items outside every sequence: as in policy_loss.  A sequence without a live item has h = 0.
     Returns (loss, rewards), rewards = beta h of the 2P sequences, without a gradient."""
-    lp = _items(log_prob, "log_prob")
-    ref = _items(ref_log_prob, "ref_log_prob", log_prob)
-    mask = _mask(mask, log_prob)
-    offsets, i64 = _offsets(offsets, log_prob.device)
-    S = offsets.numel() - 1
-    if S % 2:
-        raise ValueError(f"offsets border {S} sequences: an even number makes pairs")
-    if not 0.0 < beta < float("inf") or not 0.0 <= label_smoothing <= 0.5:
-        raise ValueError(f"0 < beta and 0 <= label_smoothing <= 0.5, got {beta}, {label_smoothing}")
-    _on_gpu(log_prob, "log_prob")
-    args = (lp.numel(), S, i64, float(beta), float(label_smoothing), int(bool(average)))
-    if log_prob.requires_grad and torch.is_grad_enabled():
-        return _PreferenceLoss.apply(lp, ref, mask, offsets, args)
-    return _preference_loss_fwd(lp, ref, mask, offsets, args)[:2]
+    return L.tape().preference_loss(log_prob, ref_log_prob, offsets, mask, beta, label_smoothing, average)
