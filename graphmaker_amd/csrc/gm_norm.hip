@@ -67,32 +67,42 @@ template <int TPR> __device__ __forceinline__ void row_add(float& a, float& b, f
 
 // A row stays in registers: TPR threads hold K x 16 bytes each, so HBM sees every element once.  A workgroup walks several
 // rows with gamma and beta in registers too, and loads the next row before it reduces the one it has: what a row waits for
-// is HBM alone.
+// is HBM alone (8191 x 8192 bf16: 53 us, the card's copy rate; reading gamma and beta and waiting for the row took 92).  Rows of
+// 1024 threads are LEAN, without either: half the registers, so that a second workgroup fits a CU.
 template <class T, int V, bool TAIL, int K, int TPR>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 k_layer_norm_fwd(int64_t M, int N, const T* __restrict__ X, int64_t ldx, Weights w, float eps, T* __restrict__ Y, int64_t ldy,
                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
     constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+    constexpr bool LEAN = TPR == 1024;
+    constexpr int HELD = LEAN ? 1 : K;
     __shared__ float red[2][16];
     const int t = threadIdx.x & (TPR - 1);
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
     if (m >= M) return;
-    Vec<T, V> r[K], next[K];
-    float ga[K][V], be[K][V];
+    Vec<T, V> r[K], next[HELD];
+    float ga[HELD][V], be[HELD][V];
+    if constexpr (!LEAN) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
+        for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
-        w.load<T, V, TAIL>(w.beta, (k * TPR + t) * V, N, 0.0f, be[k]);
+        for (int k = 0; k < K; ++k) {
+            w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
+            w.load<T, V, TAIL>(w.beta, (k * TPR + t) * V, N, 0.0f, be[k]);
+        }
     }
     for (; m < M; m += step) {
-        const int64_t ahead = m + step < M ? m + step : m;
+        if constexpr (LEAN) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) r[k] = next[k];
+            for (int k = 0; k < K; ++k) r[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
+        } else {
+            const int64_t ahead = m + step < M ? m + step : m;
 #pragma unroll
-        for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
+            for (int k = 0; k < K; ++k) r[k] = next[k];
+#pragma unroll
+            for (int k = 0; k < K; ++k) next[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
+        }
         float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -110,8 +120,13 @@ k_layer_norm_fwd(int64_t M, int N, const T* __restrict__ X, int64_t ldx, Weights
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float y[V];
+            const int h = LEAN ? 0 : k;
+            if constexpr (LEAN) {
+                w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[0]);
+                w.load<T, V, TAIL>(w.beta, (k * TPR + t) * V, N, 0.0f, be[0]);
+            }
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = __builtin_fmaf((to_f32(r[k].v[i]) - mean) * rstd, ga[k][i], be[k][i]);
+            for (int i = 0; i < V; ++i) y[i] = __builtin_fmaf((to_f32(r[k].v[i]) - mean) * rstd, ga[h][i], be[h][i]);
             store_vec<T, V, TAIL>(Y + m * ldy, (k * TPR + t) * V, N, y);
         }
         if (t == 0 && mean_out) {
@@ -129,46 +144,60 @@ k_layer_norm_bwd(int64_t M, int N, const T* __restrict__ G, int64_t ldg, const T
                  const float* __restrict__ mean, const float* __restrict__ rstd, Weights w, T* __restrict__ dX, int64_t lddx,
                  float* __restrict__ part) {
     constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+    constexpr bool LEAN = TPR == 1024;
+    constexpr int HELD = LEAN ? 1 : K;
     __shared__ float red[2][2][16];
     const int t = threadIdx.x & (TPR - 1);
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-    float ga[K][V], dga[K][V], dbe[K][V];
-    Vec<T, V> xr[K], gr[K], xn[K], gn[K];
+    float ga[HELD][V], dga[K][V], dbe[K][V];
+    Vec<T, V> xr[K], gr[K], xn[HELD], gn[HELD];
     float mu_n = 0.0f, rs_n = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) dga[k][i] = dbe[k][i] = 0.0f;
-    if (m < M) {
+    if (!LEAN && m < M) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+        for (int k = 0; k < HELD; ++k) {
             xn[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
             gn[k] = load_vec<T, V, TAIL>(G + m * ldg, (k * TPR + t) * V, N);
         }
         mu_n = mean[m];
         rs_n = rstd[m];
 #pragma unroll
-        for (int k = 0; k < K; ++k) w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
+        for (int k = 0; k < HELD; ++k) w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[k]);
     }
     for (int turn = 0; m < M; m += step, turn ^= 1) {
-        const int64_t ahead = m + step < M ? m + step : m;
-        const float mu = mu_n, rs = rs_n;
+        float mu = mu_n, rs = rs_n;
+        if constexpr (LEAN) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) { xr[k] = xn[k]; gr[k] = gn[k]; }
+            for (int k = 0; k < K; ++k) {
+                xr[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * TPR + t) * V, N);
+                gr[k] = load_vec<T, V, TAIL>(G + m * ldg, (k * TPR + t) * V, N);           // 0 behind the row: adds to no sum
+            }
+            mu = mean[m];
+            rs = rstd[m];
+        } else {
+            const int64_t ahead = m + step < M ? m + step : m;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            xn[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
-            gn[k] = load_vec<T, V, TAIL>(G + ahead * ldg, (k * TPR + t) * V, N);           // 0 behind the row: adds to no sum
+            for (int k = 0; k < K; ++k) { xr[k] = xn[k]; gr[k] = gn[k]; }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                xn[k] = load_vec<T, V, TAIL>(X + ahead * ldx, (k * TPR + t) * V, N);
+                gn[k] = load_vec<T, V, TAIL>(G + ahead * ldg, (k * TPR + t) * V, N);
+            }
+            mu_n = mean[ahead];
+            rs_n = rstd[ahead];
         }
-        mu_n = mean[ahead];
-        rs_n = rstd[ahead];
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            const int h = LEAN ? 0 : k;
+            if constexpr (LEAN) w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[0]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float g = to_f32(gr[k].v[i]), xh = (to_f32(xr[k].v[i]) - mu) * rs, gg = g * ga[k][i];
+                const float g = to_f32(gr[k].v[i]), xh = (to_f32(xr[k].v[i]) - mu) * rs, gg = g * ga[h][i];
                 if ((k * TPR + t) * V + i < N) {                    // x is 0 there, xh is not, and may be infinite
                     dga[k][i] = __builtin_fmaf(g, xh, dga[k][i]);
                     s2 = __builtin_fmaf(gg, xh, s2);
@@ -176,6 +205,7 @@ k_layer_norm_bwd(int64_t M, int N, const T* __restrict__ G, int64_t ldg, const T
                 }
                 dbe[k][i] = dbe[k][i] + g;
             }
+        }
         row_add<TPR>(s1, s2, red[turn]);
         s1 = s1 / (float)N;
         s2 = s2 / (float)N;
@@ -183,10 +213,12 @@ k_layer_norm_bwd(int64_t M, int N, const T* __restrict__ G, int64_t ldg, const T
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 float y[V];
+                const int h = LEAN ? 0 : k;
+                if constexpr (LEAN) w.load<T, V, TAIL>(w.gamma, (k * TPR + t) * V, N, 1.0f, ga[0]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float xh = (to_f32(xr[k].v[i]) - mu) * rs;
-                    y[i] = rs * ((to_f32(gr[k].v[i]) * ga[k][i] - s1) - xh * s2);
+                    y[i] = rs * ((to_f32(gr[k].v[i]) * ga[h][i] - s1) - xh * s2);
                 }
                 store_vec<T, V, TAIL>(dX + m * lddx, (k * TPR + t) * V, N, y);
             }
@@ -308,12 +340,12 @@ k_layer_norm_cols(int64_t nblk, int64_t N, const float* __restrict__ part, W* __
 // Threads a row and 16-byte pieces a thread.  A wave a row while four pieces hold it (no barrier, four rows a workgroup); a
 // workgroup where they do not, or where the rows are fewer than the waves the chip wants.  tpr = 0: too wide.
 struct RowShape { int tpr, K; };
-static inline RowShape row_shape(int64_t M, int64_t N, int vec, int most) {
+static inline RowShape row_shape(int64_t M, int64_t N, int vec, int most, int most_lean) {
     const int64_t v = (N + vec - 1) / vec;
-    const int tpr = v <= 64 || (v <= 256 && M >= 1024) ? 64 : v <= 1024 ? 256 : 1024;
+    const int tpr = v <= 64 || (v <= 256 && M >= 1024) ? 64 : v <= 256 * most ? 256 : 1024;
     int K = 1;
     while ((int64_t)K * tpr < v) K *= 2;
-    return K > most ? RowShape{0, 0} : RowShape{tpr, K};
+    return K > (tpr == 1024 ? most_lean : most) ? RowShape{0, 0} : RowShape{tpr, K};
 }
 // workgroups of the forward: what the CUs hold at once
 static inline int64_t norm_blocks_fwd(int64_t M, int rows, int threads) {
@@ -348,7 +380,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
     const Weights w{gamma, beta, weight_dtype == GM_DTYPE_F32};
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const RowShape r = row_shape(M, N, VEC<T>, 8);
+        const RowShape r = row_shape(M, N, VEC<T>, 4, 8);
 #define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)norm_blocks_fwd(M, ROWS, THREADS)), dim3(THREADS), 0, as_stream(stream), M, N, \
                        static_cast<const T*>(X), ldx, w, eps, static_cast<T*>(Y), ldy, mean, rstd)
@@ -399,7 +431,7 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
         using W = decltype(u);
         if (M > 0) {
             const Weights w{gamma, nullptr, weight_dtype == GM_DTYPE_F32};
-            const RowShape r = row_shape(M, N, VEC<T>, 4);
+            const RowShape r = row_shape(M, N, VEC<T>, 4, 16 / VEC<T>);      // the sums of 16 columns a thread at 1024 threads
 #define GM_LAUNCH_NORM(KERNEL, THREADS)                                                                                   \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,            \
                        static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part)
@@ -417,7 +449,9 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
                         case 256 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 256>), 256); break;
                         case 256 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 256>), 256); break;
                         case 1024 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 1024>), 1024); break;
-                        case 1024 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 1024>), 1024); break;
+                        case 1024 + 4:
+                            if constexpr (V == 4) GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 1024>), 1024);
+                            break;
                         default: GM_LAUNCH_NORM((k_layer_norm_bwd_long<T>), 1024); break;
                     }
                 }

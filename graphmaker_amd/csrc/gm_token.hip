@@ -46,7 +46,7 @@ k_token_embedding_fwd(int64_t n, int64_t C, int w, int shift, IndexArray tok, co
 }
 
 // ---- stable radix sort of n keys in [0, C] (C: tokens that add to no row, sorted behind the others), RADIX_BITS at a time
-constexpr int RADIX_BITS = 9, RADIX_BINS = 1 << RADIX_BITS;
+constexpr int RADIX_BITS = 9, RADIX_BINS = 1 << RADIX_BITS;         // at most; the digits of a sort are as even as can be
 constexpr int SORT_KEYS = 2048;                       // keys per workgroup: 4 waves x 8 rounds x 64 lanes
 __device__ __forceinline__ uint32_t token_key(const IndexArray& tok, int64_t i, int64_t C, int64_t padding) {
     const int64_t c = tok.at(i);
@@ -55,10 +55,11 @@ __device__ __forceinline__ uint32_t token_key(const IndexArray& tok, int64_t i, 
 
 // The place of a lane's key with digit d: the wave's next free place of the digit and the number of lower lanes with the same
 // one (found by a ballot per digit bit), so that equal digits keep their order.  Moves the digit's next free place on.
+template <int BITS>
 __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, bool in, int lane) {
     uint64_t same = __ballot(in);
 #pragma unroll
-    for (int bit = 0; bit < RADIX_BITS; ++bit) {
+    for (int bit = 0; bit < BITS; ++bit) {
         const uint64_t set = __ballot((d >> bit) & 1u);
         same &= (d >> bit) & 1u ? set : ~set;
     }
@@ -73,21 +74,22 @@ __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, bool 
 
 // counts[digit][workgroup]
 __global__ void __launch_bounds__(256)
-k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys, int shift,
+k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys, int shift, int bits,
               uint32_t* __restrict__ counts) {
     __shared__ uint32_t hist[RADIX_BINS];
-    for (int b = threadIdx.x; b < RADIX_BINS; b += 256) hist[b] = 0;
+    const int bins = 1 << bits;
+    for (int b = threadIdx.x; b < bins; b += 256) hist[b] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * SORT_KEYS;
     for (int r = 0; r < SORT_KEYS / 256; ++r) {
         const int64_t i = base + r * 256 + threadIdx.x;
         if (i < n) {
             const uint32_t key = keys ? keys[i] : token_key(tok, i, C, padding);
-            atomicAdd(&hist[(key >> shift) & (RADIX_BINS - 1)], 1u);
+            atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
         }
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < RADIX_BINS; b += 256) counts[(int64_t)b * gridDim.x + blockIdx.x] = hist[b];
+    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)b * gridDim.x + blockIdx.x] = hist[b];
 }
 
 // exclusive prefix sum of m counts (a multiple of 4) by one workgroup, SCAN_EACH a thread and step
@@ -134,12 +136,14 @@ __global__ void __launch_bounds__(1024) k_radix_scan(int64_t m, uint32_t* __rest
 }
 
 // Each wave owns SORT_KEYS/4 consecutive keys and keeps the next free place of every digit.
+template <int BITS>
 __global__ void __launch_bounds__(256)
 k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys,
                 const uint32_t* __restrict__ pos, int shift, const uint32_t* __restrict__ starts, uint32_t* __restrict__ keys_out,
                 uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t next[4][RADIX_BINS];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    constexpr int bins = 1 << BITS;
     for (int b = threadIdx.x; b < 4 * RADIX_BINS; b += 256) (&next[0][0])[b] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * SORT_KEYS + wv * (SORT_KEYS / 4);
@@ -150,11 +154,11 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
         key[r] = 0;
         if (i < n) {
             key[r] = keys ? keys[i] : token_key(tok, i, C, padding);
-            atomicAdd(&next[wv][(key[r] >> shift) & (RADIX_BINS - 1)], 1u);
+            atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
         }
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < RADIX_BINS; b += 256) {
+    for (int b = threadIdx.x; b < bins; b += 256) {
         uint32_t at = starts[(int64_t)b * gridDim.x + blockIdx.x];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -168,8 +172,8 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
     for (int r = 0; r < SORT_KEYS / 256; ++r) {
         const int64_t i = base + r * 64 + lane;
         const bool in = i < n;
-        const uint32_t d = (key[r] >> shift) & (RADIX_BINS - 1);
-        const uint32_t at = take_place(next[wv], d, in, lane);
+        const uint32_t d = (key[r] >> shift) & (bins - 1);
+        const uint32_t at = take_place<BITS>(next[wv], d, in, lane);
         if (in) {
             keys_out[at] = key[r];
             pos_out[at] = pos ? pos[i] : (uint32_t)i;
@@ -180,6 +184,7 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
 // The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch.  Wave wv holds keys
 // [wv * 1024, wv * 1024 + 1024) of the current order in registers and exchanges them through LDS.
 constexpr int SMALL_WAVES = 8, SMALL_ROUNDS = 16, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64;
+template <int BITS>
 __global__ void __launch_bounds__(SMALL_WAVES * 64)
 k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes, uint32_t* __restrict__ keys_out,
                    uint32_t* __restrict__ pos_out) {
@@ -187,6 +192,7 @@ k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes
     __shared__ uint32_t buf[SMALL_KEYS];
     __shared__ uint32_t tot[SMALL_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    constexpr int bins = 1 << BITS;
     uint32_t key[SMALL_ROUNDS], pos[SMALL_ROUNDS];
 #pragma unroll
     for (int r = 0; r < SMALL_ROUNDS; ++r) {
@@ -195,11 +201,11 @@ k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes
         key[r] = i < n ? token_key(tok, i, C, padding) : 0xFFFFFFFFu;         // behind every key in every digit: stays last
     }
     for (int p = 0; p < passes; ++p) {
-        const int shift = p * RADIX_BITS;
+        const int shift = p * BITS;
         for (int b = threadIdx.x; b < SMALL_WAVES * RADIX_BINS; b += SMALL_WAVES * 64) (&next[0][0])[b] = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r) atomicAdd(&next[wv][(key[r] >> shift) & (RADIX_BINS - 1)], 1u);
+        for (int r = 0; r < SMALL_ROUNDS; ++r) atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
         __syncthreads();
         // thread b owns digit b: starts of the digits by a scan over the workgroup, then of each wave's share of its digit
         static_assert(RADIX_BINS == SMALL_WAVES * 64, "one thread a digit");
@@ -226,8 +232,8 @@ k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes
         uint32_t place[SMALL_ROUNDS];
 #pragma unroll
         for (int r = 0; r < SMALL_ROUNDS; ++r) {
-            const uint32_t d = (key[r] >> shift) & (RADIX_BINS - 1);
-            place[r] = take_place(next[wv], d, true, lane);
+            const uint32_t d = (key[r] >> shift) & (bins - 1);
+            place[r] = take_place<BITS>(next[wv], d, true, lane);
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -322,12 +328,11 @@ struct RowSum {
 // part[2k] of the row that chunk k begins with, part[2k+1] of the row that it ends with and did not begin with.  Such a row
 // meets at least two chunks, so a chunk holds pieces of at most two of them.
 template <class T, int V, bool TAIL, int K>
-__global__ void __launch_bounds__(64)
-k_token_pieces(int64_t n, int64_t C, int w, int lanes, uint32_t cut, const uint32_t* __restrict__ keys,
-               const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G, int64_t ldg,
-               float* __restrict__ part, int64_t ldp) {
-    const int lane = threadIdx.x, col0 = blockIdx.y * 64 * V * K;
-    const uint32_t a = blockIdx.x * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
+__device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lanes, uint32_t cut, uint32_t chunk, const uint32_t* __restrict__ keys,
+                                            const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G,
+                                            int64_t ldg, float* __restrict__ part, int64_t ldp) {
+    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V * K;
+    const uint32_t a = chunk * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
     const uint32_t first = keys[a], last = keys[b - 1];
 #pragma unroll 1
     for (int end = 0; end < 2; ++end) {
@@ -339,7 +344,7 @@ k_token_pieces(int64_t n, int64_t C, int w, int lanes, uint32_t cut, const uint3
         sum.clear();
         sum.add(pos, r0 > a ? r0 : a, r1 < b ? r1 : b, G, ldg, w, col0, lanes);
         sum.join(lanes);
-        float* to = part + (2 * (int64_t)blockIdx.x + end) * ldp;
+        float* to = part + (2 * (int64_t)chunk + end) * ldp;
         if (lane < lanes)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -394,13 +399,20 @@ k_token_join(int64_t n, int64_t C, int w, int64_t ldp, int wide, uint32_t cut, c
     }
 }
 
-// every other row of dW, one wave per row and 64 V K columns
+// One wave per chunk of a long row (the first `pieces` workgroups) or per other row of dW, and 64 V K columns.  One launch for
+// both: the pieces are few waves with much to wait for, the rows many with little (101 us together, 46 + 63 us one behind the other).
 template <class T, int V, bool TAIL, int K>
 __global__ void __launch_bounds__(256)
-k_token_grad(int64_t C, int w, int lanes, uint32_t cut, const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos,
-             const T* __restrict__ G, int64_t ldg, float scale, T* __restrict__ dW, int64_t ldw) {
-    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V * K;
-    for (int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); c < C; c += (int64_t)gridDim.x * 4) {
+k_token_grad(int64_t n, int64_t C, int w, int lanes, uint32_t cut, unsigned pieces, const uint32_t* __restrict__ keys,
+             const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G, int64_t ldg,
+             float* __restrict__ part, int64_t ldp, float scale, T* __restrict__ dW, int64_t ldw) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col0 = blockIdx.y * 64 * V * K;
+    if (blockIdx.x < pieces) {
+        const uint32_t chunk = blockIdx.x * 4 + wv;
+        if ((int64_t)chunk * cut < n) token_piece<T, V, TAIL, K>(n, C, w, lanes, cut, chunk, keys, rowptr, pos, G, ldg, part, ldp);
+        return;
+    }
+    for (int64_t c = (int64_t)(blockIdx.x - pieces) * 4 + wv; c < C; c += (int64_t)(gridDim.x - pieces) * 4) {
         const uint32_t a = rowptr[c], b = rowptr[c + 1];
         if (b - a > cut) continue;
         RowSum<T, V, TAIL, K> sum;
@@ -421,23 +433,105 @@ k_token_grad(int64_t C, int w, int lanes, uint32_t cut, const uint32_t* __restri
     }
 }
 
+// ---- tables of at most FEW rows (class labels): no sort.  A wave walks `per_wave` tokens and keeps a sum of every row for its
+// 64 columns in LDS; its token is the same in all lanes, so each lane adds to its own word.  The four waves' sums are added
+// in order and go to part[workgroup][row][column], which k_token_few_join adds in order.  13,752 tokens of 10 labels x 64
+// float32: two launches and 11 us, where the sort's eight launches took 31 us.
+constexpr int FEW = 32;
+template <class T>
+__global__ void __launch_bounds__(256)
+k_token_few(int64_t n, int C, int w, int64_t padding, IndexArray tok, int64_t per_wave, const T* __restrict__ G, int64_t ldg,
+            float* __restrict__ part) {
+    __shared__ float sums[4][FEW][64];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = blockIdx.y * 64 + lane, at = col < w ? col : w - 1;
+    for (int c = 0; c < C; ++c) sums[wv][c][lane] = 0.0f;
+    const int64_t i0 = ((int64_t)blockIdx.x * 4 + wv) * per_wave, i1 = i0 + per_wave < n ? i0 + per_wave : n;
+    for (int64_t i = i0; i < i1; i += 64) {
+        const int count = i1 - i < 64 ? (int)(i1 - i) : 64;
+        const uint32_t key = token_key(tok, i + (lane < count ? lane : count - 1), C, padding);
+        for (int u0 = 0; u0 < count; u0 += 8) {
+            float g[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) g[u] = to_f32(G[(i + (u0 + u < count ? u0 + u : count - 1)) * ldg + at]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const uint32_t c = __builtin_amdgcn_readlane(key, (u0 + u) & 63);
+                if (u0 + u < count && c < (uint32_t)C) sums[wv][c][lane] = sums[wv][c][lane] + g[u];
+            }
+        }
+    }
+    __syncthreads();
+    if (col < w)
+        for (int c = wv; c < C; c += 4)
+            part[((int64_t)blockIdx.x * C + c) * w + col] = ((sums[0][c][lane] + sums[1][c][lane]) + sums[2][c][lane]) + sums[3][c][lane];
+}
+// dW from the workgroups' sums: 16 lanes of workgroups each add every 16th, then the lanes are added in order
+template <class T>
+__global__ void __launch_bounds__(1024)
+k_token_few_join(int64_t nblk, int C, int w, const float* __restrict__ part, float scale, T* __restrict__ dW, int64_t ldw) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int64_t size = (int64_t)C * w;
+    for (int64_t g0 = (int64_t)blockIdx.x * 64; g0 < size; g0 += (int64_t)gridDim.x * 64) {
+        const int64_t g = g0 + lane;
+        float acc = 0.0f;
+        if (g < size)
+#pragma unroll 8
+            for (int64_t b = wv; b < nblk; b += 16) acc = acc + part[b * size + g];
+        __syncthreads();
+        red[wv][lane] = acc;
+        __syncthreads();
+        if (wv == 0 && g < size) {
+#pragma unroll
+            for (int k = 1; k < 16; ++k) acc = acc + red[k][lane];
+            dW[g / w * ldw + g % w] = from_f32<T>(acc * scale);
+        }
+    }
+}
+// tokens a wave walks: 16 C a workgroup at least, which keeps its sums an eighth of what it reads, and at most 4096 workgroups
+static inline int64_t few_per_wave(int64_t n, int64_t C) {
+    int64_t per = 4 * C < 32 ? 32 : 4 * C;
+    while (per * 4 * 4096 < n) per *= 2;
+    return per;
+}
+static inline bool few_rows(int64_t C, int64_t w) { return C <= FEW && (w + 63) / 64 < 65536; }
+
+// fn(BITS) for the digit width of a sort, 5 to 9
+template <class Fn> static inline int with_digit(int bits, Fn&& fn) {
+    switch (bits) {
+        case 5: return fn(std::integral_constant<int, 5>{});
+        case 6: return fn(std::integral_constant<int, 6>{});
+        case 7: return fn(std::integral_constant<int, 7>{});
+        case 8: return fn(std::integral_constant<int, 8>{});
+        default: return fn(std::integral_constant<int, 9>{});
+    }
+}
+
 struct TokenLayout {
     int64_t nblk, keys[2], pos[2], counts, rowptr, part, bytes;
     uint32_t cut;
-    int passes;
+    int passes, digit;
 };
 static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
-    TokenLayout l;
+    TokenLayout l{};
+    if (few_rows(C, w)) {
+        const int64_t per = 4 * few_per_wave(n, C);
+        l.nblk = (n + per - 1) / per;
+        l.bytes = (l.nblk * C * w * 4 + 256) / 256 * 256;
+        return l;
+    }
     int bits = 1;
     while ((C >> bits) != 0) ++bits;                   // keys are 0..C
     l.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
+    l.digit = (bits + l.passes - 1) / l.passes;
+    if (l.digit < 5) l.digit = 5;                      // with_digit
     l.nblk = (n + SORT_KEYS - 1) / SORT_KEYS;
     l.cut = 64;
     while ((int64_t)l.cut * 4096 < n) l.cut *= 2;      // at most 4096 pieces of one row
     int64_t at = 0;
     auto take = [&at](int64_t words) { const int64_t p = at; at += (words * 4 + 255) / 256 * 256; return p; };
     for (int k = 0; k < 2; ++k) { l.keys[k] = take(n); l.pos[k] = take(n); }
-    l.counts = take(n > SMALL_KEYS ? l.nblk * RADIX_BINS : 0);
+    l.counts = take(n > SMALL_KEYS ? l.nblk << l.digit : 0);
     l.rowptr = take(C + 1);
     l.part = take(n > l.cut ? 2 * ((n + l.cut - 1) / l.cut) * ((w + 3) / 4 * 4) : 0);
     l.bytes = at;
@@ -490,29 +584,49 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
                "gm_token_embedding_bwd needs %lld workspace bytes (gm_token_embedding_bwd_workspace_bytes)", (long long)l.bytes);
     hipStream_t s = as_stream(stream);
     char* ws = static_cast<char*>(workspace);
+    if (few_rows(C, w)) {
+        float* few = static_cast<float*>(workspace);
+        return with_dtype(dtype, [&](auto t) -> int {
+            using T = decltype(t);
+            if (l.nblk > 0) {
+                hipLaunchKernelGGL((k_token_few<T>), dim3((unsigned)l.nblk, (unsigned)((w + 63) / 64)), dim3(256), 0, s, n, (int)C, (int)w,
+                                   padding_idx, IndexArray{tokens, tokens_i64}, few_per_wave(n, C), static_cast<const T*>(G), ldg, few);
+                GM_LAUNCH_CHECK();
+            }
+            hipLaunchKernelGGL((k_token_few_join<T>), dim3(grid_for((C * w + 63) / 64, 1024)), dim3(1024), 0, s, l.nblk, (int)C, (int)w, few,
+                               scale, static_cast<T*>(dW), ldw);
+            GM_LAUNCH_CHECK();
+            return GM_OK;
+        });
+    }
     auto u32 = [ws](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
     const IndexArray tok{tokens, tokens_i64};
     uint32_t *counts = u32(l.counts), *rowptr = u32(l.rowptr);
     const uint32_t *keys = u32(l.keys[0]), *pos = u32(l.pos[0]);
     float* part = reinterpret_cast<float*>(ws + l.part);
-    if (n > 0 && n <= SMALL_KEYS) {
-        hipLaunchKernelGGL(k_token_sort_small, dim3(1), dim3(SMALL_WAVES * 64), 0, s, (int)n, C, padding_idx, tok, l.passes,
-                           u32(l.keys[0]), u32(l.pos[0]));
-        GM_LAUNCH_CHECK();
-    }
-    for (int p = 0; p < l.passes && n > SMALL_KEYS; ++p) {
-        uint32_t *ko = u32(l.keys[p & 1]), *po = u32(l.pos[p & 1]);
-        hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
-                           p * RADIX_BITS, counts);
-        GM_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_radix_scan, dim3(1), dim3(1024), 0, s, l.nblk * RADIX_BINS, counts);
-        GM_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_radix_scatter, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
-                           p ? pos : nullptr, p * RADIX_BITS, counts, ko, po);
-        GM_LAUNCH_CHECK();
-        keys = ko;
-        pos = po;
-    }
+    const int rc = with_digit(l.digit, [&](auto digit) -> int {
+        constexpr int BITS = decltype(digit)::value;
+        if (n > 0 && n <= SMALL_KEYS) {
+            hipLaunchKernelGGL((k_token_sort_small<BITS>), dim3(1), dim3(SMALL_WAVES * 64), 0, s, (int)n, C, padding_idx, tok, l.passes,
+                               u32(l.keys[0]), u32(l.pos[0]));
+            GM_LAUNCH_CHECK();
+        }
+        for (int p = 0; p < l.passes && n > SMALL_KEYS; ++p) {
+            uint32_t *ko = u32(l.keys[p & 1]), *po = u32(l.pos[p & 1]);
+            hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr, p * BITS, BITS,
+                               counts);
+            GM_LAUNCH_CHECK();
+            hipLaunchKernelGGL(k_radix_scan, dim3(1), dim3(1024), 0, s, l.nblk << BITS, counts);
+            GM_LAUNCH_CHECK();
+            hipLaunchKernelGGL((k_radix_scatter<BITS>), dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
+                               p ? pos : nullptr, p * BITS, counts, ko, po);
+            GM_LAUNCH_CHECK();
+            keys = ko;
+            pos = po;
+        }
+        return GM_OK;
+    });
+    if (rc != GM_OK) return rc;
     hipLaunchKernelGGL(k_token_rowptr, dim3((unsigned)((C + 1 + 255) / 256)), dim3(256), 0, s, n, C, keys, rowptr);
     GM_LAUNCH_CHECK();
     const int vec = w < 16 / dtype_size(dtype) ? 1 : 16 / dtype_size(dtype);        // with_row_form
@@ -528,32 +642,28 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     while (wide < 256 && wide * 4 < w) wide *= 2;
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        int rc = GM_OK;
+        int status = GM_OK;
         with_row_form<T>(w, [&](auto v, auto tail) {
             constexpr int V = decltype(v)::value;
             constexpr bool TAIL = decltype(tail)::value;
-            rc = [&]() -> int {
+            status = [&]() -> int {
+                const unsigned pieces = n > l.cut ? (chunks + 3) / 4 : 0;
 #define GM_LAUNCH_GRAD(K_)                                                                                                \
-    do {                                                                                                                  \
-        if (n > l.cut) {                                                                                                  \
-            hipLaunchKernelGGL((k_token_pieces<T, V, TAIL, K_>), dim3(chunks, tiles), dim3(64), 0, s, n, C, (int)w, lanes, l.cut, keys, rowptr, pos, \
-                               static_cast<const T*>(G), ldg, part, ldp);                                                 \
-            GM_LAUNCH_CHECK();                                                                                            \
-            hipLaunchKernelGGL((k_token_join<T>), dim3(chunks), dim3(1024), 0, s, n, C, (int)w, ldp, wide, l.cut, keys, rowptr, part, scale, \
-                               static_cast<T*>(dW), ldw);                                                                 \
-            GM_LAUNCH_CHECK();                                                                                            \
-        }                                                                                                                 \
-        hipLaunchKernelGGL((k_token_grad<T, V, TAIL, K_>), dim3(grid_for((C + 3) / 4, 256), tiles), dim3(256), 0, s, C, (int)w, lanes,       \
-                           l.cut, rowptr, pos, static_cast<const T*>(G), ldg, scale, static_cast<T*>(dW), ldw);           \
-    } while (0)
+    hipLaunchKernelGGL((k_token_grad<T, V, TAIL, K_>), dim3(pieces + grid_for((C + 3) / 4, 512), tiles), dim3(256), 0, s, n, C, (int)w,       \
+                       lanes, l.cut, pieces, keys, rowptr, pos, static_cast<const T*>(G), ldg, part, ldp, scale,          \
+                       static_cast<T*>(dW), ldw)
                 if (K == 2) GM_LAUNCH_GRAD(2);
                 else GM_LAUNCH_GRAD(1);
 #undef GM_LAUNCH_GRAD
                 GM_LAUNCH_CHECK();
+                if (pieces) {
+                    hipLaunchKernelGGL((k_token_join<T>), dim3(chunks), dim3(1024), 0, s, n, C, (int)w, ldp, wide, l.cut, keys, rowptr, part, scale,
+                                       static_cast<T*>(dW), ldw);
+                    GM_LAUNCH_CHECK();
+                }
                 return GM_OK;
             }();
         });
-        if (rc != GM_OK) return rc;
-        return GM_OK;
+        return status;
     });
 }
