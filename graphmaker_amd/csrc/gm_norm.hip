@@ -337,12 +337,13 @@ k_layer_norm_cols(int64_t nblk, int64_t N, const float* __restrict__ part, W* __
     if (out) out[g < N ? g : g - N] = from_f32<W>(acc);
 }
 
-// Threads a row and 16-byte pieces a thread.  A wave a row while four pieces hold it (no barrier, four rows a workgroup); a
-// workgroup where they do not, or where the rows are fewer than the waves the chip wants.  tpr = 0: too wide.
+// Threads a row and 16-byte pieces a thread, from the width alone, so that a row's bits do not depend on how many others come
+// with it.  A wave a row while four pieces a lane hold it (no barrier, four rows a workgroup), then a workgroup of 256, then of
+// 1024.  tpr = 0: too wide.
 struct RowShape { int tpr, K; };
-static inline RowShape row_shape(int64_t M, int64_t N, int vec, int most, int most_lean) {
+static inline RowShape row_shape(int64_t N, int vec, int most, int most_lean) {
     const int64_t v = (N + vec - 1) / vec;
-    const int tpr = v <= 64 || (v <= 256 && M >= 1024) ? 64 : v <= 256 * most ? 256 : 1024;
+    const int tpr = v <= 64 * most ? 64 : v <= 256 * most ? 256 : 1024;
     int K = 1;
     while ((int64_t)K * tpr < v) K *= 2;
     return K > (tpr == 1024 ? most_lean : most) ? RowShape{0, 0} : RowShape{tpr, K};
@@ -380,7 +381,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
     const Weights w{gamma, beta, weight_dtype == GM_DTYPE_F32};
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const RowShape r = row_shape(M, N, VEC<T>, 4, 8);
+        const RowShape r = row_shape(N, VEC<T>, 4, 8);
 #define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)norm_blocks_fwd(M, ROWS, THREADS)), dim3(THREADS), 0, as_stream(stream), M, N, \
                        static_cast<const T*>(X), ldx, w, eps, static_cast<T*>(Y), ldy, mean, rstd)
@@ -431,7 +432,7 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
         using W = decltype(u);
         if (M > 0) {
             const Weights w{gamma, nullptr, weight_dtype == GM_DTYPE_F32};
-            const RowShape r = row_shape(M, N, VEC<T>, 4, 16 / VEC<T>);      // the sums of 16 columns a thread at 1024 threads
+            const RowShape r = row_shape(N, VEC<T>, 4, 16 / VEC<T>);      // the sums of 16 columns a thread at 1024 threads
 #define GM_LAUNCH_NORM(KERNEL, THREADS)                                                                                   \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,            \
                        static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part)

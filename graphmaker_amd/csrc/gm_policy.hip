@@ -402,10 +402,10 @@ using namespace gm;
 
 #define GM_SEQUENCE_CHECK()                                                                                               \
     GM_REQUIRE(M >= 0 && S > 0 && (M == 0 || log_prob), "bad arguments");                                                 \
-    GM_REQUIRE(M < (1ll << 40) && S < (1ll << 31), "M or the number of sequences too large")
+    GM_REQUIRE(M < (1ll << 34) && S < (1ll << 31), "2^34 items or 2^31 sequences or more")
 
 extern "C" int64_t gm_sequence_loss_workspace_bytes(int64_t M, int64_t S) {
-    if (M < 0 || S <= 0 || M >= (1ll << 40) || S >= (1ll << 31)) return -1;
+    if (M < 0 || S <= 0 || M >= (1ll << 34) || S >= (1ll << 31)) return -1;
     return sequence_layout(M, S).bytes;
 }
 
@@ -452,7 +452,7 @@ extern "C" int gm_preference_loss_fwd(int64_t M, int64_t P, const float* log_pro
 
 extern "C" int gm_sequence_loss_bwd(int64_t M, int64_t S, const float* slope, const uint8_t* mask, const void* offsets, int offsets_i64,
                                     const float* weight, const float* g, float* dlog_prob, gm_stream_t stream) {
-    GM_REQUIRE(M >= 0 && S > 0 && M < (1ll << 40) && S < (1ll << 31) && (offsets || S == 1), "bad arguments");
+    GM_REQUIRE(M >= 0 && S > 0 && M < (1ll << 34) && S < (1ll << 31) && (offsets || S == 1), "bad arguments");
     if (M == 0) return GM_OK;
     GM_REQUIRE(weight && g && dlog_prob, "bad arguments");
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};

@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
@@ -97,6 +98,8 @@ bool records(const Tensor& t) { return t.defined() && t.requires_grad() && at::G
 // Gradients of an operator without a second derivative: who differentiates them (create_graph) gets an error, not zeros.
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& t : grads)
+        if (t.defined()) t.requires_grad_(true);
     auto error = std::make_shared<torch::autograd::DelayedError>("this graphmaker_amd operator has no second derivative", (int64_t)grads.size());
     return (*error)(std::move(grads));
 }
@@ -472,6 +475,8 @@ PYBIND11_MODULE(gm_tape, m) {
             if (p) std::rethrow_exception(p);
         } catch (const HipError& e) {
             PyErr_SetString(error_class ? error_class.ptr() : PyExc_RuntimeError, e.what());
+        } catch (const c10::Error&) {                  // torch's own, such as running out of memory
+            torch::translate_exception_to_python(p);
         }
     });
     const py::call_guard<py::gil_scoped_release> no_lock;

@@ -86,7 +86,8 @@ def check_embedding(weight, tokens, scale, padding, dev, seed=1):
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("n, C, w", [(1, 1, 1), (1, 300, 8), (7, 5, 3), (64, 2, 64), (65, 511, 66), (513, 512, 33), (2049, 513, 128),
-                                     (1000, 100003, 16), (5000, 10, 65), (4097, 262145, 8), (100, 7, 1030)])
+                                     (1000, 100003, 16), (5000, 10, 65), (4097, 262145, 8), (100, 7, 1030), (8193, 33, 40),
+                                     (150001, 200000, 3), (300001, 1000, 2), (70001, 32, 9)])
 def test_token_embedding(dev, dt, n, C, w):
     g = torch.Generator().manual_seed(n + C + w)
     tokens = (torch.rand(n, generator=g) ** 3 * C).long().clamp(max=C - 1)       # low rows often, most never
@@ -190,7 +191,8 @@ def check_norm(x, gamma, beta, g, dev, eps=1e-5):
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("M, N", [(1, 1), (1, 2), (3, 7), (5, 64), (4, 65), (130, 96), (67, 512), (1, 1000), (9, 1023), (64, 1024),
-                                  (3, 2049), (2, 4096), (33, 5000), (7, 8192), (5, 16384), (2, 20001), (1, 70000), (700, 24)])
+                                  (3, 2049), (2, 4096), (33, 5000), (7, 8192), (5, 16384), (2, 20001), (1, 70000), (700, 24),
+                                  (5000, 96), (1300, 2056), (300, 16400)])
 def test_layer_norm(dev, dt, M, N):
     t = DT[dt]
     x = (rnd(N, M, N) * (1 + torch.arange(M)[:, None] % 3) + 0.7).to(t)
@@ -376,6 +378,49 @@ def test_class_log_prob_strides_shapes(dev, dt, V):
     assert ag.class_log_prob(four[:0], cc[:0]).shape == (0, 3, 4)
     e = four[:0].detach().requires_grad_(True)
     assert torch.autograd.grad(ag.class_log_prob(e, cc[:0]).sum(), [e])[0].shape == e.shape
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("V, times", [(2, 70000), (3, 9000), (7, 9000), (10, 9000), (100, 2000), (601, 600), (2049, 60), (5001, 60)])
+def test_a_row_does_not_depend_on_the_rows_around_it(dev, dt, V, times):
+    """The same 70 rows at other places of a larger batch, at other alignments and in other workgroups: the same bits, of the
+    log-probabilities and their gradients, and of layer_norm's rows."""
+    x = rnd(V, 70, V, dtype=DT[dt]).to(dev)
+    c = torch.randint(0, V, (70,), generator=torch.Generator().manual_seed(1)).to(dev)
+    g = rnd(2, 70).to(dev)
+    shift = 13                                           # the batch starts with the last rows
+    big = torch.cat([x[-shift:], x.repeat(times, 1)]).requires_grad_(True)
+    lp = ag.class_log_prob(big, torch.cat([c[-shift:], c.repeat(times)]))
+    (dx,) = torch.autograd.grad(lp, [big], torch.cat([g[-shift:], g.repeat(times)]))
+    first, grad = lp[:70], dx[:70]
+    for k in (1, times // 2, times - 1):
+        assert torch.equal(lp[70 * k:70 * k + 70], first) and torch.equal(dx[70 * k:70 * k + 70], grad)
+    y = ag.layer_norm(big.detach())
+    few = ag.layer_norm(big.detach()[:70])
+    assert torch.equal(y[:70], few) and torch.equal(y[70 * (times - 1):70 * times], few)
+
+
+def test_second_derivatives_are_refused(dev):
+    """create_graph is allowed; differentiating the gradient is an error, not silent zeros."""
+    x = rnd(1, 6, 40).to(dev).requires_grad_(True)
+    y = ag.layer_norm(x)
+    (dx,) = torch.autograd.grad(y.square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dx.sum().backward()
+    lp = ag.class_log_prob(x, torch.zeros(6, dtype=torch.int64, device=dev))
+    (dx,) = torch.autograd.grad(lp.square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dx.sum().backward()
+
+
+def test_tensors_on_different_devices_are_refused(dev):
+    W, x = torch.zeros(4, 8, device=dev), torch.zeros(6, device=dev)
+    for call in (lambda: ag.token_embedding(W, torch.zeros(3, dtype=torch.int64)), lambda: ag.layer_norm(W, torch.ones(8)),
+                 lambda: ag.class_log_prob(W, torch.zeros(4, dtype=torch.int64)), lambda: ag.policy_loss(x, torch.zeros(6), x),
+                 lambda: ag.policy_loss(x, x, x, mask=torch.ones(6, dtype=torch.bool)),
+                 lambda: ag.preference_loss(x, x, torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="expected cuda"):
+            call()
 
 
 def test_class_log_prob_equals_the_two_class_cross_entropy(dev):
