@@ -20,8 +20,9 @@ float32, bfloat16 or float16 rows, sums in float32 or float64):
     policy_loss(log_prob, old_log_prob, advantage, ...)            clipped policy loss with a KL term
     preference_loss(log_prob, ref_log_prob, offsets, ...)          loss of preferred over rejected sequences
 They enqueue on the current stream of their tensors' device, keep their workspaces to one call, read nothing back to the
-host and can be captured in a HIP graph, forward and backward.  Capture a backward pass only when no graph recorded eagerly
-over the same leaf tensors is still alive: torch ties a leaf's gradient accumulation to the stream of the first such graph.
+host and can be captured in a HIP graph, forward and backward.  A captured call is refused while a graph that was recorded
+eagerly on another stream over the same leaf tensor is alive (torch runs the leaf's gradient accumulation on that stream, and
+the process would end): drop such graphs, their losses and outputs, before capturing.
 """
 import ctypes
 

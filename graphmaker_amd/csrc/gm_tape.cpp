@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -93,7 +94,22 @@ const uint8_t* bytes(const Tensor& t) { return static_cast<const uint8_t*>(at_of
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
 Tensor workspace(int64_t size, const Tensor& like) { return size > 0 ? empty({size}, at::kByte, like) : Tensor(); }
 
-bool records(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+// Whether a call on t is recorded.  A captured call on a leaf whose gradient is accumulated on another stream is refused:
+// torch ties a leaf's accumulation to the stream of the first graph that is alive, a backward pass inside the capture would
+// run it there, and that ends the process.
+bool records(const Tensor& t) {
+    if (!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled()) return false;
+    if (t.is_leaf() && t.is_cuda()) {
+        const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t.device().index());
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(now.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone) {
+            const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+            if (node && node->stream() && node->stream()->id() != now.id())
+                throw HipError("captured while a graph recorded on another stream over the same leaf tensor is alive: drop that graph first");
+        }
+    }
+    return true;
+}
 
 // Gradients of an operator without a second derivative: who differentiates them (create_graph) gets an error, not zeros.
 variable_list once(variable_list grads) {

@@ -752,6 +752,32 @@ def test_fine_tuning_step_in_a_graph(dev):
                 assert torch.equal(got, w), (turn, k)
 
 
+def test_capture_beside_a_living_eager_graph_is_refused(dev):
+    """Refused before anything is captured; fine once the eager graph is gone, and with leaves that it does not hold."""
+    x, w = rnd(1, 30, 64).to(dev), (1 + 0.1 * rnd(2, 64)).to(dev).requires_grad_(True)
+    emb = rnd(3, 40, 64).to(dev).requires_grad_(True)
+    tok = torch.arange(30, device=dev)
+    alive = ag.layer_norm(x, w)                          # recorded eagerly on the default stream
+    held = ag.token_embedding(emb, tok)
+    torch.cuda.synchronize()
+    for call in (lambda: ag.layer_norm(x, w), lambda: ag.token_embedding(emb, tok)):
+        with pytest.raises(RuntimeError, match="same leaf tensor is alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive, held
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ag.layer_norm(x, w)
+        y = y + ag.layer_norm(y, w)                      # the same leaf twice inside the capture
+        (dw,) = torch.autograd.grad(y.sum(), [w])
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        z = ag.layer_norm(x, w)
+        z = z + ag.layer_norm(z, w)
+        assert torch.equal(z, y) and torch.equal(torch.autograd.grad(z.sum(), [w])[0], dw)
+
+
 def test_upstream_gradients_and_inplace_loss(dev):
     """The losses are ordinary scalars: scaled in place, summed, used twice, or not used at all."""
     lp, old, _ = (t.to(dev) for t in ratios(4, 500))
