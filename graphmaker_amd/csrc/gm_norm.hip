@@ -371,7 +371,7 @@ using namespace gm;
     GM_REQUIRE(M >= 0 && N > 0, "bad arguments");                                                                         \
     GM_REQUIRE(dtype_ok(dtype) && (weight_dtype == dtype || weight_dtype == GM_DTYPE_F32),                                \
                "dtype %d with weight_dtype %d: the weights have the rows' type or are float32", dtype, weight_dtype);     \
-    GM_REQUIRE(M < (1ll << 31) && N < (1ll << 30), "M of 2^31 or more, or N of 2^30 or more")
+    GM_REQUIRE(M < (1ll << 31) && N < (1ll << 26), "M of 2^31 or more, or N of 2^26 or more")
 
 extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ldx, int dtype, const void* gamma, const void* beta,
                                  int weight_dtype, float eps, void* Y, int64_t ldy, float* mean, float* rstd, gm_stream_t stream) {
@@ -412,7 +412,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
 }
 
 extern "C" int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
-    if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 30)) return -1;
+    if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 26)) return -1;
     return norm_blocks(M) * 2 * N * 4;
 }
 

@@ -181,75 +181,84 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
     }
 }
 
-// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch.  Wave wv holds keys
-// [wv * 1024, wv * 1024 + 1024) of the current order in registers and exchanges them through LDS.
-constexpr int SMALL_WAVES = 8, SMALL_ROUNDS = 16, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64;
+// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch.  Each wave holds `rounds` x 64 keys that
+// are consecutive in the current order in registers; the keys change places through LDS.
+constexpr int SMALL_WAVES = 16, SMALL_ROUNDS = 8, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64, SMALL_BITS = 8;
 template <int BITS>
 __global__ void __launch_bounds__(SMALL_WAVES * 64)
 k_token_sort_small(int n, int64_t C, int64_t padding, IndexArray tok, int passes, uint32_t* __restrict__ keys_out,
                    uint32_t* __restrict__ pos_out) {
-    __shared__ uint32_t next[SMALL_WAVES][RADIX_BINS];
-    __shared__ uint32_t buf[SMALL_KEYS];
-    __shared__ uint32_t tot[SMALL_WAVES];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    static_assert(BITS <= SMALL_BITS, "a thread a digit in the first four waves, and the counts' place in LDS");
     constexpr int bins = 1 << BITS;
+    __shared__ uint32_t next[SMALL_WAVES][bins];
+    __shared__ uint32_t buf[SMALL_KEYS];
+    __shared__ uint32_t tot[4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int rounds = (n + SMALL_WAVES * 64 - 1) / (SMALL_WAVES * 64);
     uint32_t key[SMALL_ROUNDS], pos[SMALL_ROUNDS];
 #pragma unroll
     for (int r = 0; r < SMALL_ROUNDS; ++r) {
-        const int i = (wv * SMALL_ROUNDS + r) * 64 + lane;
+        const int i = (wv * rounds + r) * 64 + lane;
         pos[r] = (uint32_t)i;
-        key[r] = i < n ? token_key(tok, i, C, padding) : 0xFFFFFFFFu;         // behind every key in every digit: stays last
+        key[r] = r < rounds && i < n ? token_key(tok, i, C, padding) : 0;
     }
     for (int p = 0; p < passes; ++p) {
         const int shift = p * BITS;
-        for (int b = threadIdx.x; b < SMALL_WAVES * RADIX_BINS; b += SMALL_WAVES * 64) (&next[0][0])[b] = 0;
+        for (int b = threadIdx.x; b < SMALL_WAVES * bins; b += SMALL_WAVES * 64) (&next[0][0])[b] = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r) atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
+        for (int r = 0; r < SMALL_ROUNDS; ++r)
+            if (r < rounds && (wv * rounds + r) * 64 + lane < n) atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
         __syncthreads();
-        // thread b owns digit b: starts of the digits by a scan over the workgroup, then of each wave's share of its digit
-        static_assert(RADIX_BINS == SMALL_WAVES * 64, "one thread a digit");
-        uint32_t sum = 0;
+        // thread b owns digit b: the digits' starts by a scan, then the start of each wave's share
+        uint32_t sum = 0, s = 0;
+        if (threadIdx.x < 256) {
+            if (threadIdx.x < bins)
 #pragma unroll
-        for (int k = 0; k < SMALL_WAVES; ++k) sum += next[k][threadIdx.x];
-        uint32_t s = sum;
+                for (int k = 0; k < SMALL_WAVES; ++k) sum += next[k][threadIdx.x];
+            s = sum;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t t = __shfl_up(s, off);
-            if (lane >= off) s += t;
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t t = __shfl_up(s, off);
+                if (lane >= off) s += t;
+            }
+            if (lane == 63) tot[wv] = s;
         }
-        if (lane == 63) tot[wv] = s;
         __syncthreads();
-        uint32_t at = s - sum;
-        for (int k = 0; k < wv; ++k) at += tot[k];
+        if (threadIdx.x < bins) {
+            uint32_t at = s - sum;
+            for (int k = 0; k < wv; ++k) at += tot[k];
 #pragma unroll
-        for (int k = 0; k < SMALL_WAVES; ++k) {
-            const uint32_t c = next[k][threadIdx.x];
-            next[k][threadIdx.x] = at;
-            at += c;
+            for (int k = 0; k < SMALL_WAVES; ++k) {
+                const uint32_t c = next[k][threadIdx.x];
+                next[k][threadIdx.x] = at;
+                at += c;
+            }
         }
         __syncthreads();
         uint32_t place[SMALL_ROUNDS];
 #pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r) {
-            const uint32_t d = (key[r] >> shift) & (bins - 1);
-            place[r] = take_place<BITS>(next[wv], d, true, lane);
-        }
+        for (int r = 0; r < SMALL_ROUNDS; ++r)
+            if (r < rounds) place[r] = take_place<BITS>(next[wv], (key[r] >> shift) & (bins - 1), (wv * rounds + r) * 64 + lane < n, lane);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             uint32_t(&x)[SMALL_ROUNDS] = half ? pos : key;
 #pragma unroll
-            for (int r = 0; r < SMALL_ROUNDS; ++r) buf[place[r]] = x[r];
+            for (int r = 0; r < SMALL_ROUNDS; ++r)
+                if (r < rounds && (wv * rounds + r) * 64 + lane < n) buf[place[r]] = x[r];
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < SMALL_ROUNDS; ++r) x[r] = buf[(wv * SMALL_ROUNDS + r) * 64 + lane];
+            for (int r = 0; r < SMALL_ROUNDS; ++r) {
+                const int i = (wv * rounds + r) * 64 + lane;
+                if (r < rounds && i < n) x[r] = buf[i];
+            }
             __syncthreads();
         }
     }
 #pragma unroll
     for (int r = 0; r < SMALL_ROUNDS; ++r) {
-        const int i = (wv * SMALL_ROUNDS + r) * 64 + lane;
-        if (i < n) {
+        const int i = (wv * rounds + r) * 64 + lane;
+        if (r < rounds && i < n) {
             keys_out[i] = key[r];
             pos_out[i] = pos[r];
         }
@@ -522,7 +531,8 @@ static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
     }
     int bits = 1;
     while ((C >> bits) != 0) ++bits;                   // keys are 0..C
-    l.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
+    const int most = n > SMALL_KEYS ? RADIX_BITS : SMALL_BITS;
+    l.passes = (bits + most - 1) / most;
     l.digit = (bits + l.passes - 1) / l.passes;
     if (l.digit < 5) l.digit = 5;                      // with_digit
     l.nblk = (n + SORT_KEYS - 1) / SORT_KEYS;
@@ -606,10 +616,12 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     float* part = reinterpret_cast<float*>(ws + l.part);
     const int rc = with_digit(l.digit, [&](auto digit) -> int {
         constexpr int BITS = decltype(digit)::value;
-        if (n > 0 && n <= SMALL_KEYS) {
-            hipLaunchKernelGGL((k_token_sort_small<BITS>), dim3(1), dim3(SMALL_WAVES * 64), 0, s, (int)n, C, padding_idx, tok, l.passes,
-                               u32(l.keys[0]), u32(l.pos[0]));
-            GM_LAUNCH_CHECK();
+        if constexpr (BITS <= SMALL_BITS) {
+            if (n > 0 && n <= SMALL_KEYS) {
+                hipLaunchKernelGGL((k_token_sort_small<BITS>), dim3(1), dim3(SMALL_WAVES * 64), 0, s, (int)n, C, padding_idx, tok, l.passes,
+                                   u32(l.keys[0]), u32(l.pos[0]));
+                GM_LAUNCH_CHECK();
+            }
         }
         for (int p = 0; p < l.passes && n > SMALL_KEYS; ++p) {
             uint32_t *ko = u32(l.keys[p & 1]), *po = u32(l.pos[p & 1]);

@@ -169,7 +169,8 @@ def test_workspace_sizes():
     assert lib.gm_token_embedding_bwd_workspace_bytes(-1, 5, 8) == -1
     assert lib.gm_token_embedding_bwd_workspace_bytes(BIG, 5, 8) == -1
     assert lib.gm_layer_norm_bwd_workspace_bytes(0, 8) >= 0
-    assert lib.gm_layer_norm_bwd_workspace_bytes(8, 0) == -1
+    assert lib.gm_layer_norm_bwd_workspace_bytes(8, 0) == -1 == lib.gm_layer_norm_bwd_workspace_bytes(8, 1 << 26)
+    assert lib.gm_class_log_prob_stats_floats(8, 1 << 28, 1) == -1 == lib.gm_sequence_loss_workspace_bytes(1 << 34, 1)
     assert lib.gm_class_log_prob_workspace_bytes(8, 0, 0) == -1 == lib.gm_class_log_prob_workspace_bytes(8, 8, 3)
     assert lib.gm_class_log_prob_stats_floats(8, 3, 0) == 0 and lib.gm_class_log_prob_stats_floats(8, 4, 0) == 16
     assert lib.gm_class_log_prob_stats_floats(8, 7, 1) == 0 and lib.gm_class_log_prob_stats_floats(8, 8, 1) == 16
