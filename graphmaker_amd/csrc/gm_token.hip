@@ -279,35 +279,29 @@ k_token_rowptr(int64_t n, int64_t C, const uint32_t* __restrict__ keys, uint32_t
     rowptr[c] = (uint32_t)lo;
 }
 
-// ---- sums of gradient rows.  A wave covers K x 64 x V columns, or a narrow row with `lanes` lanes (a power of two) and
+// ---- sums of gradient rows.  A wave covers 64 x V columns, or a narrow row with `lanes` lanes (a power of two) and
 // per = 64 / lanes rows side by side, joined at the end.  The lanes fetch 64 positions at once; the rows of up to 8 rounds
 // are then in flight together (walked one by one, each row waits for its position and then for itself).
-template <class T, int V, bool TAIL, int K>
+template <class T, int V, bool TAIL>
 struct RowSum {
-    float acc[K][V];
+    float acc[V];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[k][v] = 0.0f;
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
     }
     // R rounds from round r; an entry behind the last one loads from the last one's row and sees zeros
     template <int R>
     __device__ __forceinline__ void rounds(int r, int count, int sub, int per, uint32_t p, const T* __restrict__ G, int64_t ldg, int w, int col) {
-        Vec<T, V> x[R][K];
+        Vec<T, V> x[R];
 #pragma unroll
         for (int u = 0; u < R; ++u) {
             const int e = (r + u) * per + sub;
-            const T* row = G + (int64_t)__shfl(p, e & 63) * ldg;
-#pragma unroll
-            for (int k = 0; k < K; ++k) x[u][k] = load_vec<T, V, TAIL>(row, e < count ? col + k * 64 * V : w, w);
+            x[u] = load_vec<T, V, TAIL>(G + (int64_t)__shfl(p, e & 63) * ldg, e < count ? col : w, w);
         }
 #pragma unroll
         for (int u = 0; u < R; ++u)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[k][v] = acc[k][v] + to_f32(x[u][k].v[v]);
+            for (int v = 0; v < V; ++v) acc[v] = acc[v] + to_f32(x[u].v[v]);
     }
     // rows at the sorted positions [a, b)
     __device__ __forceinline__ void add(const uint32_t* __restrict__ pos, uint32_t a, uint32_t b, const T* __restrict__ G, int64_t ldg, int w,
@@ -327,20 +321,18 @@ struct RowSum {
     __device__ __forceinline__ void join(int lanes) {
         for (int off = 32; off >= lanes; off >>= 1)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[k][v] = acc[k][v] + __shfl_xor(acc[k][v], off);
+            for (int v = 0; v < V; ++v) acc[v] = acc[v] + __shfl_xor(acc[v], off);
     }
 };
 
 // A row of more than `cut` tokens is summed in pieces, one for each chunk of `cut` sorted positions that it meets:
 // part[2k] of the row that chunk k begins with, part[2k+1] of the row that it ends with and did not begin with.  Such a row
 // meets at least two chunks, so a chunk holds pieces of at most two of them.
-template <class T, int V, bool TAIL, int K>
+template <class T, int V, bool TAIL>
 __device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lanes, uint32_t cut, uint32_t chunk, const uint32_t* __restrict__ keys,
                                             const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G,
                                             int64_t ldg, float* __restrict__ part, int64_t ldp) {
-    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V * K;
+    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V;
     const uint32_t a = chunk * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
     const uint32_t first = keys[a], last = keys[b - 1];
 #pragma unroll 1
@@ -349,19 +341,16 @@ __device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lan
         if (c >= C || (end && last == first)) continue;
         const uint32_t r0 = rowptr[c], r1 = rowptr[c + 1];
         if (r1 - r0 <= cut) continue;
-        RowSum<T, V, TAIL, K> sum;
+        RowSum<T, V, TAIL> sum;
         sum.clear();
         sum.add(pos, r0 > a ? r0 : a, r1 < b ? r1 : b, G, ldg, w, col0, lanes);
         sum.join(lanes);
         float* to = part + (2 * (int64_t)chunk + end) * ldp;
+        const int col = col0 + lane * V;
         if (lane < lanes)
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int col = col0 + (lane + k * 64) * V;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (col + v < w) to[col + v] = sum.acc[k][v];
-            }
+            for (int v = 0; v < V; ++v)
+                if (col + v < w) to[col + v] = sum.acc[v];
     }
 }
 
@@ -408,37 +397,34 @@ k_token_join(int64_t n, int64_t C, int w, int64_t ldp, int wide, uint32_t cut, c
     }
 }
 
-// One wave per chunk of a long row (the first `pieces` workgroups) or per other row of dW, and 64 V K columns.  One launch for
-// both: the pieces are few waves with much to wait for, the rows many with little (101 us together, 46 + 63 us one behind the other).
-template <class T, int V, bool TAIL, int K>
+// One wave per chunk of a long row (the first `pieces` workgroups) or per other row of dW, and 64 V columns.  One launch for
+// both: the pieces are few waves with much to wait for, the rows many with little (99 us together, 46 + 63 us one behind the other).
+template <class T, int V, bool TAIL>
 __global__ void __launch_bounds__(256)
 k_token_grad(int64_t n, int64_t C, int w, int lanes, uint32_t cut, unsigned pieces, const uint32_t* __restrict__ keys,
              const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G, int64_t ldg,
              float* __restrict__ part, int64_t ldp, float scale, T* __restrict__ dW, int64_t ldw) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col0 = blockIdx.y * 64 * V * K;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col0 = blockIdx.y * 64 * V;
     if (blockIdx.x < pieces) {
         const uint32_t chunk = blockIdx.x * 4 + wv;
-        if ((int64_t)chunk * cut < n) token_piece<T, V, TAIL, K>(n, C, w, lanes, cut, chunk, keys, rowptr, pos, G, ldg, part, ldp);
+        if ((int64_t)chunk * cut < n) token_piece<T, V, TAIL>(n, C, w, lanes, cut, chunk, keys, rowptr, pos, G, ldg, part, ldp);
         return;
     }
     for (int64_t c = (int64_t)(blockIdx.x - pieces) * 4 + wv; c < C; c += (int64_t)(gridDim.x - pieces) * 4) {
         const uint32_t a = rowptr[c], b = rowptr[c + 1];
         if (b - a > cut) continue;
-        RowSum<T, V, TAIL, K> sum;
+        RowSum<T, V, TAIL> sum;
         sum.clear();
         if (a < b) {
             sum.add(pos, a, b, G, ldg, w, col0, lanes);
             sum.join(lanes);
         }
-        if (lane < lanes)
+        if (lane < lanes) {
+            float y[V];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int col = col0 + (lane + k * 64) * V;
-                float y[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) y[v] = sum.acc[k][v] * scale;
-                store_vec<T, V, TAIL>(dW + c * ldw, col, w, y);
-            }
+            for (int v = 0; v < V; ++v) y[v] = sum.acc[v] * scale;
+            store_vec<T, V, TAIL>(dW + c * ldw, col0 + lane * V, w, y);
+        }
     }
 }
 
@@ -645,8 +631,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     const int64_t vecs = (w + vec - 1) / vec;
     int lanes = 64;
     while (lanes > 1 && lanes / 2 >= vecs) lanes /= 2;
-    const int K = vecs > 64 ? 2 : 1;                    // a wave's two accesses to each row of a wide table
-    const unsigned tiles = (unsigned)((vecs + 64 * K - 1) / (64 * K));
+    const unsigned tiles = (unsigned)((vecs + 63) / 64);
     const unsigned chunks = (unsigned)((n + l.cut - 1) / l.cut);
     GM_REQUIRE(tiles < 65536u, "w too large");
     const int64_t ldp = (w + 3) / 4 * 4;
@@ -660,13 +645,9 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
             constexpr bool TAIL = decltype(tail)::value;
             status = [&]() -> int {
                 const unsigned pieces = n > l.cut ? (chunks + 3) / 4 : 0;
-#define GM_LAUNCH_GRAD(K_)                                                                                                \
-    hipLaunchKernelGGL((k_token_grad<T, V, TAIL, K_>), dim3(pieces + grid_for((C + 3) / 4, 512), tiles), dim3(256), 0, s, n, C, (int)w,       \
-                       lanes, l.cut, pieces, keys, rowptr, pos, static_cast<const T*>(G), ldg, part, ldp, scale,          \
-                       static_cast<T*>(dW), ldw)
-                if (K == 2) GM_LAUNCH_GRAD(2);
-                else GM_LAUNCH_GRAD(1);
-#undef GM_LAUNCH_GRAD
+                hipLaunchKernelGGL((k_token_grad<T, V, TAIL>), dim3(pieces + grid_for((C + 3) / 4, 512), tiles), dim3(256), 0, s, n, C, (int)w,
+                                   lanes, l.cut, pieces, keys, rowptr, pos, static_cast<const T*>(G), ldg, part, ldp, scale,
+                                   static_cast<T*>(dW), ldw);
                 GM_LAUNCH_CHECK();
                 if (pieces) {
                     hipLaunchKernelGGL((k_token_join<T>), dim3(chunks), dim3(1024), 0, s, n, C, (int)w, ldp, wide, l.cut, keys, rowptr, part, scale,

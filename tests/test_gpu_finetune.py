@@ -705,6 +705,35 @@ def test_fine_tuning_step_against_differences(dev):
         assert abs((up - down) / (2 * step) - slope) <= tol, (name, (up - down) / (2 * step), slope, tol)
 
 
+def test_policy_step_of_the_denoiser(dev):
+    """A node tower's attribute draws: at ratio 1 and advantage 1 the policy loss is -1 and has the gradient of the mean cross
+    entropy, which softmax_ce2 gives for the same logits.  The two logit gradients differ by a few roundings of each element
+    and go through the same backward kernels: 64 u of each sum's terms, taken as 64 times the largest gradient."""
+    import graphmaker_amd as gm
+    from graphmaker_amd import ops
+    torch.manual_seed(0)
+    n, F, Y = 90, 12, 4
+    tower = gm.GNNTower(num_attrs_X=F, num_classes_X=2, num_classes_Y=Y, hidden_t=8, hidden_X=32, hidden_Y=16, out_size=2 * F,
+                        num_gnn_layers=2, dropout=0.0, node_mode=True).to(dev).train()
+    E = (torch.rand(n, n, generator=torch.Generator().manual_seed(1)) < 0.1).long().triu(1)
+    adj = ops.adjacency_from_bitmap(ops.bitmap_from_dense((E + E.t()).to(dev)), n)
+    g = torch.Generator().manual_seed(2)
+    x_t, drawn = (torch.randint(0, 2, (n, F), generator=g) for _ in range(2))
+    X = torch.nn.functional.one_hot(x_t, 2).float().reshape(n, -1).to(dev)
+    labels = torch.randint(0, Y, (n,), generator=g).to(dev)
+    t = torch.tensor([0.5], device=dev)
+    logits = tower(t, X, labels, adj)
+    ce = ag.softmax_ce2(logits.reshape(-1, 2), drawn.to(torch.uint8).reshape(-1).to(dev))
+    want = torch.autograd.grad(ce, list(tower.parameters()))
+    lp = ag.class_log_prob(tower(t, X, labels, adj), drawn.to(dev))
+    assert lp.shape == (n, F)
+    loss, stats = ag.policy_loss(lp, lp.detach(), torch.ones(1, device=dev), offsets=torch.tensor([0, n * F], device=dev))
+    got = torch.autograd.grad(loss, list(tower.parameters()))
+    assert abs(float(loss.detach()) + 1.0) <= 2 * U and stats.tolist()[2:] == [0.0, float(n * F)]
+    for (name, _), a, b in zip(tower.named_parameters(), got, want):
+        close(a, b.cpu(), 64 * 64 * U * b.abs().max().item() + 1e-9, name)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_fine_tuning_step_is_reproducible_on_any_stream(dev, dt):
     p, batch = fine_tuning_setup(dev, DT[dt])
