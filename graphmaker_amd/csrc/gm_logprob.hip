@@ -259,7 +259,7 @@ k_log_prob_join(int N, int parts, const float2* __restrict__ part, const T* __re
 }
 
 // columns head + [blockIdx.y * span, + span) of a row, span = LONG_PIECES steps, the head with the first
-template <class T>
+template <class T, bool PAST>
 __global__ void __launch_bounds__(256)
 k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore,
                     const float2* __restrict__ stats, T* __restrict__ dX, int64_t lddx) {
@@ -284,7 +284,7 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
         const bool whole = head + (int)(blockIdx.y + 1) * (LONG_PIECES * STEP) <= N;          // uniform
         if (whole) {
 #pragma unroll
-            for (int u = 0; u < LONG_PIECES; ++u) r[u] = *reinterpret_cast<const Vec<T, V>*>(row + j + u * STEP);
+            for (int u = 0; u < LONG_PIECES; ++u) r[u] = get_vec<PAST, T, V>(row + j + u * STEP);
         } else {
 #pragma unroll
             for (int u = 0; u < LONG_PIECES; ++u) r[u] = load_vec<T, V, true>(row, j + u * STEP, N);
@@ -306,7 +306,7 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
                 Vec<T, V> d;
 #pragma unroll
                 for (int i = 0; i < V; ++i) d.v[i] = from_f32<T>(y[i]);
-                *reinterpret_cast<Vec<T, V>*>(out + col) = d;
+                put_vec<PAST, T, V>(out + col, d);
             } else {
                 store_vec<T, V, true>(out, col, N, y);
             }
@@ -466,8 +466,10 @@ extern "C" int gm_class_log_prob_bwd(int64_t M, int64_t V, const float* g, const
         } else {
             const int64_t span = LONG_PIECES * 256 * VEC<T>, parts = (V + span - 1) / span;
             const int64_t most = ((1ll << 32) - 1) / 256 / parts;              // a launch has less than 2^32 threads in all
-            hipLaunchKernelGGL((k_log_prob_long_bwd<T>), dim3((unsigned)(M < most ? M : most), (unsigned)parts), dim3(256), 0, s, M, (int)V, g, X,
+            with_past(2 * M * V * (int64_t)sizeof(T), [&](auto past) {
+                hipLaunchKernelGGL((k_log_prob_long_bwd<T, decltype(past)::value>), dim3((unsigned)(M < most ? M : most), (unsigned)parts), dim3(256), 0, s, M, (int)V, g, X,
                                ldx, cls, ignore_index, st, dX, lddx);
+            });
         }
         GM_LAUNCH_CHECK();
         return GM_OK;
