@@ -9,7 +9,7 @@
 //
 // HBM-bound: the forward reads the logits once, the backward reads them and writes as much.  Three forms by the row's size:
 //   narrow   under 16 bytes: one thread a row, which forms the softmax again in the backward instead of keeping stats
-//   held     up to 4 pieces of 16 bytes a lane: 1 to 64 lanes a row, the row in registers
+//   held     up to 5 pieces of 16 bytes a lane: 1 to 64 lanes a row, the row in registers
 //   long     a workgroup a row, or several where rows are few, with one running (maximum, sum) a thread
 #include "gm_rows.h"
 
@@ -76,7 +76,9 @@ k_log_prob_narrow(int64_t M, const float* __restrict__ g, const T* __restrict__ 
     }
 }
 
-// ---- held: LANES lanes a row, K pieces of V elements a lane
+// ---- held: LANES lanes a row, K pieces of V elements a lane.  Rows of 64 lanes add enough terms for exp_quick; with exp_any
+// the forward of rows of 256 to 2000 bf16 logits is bound by its arithmetic (3.7 to 4.2 TB/s).
+template <int LANES> __device__ __forceinline__ float exp_row(float x) { return LANES == 64 ? exp_quick(x) : exp_any(x); }
 template <class T, int V, bool TAIL, int K, int LANES>
 __global__ void __launch_bounds__(256)
 k_log_prob_held(int64_t M, int N, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore, float* __restrict__ lp,
@@ -101,7 +103,7 @@ k_log_prob_held(int64_t M, int N, const T* __restrict__ X, int64_t ldx, IndexArr
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s = s + exp_any(or_neg_inf(to_f32(r[k].v[i]), (k * LANES + t) * V + i < N) - mx);
+            for (int i = 0; i < V; ++i) s = s + exp_row<LANES>(or_neg_inf(to_f32(r[k].v[i]), (k * LANES + t) * V + i < N) - mx);
 #pragma unroll
         for (int off = LANES / 2; off >= 1; off >>= 1) s = s + __shfl_xor(s, off);
         if (t == 0) {
@@ -131,7 +133,7 @@ k_log_prob_held_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
             float y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float v = -gu * exp_any((to_f32(r[k].v[i]) - st.x) - st.y);
+                const float v = -gu * exp_row<LANES>((to_f32(r[k].v[i]) - st.x) - st.y);
                 y[i] = gu == 0.0f ? 0.0f : (col + i == c ? gu + v : v) + bad;
             }
             store_vec<T, V, TAIL>(dX + m * lddx, col, N, y);
@@ -347,8 +349,8 @@ static inline LogProbShape log_prob_shape(int64_t N, int vec) {
     const int64_t v = (N + vec - 1) / vec;
     int lanes = 1, K = 1;
     while (lanes < 64 && lanes < v) lanes *= 2;
-    while ((int64_t)lanes * K < v) K *= 2;
-    return K > 4 ? LogProbShape{0, 0} : LogProbShape{lanes, K};
+    while ((int64_t)lanes * K < v) ++K;
+    return K > 5 ? LogProbShape{0, 0} : LogProbShape{lanes, K};
 }
 static inline int64_t held_blocks(int64_t M, int lanes) {
     const int64_t want = (M + 256 / lanes - 1) / (256 / lanes);
@@ -366,16 +368,18 @@ template <class T, class Fn> static inline void with_held(int64_t N, Fn&& fn) {
             const LogProbShape r = log_prob_shape(N, VEC<T>);
             auto with = [&](auto lanes, auto k) { fn(v, tail, k, lanes); };
             using std::integral_constant;
-            switch (r.lanes * 8 + r.K) {
-                case 1 * 8 + 1: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
-                case 2 * 8 + 1: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;
-                case 4 * 8 + 1: with(integral_constant<int, 4>{}, integral_constant<int, 1>{}); break;
-                case 8 * 8 + 1: with(integral_constant<int, 8>{}, integral_constant<int, 1>{}); break;
-                case 16 * 8 + 1: with(integral_constant<int, 16>{}, integral_constant<int, 1>{}); break;
-                case 32 * 8 + 1: with(integral_constant<int, 32>{}, integral_constant<int, 1>{}); break;
-                case 64 * 8 + 1: with(integral_constant<int, 64>{}, integral_constant<int, 1>{}); break;
-                case 64 * 8 + 2: with(integral_constant<int, 64>{}, integral_constant<int, 2>{}); break;
-                default: with(integral_constant<int, 64>{}, integral_constant<int, 4>{}); break;
+            switch (r.lanes * 16 + r.K) {
+                case 1 * 16 + 1: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
+                case 2 * 16 + 1: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;
+                case 4 * 16 + 1: with(integral_constant<int, 4>{}, integral_constant<int, 1>{}); break;
+                case 8 * 16 + 1: with(integral_constant<int, 8>{}, integral_constant<int, 1>{}); break;
+                case 16 * 16 + 1: with(integral_constant<int, 16>{}, integral_constant<int, 1>{}); break;
+                case 32 * 16 + 1: with(integral_constant<int, 32>{}, integral_constant<int, 1>{}); break;
+                case 64 * 16 + 1: with(integral_constant<int, 64>{}, integral_constant<int, 1>{}); break;
+                case 64 * 16 + 2: with(integral_constant<int, 64>{}, integral_constant<int, 2>{}); break;
+                case 64 * 16 + 3: with(integral_constant<int, 64>{}, integral_constant<int, 3>{}); break;
+                case 64 * 16 + 4: with(integral_constant<int, 64>{}, integral_constant<int, 4>{}); break;
+                default: with(integral_constant<int, 64>{}, integral_constant<int, 5>{}); break;
             }
         }
     });

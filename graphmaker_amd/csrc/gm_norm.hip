@@ -39,8 +39,13 @@ struct Weights {
 
 // sum of v over the TPR threads of a row, in each of them.  `red` holds one float a wave and is a fresh one at every call
 // between two barriers of the workgroup.
+template <int TPR> __device__ __forceinline__ float lanes_add(float v) {
+#pragma unroll
+    for (int off = (TPR < 64 ? TPR : 64) / 2; off >= 1; off >>= 1) v = v + __shfl_xor(v, off);
+    return v;
+}
 template <int TPR> __device__ __forceinline__ float row_add(float v, float* red) {
-    v = wave_add(v);
+    v = lanes_add<TPR>(v);
     if (TPR > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -53,8 +58,8 @@ template <int TPR> __device__ __forceinline__ float row_add(float v, float* red)
 
 // the same of two values behind one barrier
 template <int TPR> __device__ __forceinline__ void row_add(float& a, float& b, float (*red)[16]) {
-    a = wave_add(a);
-    b = wave_add(b);
+    a = lanes_add<TPR>(a);
+    b = lanes_add<TPR>(b);
     if (TPR > 64) {
         if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = a; red[1][threadIdx.x >> 6] = b; }
         __syncthreads();
@@ -338,15 +343,17 @@ k_layer_norm_cols(int64_t nblk, int64_t N, const float* __restrict__ part, W* __
 }
 
 // Threads a row and 16-byte pieces a thread, from the width alone, so that a row's bits do not depend on how many others come
-// with it.  A wave a row while four pieces a lane hold it (no barrier, four rows a workgroup), then a workgroup of 256, then of
-// 1024.  tpr = 0: too wide.
+// with it: as few threads as hold the row in four pieces, 8 to a wave (no barrier, several rows a workgroup; 2.8 million rows of
+// 24 bf16 took 746 us with a wave each and 96 us with 8 lanes), then 256, 512 and 1024.  tpr = 0: too wide.
 struct RowShape { int tpr, K; };
-static inline RowShape row_shape(int64_t N, int vec, int most, int most_lean) {
+static inline RowShape row_shape(int64_t N, int vec, int most) {
     const int64_t v = (N + vec - 1) / vec;
-    const int tpr = v <= 64 * most ? 64 : v <= 256 * most ? 256 : 1024;
-    int K = 1;
-    while ((int64_t)K * tpr < v) K *= 2;
-    return K > (tpr == 1024 ? most_lean : most) ? RowShape{0, 0} : RowShape{tpr, K};
+    if (v <= 8) return {8, 1};
+    if (v <= 16) return {16, 1};
+    if (v <= 32) return {32, 1};
+    for (const int tpr : {64, 256, 512, 1024})
+        if (v <= 4 * tpr && !(tpr == 1024 && v > most * 1024)) return {tpr, (int)((v + tpr - 1) / tpr)};
+    return v <= 8 * 1024 && most >= 8 ? RowShape{1024, 8} : RowShape{0, 0};
 }
 // workgroups of the forward: what the CUs hold at once
 static inline int64_t norm_blocks_fwd(int64_t M, int rows, int threads) {
@@ -354,7 +361,7 @@ static inline int64_t norm_blocks_fwd(int64_t M, int rows, int threads) {
     return want < most ? want : most;
 }
 // workgroups of the backward: two on every CU, each with as many rows as it takes
-static inline int64_t norm_blocks(int64_t M) { return M < 512 ? M : 512; }
+static inline int64_t norm_blocks(int64_t M, int rows) { return M < 512 * rows ? (M + rows - 1) / rows : 512; }
 
 template <class Fn> static inline int with_weight_dtype(int dtype, int weight_dtype, Fn&& fn) {
     return with_dtype(dtype, [&](auto t) -> int {
@@ -381,7 +388,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
     const Weights w{gamma, beta, weight_dtype == GM_DTYPE_F32};
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const RowShape r = row_shape(N, VEC<T>, 4, 8);
+        const RowShape r = row_shape(N, VEC<T>, 8);
 #define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)norm_blocks_fwd(M, ROWS, THREADS)), dim3(THREADS), 0, as_stream(stream), M, N, \
                        static_cast<const T*>(X), ldx, w, eps, static_cast<T*>(Y), ldy, mean, rstd)
@@ -389,18 +396,24 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
             constexpr int V = decltype(v)::value;
             constexpr bool TAIL = decltype(tail)::value;
             if constexpr (V == 1) {
-                GM_LAUNCH_NORM((k_layer_norm_fwd<T, 1, false, 1, 64>), 4, 256);
+                GM_LAUNCH_NORM((k_layer_norm_fwd<T, 1, false, 1, 8>), 32, 256);
             } else {
-                switch (r.tpr + r.K) {
-                    case 64 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 64>), 4, 256); break;
-                    case 64 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 64>), 4, 256); break;
-                    case 64 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 64>), 4, 256); break;
-                    case 256 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 256>), 1, 256); break;
-                    case 256 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 256>), 1, 256); break;
-                    case 256 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 256>), 1, 256); break;
-                    case 1024 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 1024>), 1, 1024); break;
-                    case 1024 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 1024>), 1, 1024); break;
-                    case 1024 + 8: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 8, 1024>), 1, 1024); break;
+                switch (r.tpr * 16 + r.K) {
+                    case 8 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 8>), 32, 256); break;
+                    case 16 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 16>), 16, 256); break;
+                    case 32 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 32>), 8, 256); break;
+                    case 64 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 1, 64>), 4, 256); break;
+                    case 64 * 16 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 64>), 4, 256); break;
+                    case 64 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 3, 64>), 4, 256); break;
+                    case 64 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 64>), 4, 256); break;
+                    case 256 * 16 + 2: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 2, 256>), 1, 256); break;
+                    case 256 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 3, 256>), 1, 256); break;
+                    case 256 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 256>), 1, 256); break;
+                    case 512 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 3, 512>), 1, 512); break;
+                    case 512 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 512>), 1, 512); break;
+                    case 1024 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 3, 1024>), 1, 1024); break;
+                    case 1024 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 4, 1024>), 1, 1024); break;
+                    case 1024 * 16 + 8: GM_LAUNCH_NORM((k_layer_norm_fwd<T, V, TAIL, 8, 1024>), 1, 1024); break;
                     default: GM_LAUNCH_NORM((k_layer_norm_fwd_long<T>), 1, 1024); break;
                 }
             }
@@ -413,7 +426,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
 
 extern "C" int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
     if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 26)) return -1;
-    return norm_blocks(M) * 2 * N * 4;
+    return norm_blocks(M, 1) * 2 * N * 4;               // whatever the row type
 }
 
 extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ldg, const void* X, int64_t ldx, int dtype,
@@ -422,7 +435,8 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
     GM_NORM_CHECK();
     GM_REQUIRE(M == 0 || (G && X && mean && rstd && ldg >= N && ldx >= N && (!dX || lddx >= N)), "bad arguments");
     const bool cols = dgamma || dbeta;
-    const int64_t nblk = norm_blocks(M), need = nblk * 2 * N * 4;
+    int64_t nblk = norm_blocks(M, 1);
+    const int64_t need = nblk * 2 * N * 4;
     GM_REQUIRE(!cols || M == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
                "gm_layer_norm_bwd needs %lld workspace bytes (gm_layer_norm_bwd_workspace_bytes)", (long long)need);
     hipStream_t s = as_stream(stream);
@@ -432,28 +446,35 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
         using W = decltype(u);
         if (M > 0) {
             const Weights w{gamma, nullptr, weight_dtype == GM_DTYPE_F32};
-            const RowShape r = row_shape(N, VEC<T>, 4, 16 / VEC<T>);      // the sums of 16 columns a thread at 1024 threads
-#define GM_LAUNCH_NORM(KERNEL, THREADS)                                                                                   \
-    hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,            \
-                       static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part)
+            const RowShape r = row_shape(N, VEC<T>, 4);
+#define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
+    do {                                                                                                                  \
+        nblk = norm_blocks(M, ROWS);                                                                                      \
+        hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,        \
+                           static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part);                \
+    } while (0)
             with_row_form<T>(N, [&](auto v, auto tail) {
                 constexpr int V = decltype(v)::value;
                 constexpr bool TAIL = decltype(tail)::value;
                 if constexpr (V == 1) {
-                    GM_LAUNCH_NORM((k_layer_norm_bwd<T, 1, false, 1, 64>), 256);
+                    GM_LAUNCH_NORM((k_layer_norm_bwd<T, 1, false, 1, 8>), 32, 256);
                 } else {
-                    switch (r.tpr + r.K) {
-                        case 64 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 64>), 256); break;
-                        case 64 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 64>), 256); break;
-                        case 64 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 64>), 256); break;
-                        case 256 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 256>), 256); break;
-                        case 256 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 256>), 256); break;
-                        case 256 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 256>), 256); break;
-                        case 1024 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 1024>), 1024); break;
-                        case 1024 + 4:
-                            if constexpr (V == 4) GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 1024>), 1024);
-                            break;
-                        default: GM_LAUNCH_NORM((k_layer_norm_bwd_long<T>), 1024); break;
+                    switch (r.tpr * 16 + r.K) {
+                        case 8 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 8>), 32, 256); break;
+                        case 16 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 16>), 16, 256); break;
+                        case 32 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 32>), 8, 256); break;
+                        case 64 * 16 + 1: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 1, 64>), 4, 256); break;
+                        case 64 * 16 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 64>), 4, 256); break;
+                        case 64 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 3, 64>), 4, 256); break;
+                        case 64 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 64>), 4, 256); break;
+                        case 256 * 16 + 2: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 2, 256>), 1, 256); break;
+                        case 256 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 3, 256>), 1, 256); break;
+                        case 256 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 256>), 1, 256); break;
+                        case 512 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 3, 512>), 1, 512); break;
+                        case 512 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 512>), 1, 512); break;
+                        case 1024 * 16 + 3: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 3, 1024>), 1, 1024); break;
+                        case 1024 * 16 + 4: GM_LAUNCH_NORM((k_layer_norm_bwd<T, V, TAIL, 4, 1024>), 1, 1024); break;
+                        default: GM_LAUNCH_NORM((k_layer_norm_bwd_long<T>), 1, 1024); break;
                     }
                 }
             });

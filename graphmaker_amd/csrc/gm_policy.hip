@@ -152,6 +152,32 @@ k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whol
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int64_t a = (int64_t)blockIdx.x * chunk, b = a + chunk < q.M ? a + chunk : q.M;
     const int64_t s0 = q.of_wave(a, 0, q.S - 1), s1 = q.of_wave(b - 1, s0, q.S - 1);
+    if (s1 - s0 >= 64) {                                 // many: a lane each, and a wave together for those of over 32 items
+        for (int64_t base = s0 + wv * 64; base <= s1; base += 256) {
+            const int64_t s = base + lane;
+            const int64_t lo = s <= s1 ? q.lo(s) : 0, hi = s <= s1 ? q.hi(s) : 0;
+            const int64_t i0 = lo > a ? lo : a, i1 = hi < b ? hi : b;
+            Sums<Q>* to = lo >= a && hi <= b ? whole + s : piece + 2 * (int64_t)blockIdx.x + (lo < a ? 0 : 1);
+            if (i0 < i1 && i1 - i0 <= 32) {
+                const float of_seq = f.of_sequence(s);
+                typename F::Acc acc;
+                for (int64_t i = i0; i < i1; ++i) f.template add<1>(i, of_seq, acc);
+                *to = F::sums(acc);
+            }
+            for (uint64_t left = __ballot(i1 - i0 > 32); left; left &= left - 1) {
+                const int from = __ffsll((unsigned long long)left) - 1;
+                const int64_t j0 = __shfl(i0, from), j1 = __shfl(i1, from);
+                const float of_seq = f.of_sequence(base + from);
+                typename F::Acc acc;
+                for (int64_t i = j0 + lane; i < j1; i += 64) f.template add<1>(i, of_seq, acc);
+                Sums<Q> sum = F::sums(acc);
+#pragma unroll
+                for (int c = 0; c < Q; ++c) sum.v[c] = wave_add(sum.v[c]);
+                if (lane == from) *to = sum;
+            }
+        }
+        return;
+    }
     const bool alone = s0 == s1;                         // one sequence: all four waves sum it together, else one wave each
     const int t = alone ? (int)threadIdx.x : lane, threads = alone ? 256 : 64;
     for (int64_t s = s0 + (alone ? 0 : wv); s <= s1; s += 4) {
@@ -201,11 +227,22 @@ __device__ __forceinline__ Sums<Q> gather_sequence(const Sequences& q, int64_t c
 }
 template <int Q>
 __global__ void __launch_bounds__(256)
-k_sequence_gather(Sequences q, int64_t chunk, Sums<Q>* __restrict__ whole, const Sums<Q>* __restrict__ piece) {
-    const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (s >= q.S) return;
-    const Sums<Q> sum = gather_sequence<Q, 64>(q, chunk, s, threadIdx.x & 63, whole, piece);
-    if ((threadIdx.x & 63) == 0) whole[s] = sum;
+k_sequence_gather(Sequences q, int64_t chunk, int per, Sums<Q>* __restrict__ whole, const Sums<Q>* __restrict__ piece) {
+    // a lane looks at each of a wave's `per` sequences, the wave sums those that cross chunks: all of a few thousand may, of
+    // more only as many as there are chunks
+    const int lane = threadIdx.x & 63;
+    const int64_t step = (int64_t)gridDim.x * 4 * per;
+    for (int64_t base = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per; base < q.S; base += step) {
+        const int64_t s = base + lane;
+        const bool mine = lane < per && s < q.S;
+        const int64_t lo = mine ? q.lo(s) : 0, hi = mine ? q.hi(s) : 0;
+        if (mine && lo >= hi) whole[s] = Sums<Q>{};
+        for (uint64_t left = __ballot(lo < hi && lo / chunk != (hi - 1) / chunk); left; left &= left - 1) {
+            const int64_t t = base + __ffsll((unsigned long long)left) - 1;
+            const Sums<Q> sum = gather_sequence<Q, 64>(q, chunk, t, lane, whole, piece);
+            if (lane == 0) whole[t] = sum;
+        }
+    }
 }
 // the same into LDS by a workgroup of 1024 threads, for up to SEQ_FUSED sequences: all of them at once
 template <int Q, int LANES>
@@ -249,11 +286,11 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
     __shared__ Sums<4> held[SEQ_FUSED];
     if (gather) gather_all<4>(q, chunk, whole, piece, held);
     double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};           // the sums, live items, sequences that have one
+#pragma unroll 4
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
         const Sums<4> w = gather ? held[s] : whole[s];
-        if (w.v[3] <= 0.0) continue;
-        const double unit = by_sequence ? 1.0 / w.v[3] : 1.0;
-        tot[4] += 1.0;
+        const double unit = w.v[3] > 0.0 && by_sequence ? 1.0 / w.v[3] : 1.0;
+        tot[4] += w.v[3] > 0.0 ? 1.0 : 0.0;
 #pragma unroll
         for (int c = 0; c < 3; ++c) tot[c] += w.v[c] * unit;
         tot[3] += w.v[3];
@@ -261,6 +298,7 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
     block_add(tot, red);
     const double over = by_sequence ? tot[4] : tot[3];
     const double norm = over > 0.0 ? 1.0 / over : 0.0;    // no live item: the loss and every gradient are 0
+#pragma unroll 4
     for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
         const double n = gather ? held[s].v[3] : whole[s].v[3];
         if (weight) weight[s] = n > 0.0 ? (float)(by_sequence ? norm / n : norm) : 0.0f;
@@ -283,6 +321,7 @@ k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double 
     if (gather) gather_all<2>(q, chunk, whole, piece, held);
     const int64_t P = q.S / 2;
     double tot[1] = {0.0};
+#pragma unroll 2
     for (int64_t p = threadIdx.x; p < P; p += 1024) {
         double h[2], unit[2];
 #pragma unroll
@@ -352,6 +391,11 @@ k_sequence_spread(Sequences q, int64_t chunk, const float* __restrict__ slope, c
     }
 }
 
+static inline unsigned gather_blocks(int64_t S, int per) {
+    const int64_t want = (S + 4 * per - 1) / (4 * per);
+    return (unsigned)(want < 4096 ? want : 4096);
+}
+
 struct SequenceLayout { int64_t nchunk, whole, piece, bytes; };
 static inline SequenceLayout sequence_layout(int64_t M, int64_t S) {
     SequenceLayout l;
@@ -379,7 +423,8 @@ static int launch_sequence_loss(const Sequences& q, const F& f, void* workspace,
     }
     const int fused = q.S <= SEQ_FUSED;
     if (!fused) {
-        hipLaunchKernelGGL((k_sequence_gather<Q>), dim3((unsigned)((q.S + 3) / 4)), dim3(256), 0, s, q, chunk, whole, piece);
+        const int per = q.S <= 16384 ? 1 : 64;
+        hipLaunchKernelGGL((k_sequence_gather<Q>), dim3(gather_blocks(q.S, per)), dim3(256), 0, s, q, chunk, per, whole, piece);
         GM_LAUNCH_CHECK();
     }
     finish(chunk, fused, whole, piece);

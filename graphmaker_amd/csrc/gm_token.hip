@@ -47,7 +47,13 @@ k_token_embedding_fwd(int64_t n, int64_t C, int w, int shift, IndexArray tok, co
 
 // ---- stable radix sort of n keys in [0, C] (C: tokens that add to no row, sorted behind the others), RADIX_BITS at a time
 constexpr int RADIX_BITS = 9, RADIX_BINS = 1 << RADIX_BITS;         // at most; the digits of a sort are as even as can be
-constexpr int SORT_KEYS = 2048;                       // keys per workgroup: 4 waves x 8 rounds x 64 lanes
+constexpr int SORT_STEP = 2048;                       // a workgroup's keys in steps of 4 waves x 8 rounds x 64 lanes
+// keys of a workgroup: enough that the counts of all workgroups stay a few steps of the scan, with two to four workgroups a CU
+static inline int64_t sort_keys(int64_t n) {
+    int64_t keys = SORT_STEP;
+    while (keys * 512 < n) keys *= 2;
+    return keys;
+}
 __device__ __forceinline__ uint32_t token_key(const IndexArray& tok, int64_t i, int64_t C, int64_t padding) {
     const int64_t c = tok.at(i);
     return c >= 0 && c < C && c != padding ? (uint32_t)c : (uint32_t)C;
@@ -74,15 +80,16 @@ __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, bool 
 
 // counts[digit][workgroup]
 __global__ void __launch_bounds__(256)
-k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys, int shift, int bits,
+k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys, int64_t each, int shift, int bits,
               uint32_t* __restrict__ counts) {
     __shared__ uint32_t hist[RADIX_BINS];
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += 256) hist[b] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_KEYS;
-    for (int r = 0; r < SORT_KEYS / 256; ++r) {
-        const int64_t i = base + r * 256 + threadIdx.x;
+    const int64_t base = (int64_t)blockIdx.x * each;
+#pragma unroll 8
+    for (int64_t r = 0; r < each; r += 256) {
+        const int64_t i = base + r + threadIdx.x;
         if (i < n) {
             const uint32_t key = keys ? keys[i] : token_key(tok, i, C, padding);
             atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
@@ -135,27 +142,32 @@ __global__ void __launch_bounds__(1024) k_radix_scan(int64_t m, uint32_t* __rest
     }
 }
 
-// Each wave owns SORT_KEYS/4 consecutive keys and keeps the next free place of every digit.
+// Each wave owns a quarter of the workgroup's `each` keys, consecutive ones, and keeps the next free place of every digit.
 template <int BITS>
 __global__ void __launch_bounds__(256)
 k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys,
-                const uint32_t* __restrict__ pos, int shift, const uint32_t* __restrict__ starts, uint32_t* __restrict__ keys_out,
+                const uint32_t* __restrict__ pos, int64_t each, int shift, const uint32_t* __restrict__ starts, uint32_t* __restrict__ keys_out,
                 uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t next[4][RADIX_BINS];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     constexpr int bins = 1 << BITS;
     for (int b = threadIdx.x; b < 4 * RADIX_BINS; b += 256) (&next[0][0])[b] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_KEYS + wv * (SORT_KEYS / 4);
-    uint32_t key[SORT_KEYS / 256];
+    constexpr int ROUNDS = SORT_STEP / 256;
+    const int64_t base = (int64_t)blockIdx.x * each + wv * (each / 4);
+    uint32_t key[ROUNDS];
+    auto fetch = [&](int64_t from) {
 #pragma unroll
-    for (int r = 0; r < SORT_KEYS / 256; ++r) {
-        const int64_t i = base + r * 64 + lane;
-        key[r] = 0;
-        if (i < n) {
-            key[r] = keys ? keys[i] : token_key(tok, i, C, padding);
-            atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int64_t i = from + r * 64 + lane;
+            key[r] = i >= n ? 0 : keys ? keys[i] : token_key(tok, i, C, padding);
         }
+    };
+    for (int64_t off = 0; off < each / 4; off += ROUNDS * 64) {
+        fetch(base + off);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (base + off + r * 64 + lane < n) atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += 256) {
@@ -168,15 +180,17 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
         }
     }
     __syncthreads();
+    for (int64_t off = 0; off < each / 4; off += ROUNDS * 64) {
+        if (each > SORT_STEP) fetch(base + off);         // a single step still has its keys
 #pragma unroll
-    for (int r = 0; r < SORT_KEYS / 256; ++r) {
-        const int64_t i = base + r * 64 + lane;
-        const bool in = i < n;
-        const uint32_t d = (key[r] >> shift) & (bins - 1);
-        const uint32_t at = take_place<BITS>(next[wv], d, in, lane);
-        if (in) {
-            keys_out[at] = key[r];
-            pos_out[at] = pos ? pos[i] : (uint32_t)i;
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int64_t i = base + off + r * 64 + lane;
+            const bool in = i < n;
+            const uint32_t at = take_place<BITS>(next[wv], (key[r] >> shift) & (bins - 1), in, lane);
+            if (in) {
+                keys_out[at] = key[r];
+                pos_out[at] = pos ? pos[i] : (uint32_t)i;
+            }
         }
     }
 }
@@ -329,10 +343,10 @@ struct RowSum {
 // part[2k] of the row that chunk k begins with, part[2k+1] of the row that it ends with and did not begin with.  Such a row
 // meets at least two chunks, so a chunk holds pieces of at most two of them.
 template <class T, int V, bool TAIL>
-__device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lanes, uint32_t cut, uint32_t chunk, const uint32_t* __restrict__ keys,
+__device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lanes, uint32_t cut, uint32_t chunk, int col0, const uint32_t* __restrict__ keys,
                                             const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G,
                                             int64_t ldg, float* __restrict__ part, int64_t ldp) {
-    const int lane = threadIdx.x & 63, col0 = blockIdx.y * 64 * V;
+    const int lane = threadIdx.x & 63;
     const uint32_t a = chunk * cut, b = (int64_t)a + cut < n ? a + cut : (uint32_t)n;
     const uint32_t first = keys[a], last = keys[b - 1];
 #pragma unroll 1
@@ -404,26 +418,30 @@ __global__ void __launch_bounds__(256)
 k_token_grad(int64_t n, int64_t C, int w, int lanes, uint32_t cut, unsigned pieces, const uint32_t* __restrict__ keys,
              const uint32_t* __restrict__ rowptr, const uint32_t* __restrict__ pos, const T* __restrict__ G, int64_t ldg,
              float* __restrict__ part, int64_t ldp, float scale, T* __restrict__ dW, int64_t ldw) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col0 = blockIdx.y * 64 * V;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     if (blockIdx.x < pieces) {
         const uint32_t chunk = blockIdx.x * 4 + wv;
-        if ((int64_t)chunk * cut < n) token_piece<T, V, TAIL>(n, C, w, lanes, cut, chunk, keys, rowptr, pos, G, ldg, part, ldp);
+        if ((int64_t)chunk * cut < n)
+            for (int col0 = blockIdx.y * 64 * V; col0 < w; col0 += gridDim.y * 64 * V)
+                token_piece<T, V, TAIL>(n, C, w, lanes, cut, chunk, col0, keys, rowptr, pos, G, ldg, part, ldp);
         return;
     }
     for (int64_t c = (int64_t)(blockIdx.x - pieces) * 4 + wv; c < C; c += (int64_t)(gridDim.x - pieces) * 4) {
         const uint32_t a = rowptr[c], b = rowptr[c + 1];
         if (b - a > cut) continue;
-        RowSum<T, V, TAIL> sum;
-        sum.clear();
-        if (a < b) {
-            sum.add(pos, a, b, G, ldg, w, col0, lanes);
-            sum.join(lanes);
-        }
-        if (lane < lanes) {
-            float y[V];
+        for (int col0 = blockIdx.y * 64 * V; col0 < w; col0 += gridDim.y * 64 * V) {
+            RowSum<T, V, TAIL> sum;
+            sum.clear();
+            if (a < b) {
+                sum.add(pos, a, b, G, ldg, w, col0, lanes);
+                sum.join(lanes);
+            }
+            if (lane < lanes) {
+                float y[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) y[v] = sum.acc[v] * scale;
-            store_vec<T, V, TAIL>(dW + c * ldw, col0 + lane * V, w, y);
+                for (int v = 0; v < V; ++v) y[v] = sum.acc[v] * scale;
+                store_vec<T, V, TAIL>(dW + c * ldw, col0 + lane * V, w, y);
+            }
         }
     }
 }
@@ -521,7 +539,7 @@ static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
     l.passes = (bits + most - 1) / most;
     l.digit = (bits + l.passes - 1) / l.passes;
     if (l.digit < 5) l.digit = 5;                      // with_digit
-    l.nblk = (n + SORT_KEYS - 1) / SORT_KEYS;
+    l.nblk = (n + sort_keys(n) - 1) / sort_keys(n);
     l.cut = 64;
     while ((int64_t)l.cut * 4096 < n) l.cut *= 2;      // at most 4096 pieces of one row
     int64_t at = 0;
@@ -611,13 +629,13 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
         }
         for (int p = 0; p < l.passes && n > SMALL_KEYS; ++p) {
             uint32_t *ko = u32(l.keys[p & 1]), *po = u32(l.pos[p & 1]);
-            hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr, p * BITS, BITS,
-                               counts);
+            hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr, sort_keys(n),
+                               p * BITS, BITS, counts);
             GM_LAUNCH_CHECK();
             hipLaunchKernelGGL(k_radix_scan, dim3(1), dim3(1024), 0, s, l.nblk << BITS, counts);
             GM_LAUNCH_CHECK();
             hipLaunchKernelGGL((k_radix_scatter<BITS>), dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
-                               p ? pos : nullptr, p * BITS, counts, ko, po);
+                               p ? pos : nullptr, sort_keys(n), p * BITS, counts, ko, po);
             GM_LAUNCH_CHECK();
             keys = ko;
             pos = po;
@@ -631,9 +649,11 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     const int64_t vecs = (w + vec - 1) / vec;
     int lanes = 64;
     while (lanes > 1 && lanes / 2 >= vecs) lanes /= 2;
-    const unsigned tiles = (unsigned)((vecs + 63) / 64);
+    // a wave walks the tiles of its row where the rows alone fill the chip eight times over
+    int64_t tiles = (vecs + 63) / 64;
+    if (tiles > 1 && C >= 65536 / tiles) tiles = C >= 65536 ? 1 : (65536 + C - 1) / C;
     const unsigned chunks = (unsigned)((n + l.cut - 1) / l.cut);
-    GM_REQUIRE(tiles < 65536u, "w too large");
+    GM_REQUIRE(tiles < 65536, "w too large");
     const int64_t ldp = (w + 3) / 4 * 4;
     int wide = 1;
     while (wide < 256 && wide * 4 < w) wide *= 2;
@@ -645,7 +665,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
             constexpr bool TAIL = decltype(tail)::value;
             status = [&]() -> int {
                 const unsigned pieces = n > l.cut ? (chunks + 3) / 4 : 0;
-                hipLaunchKernelGGL((k_token_grad<T, V, TAIL>), dim3(pieces + grid_for((C + 3) / 4, 512), tiles), dim3(256), 0, s, n, C, (int)w,
+                hipLaunchKernelGGL((k_token_grad<T, V, TAIL>), dim3(pieces + grid_for((C + 3) / 4, 512), (unsigned)tiles), dim3(256), 0, s, n, C, (int)w,
                                    lanes, l.cut, pieces, keys, rowptr, pos, static_cast<const T*>(G), ldg, part, ldp, scale,
                                    static_cast<T*>(dW), ldw);
                 GM_LAUNCH_CHECK();

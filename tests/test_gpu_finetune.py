@@ -192,7 +192,7 @@ def check_norm(x, gamma, beta, g, dev, eps=1e-5):
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("M, N", [(1, 1), (1, 2), (3, 7), (5, 64), (4, 65), (130, 96), (67, 512), (1, 1000), (9, 1023), (64, 1024),
                                   (3, 2049), (2, 4096), (33, 5000), (7, 8192), (5, 16384), (2, 20001), (1, 70000), (700, 24),
-                                  (5000, 96), (1300, 2056), (300, 16400)])
+                                  (5000, 96), (1300, 2056), (300, 16400), (20, 700), (20, 1500), (2, 40000), (9000, 40)])
 def test_layer_norm(dev, dt, M, N):
     t = DT[dt]
     x = (rnd(N, M, N) * (1 + torch.arange(M)[:, None] % 3) + 0.7).to(t)
@@ -309,7 +309,7 @@ def check_log_prob(x, c, g, dev, ignore=-100, index=torch.int64):
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("M, V", [(1, 1), (1, 2), (257, 2), (300, 3), (65, 5), (64, 10), (33, 16), (31, 17), (9, 33), (70, 64), (5, 65),
                                   (17, 100), (6, 257), (4, 512), (3, 1000), (9, 1025), (2, 4096), (5, 5003), (1, 9001), (3, 33001),
-                                  (1, 131075), (40, 8192)])
+                                  (1, 131075), (40, 8192), (7, 1600), (5, 2400)])
 def test_class_log_prob(dev, dt, M, V):
     g = torch.Generator().manual_seed(M * 7 + V)
     x = (2.0 * torch.randn(M, V, generator=g)).to(DT[dt])
@@ -524,7 +524,8 @@ def ragged(seed, S, M):
 
 
 @pytest.mark.parametrize("reduction", ["token", "sequence"])
-@pytest.mark.parametrize("S, M", [(1, 1), (1, 5000), (2, 3), (5, 1024), (7, 9000), (64, 3001), (65, 3001), (300, 20000), (500, 400), (3000, 6000)])
+@pytest.mark.parametrize("S, M", [(1, 1), (1, 5000), (2, 3), (5, 1024), (7, 9000), (64, 3001), (65, 3001), (300, 20000), (500, 400), (3000, 6000),
+                                  (20000, 60000), (17000, 900)])
 def test_policy_loss_of_sequences(dev, reduction, S, M):
     lp, old, ref = ratios(S + M, M)
     mask = torch.rand(M, generator=torch.Generator().manual_seed(M)) < 0.6
@@ -608,7 +609,7 @@ def check_preference(lp, ref, offsets, dev, mask=None, beta=0.1, smoothing=0.0, 
 
 
 @pytest.mark.parametrize("average", [False, True])
-@pytest.mark.parametrize("P, M", [(1, 2), (1, 5000), (3, 40), (16, 1024), (32, 9000), (33, 9001), (200, 30000), (1500, 2000)])
+@pytest.mark.parametrize("P, M", [(1, 2), (1, 5000), (3, 40), (16, 1024), (32, 9000), (33, 9001), (200, 30000), (1500, 2000), (10000, 70000)])
 def test_preference_loss(dev, average, P, M):
     lp = -rnd(P, M).abs()
     ref = lp + 0.2 * rnd(P + 1, M)
