@@ -413,15 +413,15 @@ using namespace gm;
 #define GM_LOGPROB_CHECK()                                                                                                \
     GM_REQUIRE(M >= 0 && V > 0, "bad arguments");                                                                         \
     GM_REQUIRE(dtype_ok(dtype), "dtype %d is none of GM_DTYPE_*", dtype);                                                 \
-    GM_REQUIRE(M < (1ll << 31) && V < (1ll << 28), "M of 2^31 or more, or V of 2^28 or more")
+    GM_REQUIRE(M < (1ll << 31) && V < (1ll << 27), "M of 2^31 or more, or V of 2^27 or more")
 
 extern "C" int64_t gm_class_log_prob_stats_floats(int64_t M, int64_t V, int dtype) {
-    if (M < 0 || V <= 0 || M >= (1ll << 31) || V >= (1ll << 28) || !dtype_ok(dtype)) return -1;
+    if (M < 0 || V <= 0 || M >= (1ll << 31) || V >= (1ll << 27) || !dtype_ok(dtype)) return -1;
     return V < 16 / dtype_size(dtype) ? 0 : 2 * M;
 }
 
 extern "C" int64_t gm_class_log_prob_workspace_bytes(int64_t M, int64_t V, int dtype) {
-    if (M < 0 || V <= 0 || M >= (1ll << 31) || V >= (1ll << 28) || !dtype_ok(dtype)) return -1;
+    if (M < 0 || V <= 0 || M >= (1ll << 31) || V >= (1ll << 27) || !dtype_ok(dtype)) return -1;
     const int vec = 16 / dtype_size(dtype);
     if (V < vec || log_prob_shape(V, vec).lanes) return 0;
     const int64_t parts = long_parts(M, V, vec);

@@ -332,8 +332,8 @@ k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double 
             rewards[2 * p + k] = (float)(beta * h[k]);
         }
         const double z = beta * (h[0] - h[1]), e = exp(-fabs(z));
-        const double up = (z < 0.0 ? -z : 0.0) + log1p(e);              // -log sig(z); z NaN: e is
-        tot[0] += smoothing != 0.0 ? (1.0 - smoothing) * up + smoothing * (up + z) : up;
+        const double up = (z < 0.0 ? -z : 0.0) + log1p(e), down = (z > 0.0 ? z : 0.0) + log1p(e);    // -log sig(z), -log sig(-z); z NaN: e is
+        tot[0] += smoothing != 0.0 ? (1.0 - smoothing) * up + smoothing * down : up;
         const double dz = (smoothing - (z >= 0.0 ? e : 1.0) / (1.0 + e)) / (double)P;    // sig(z) - 1 = -sig(-z)
         if (weight) {
             weight[2 * p] = (float)(beta * dz * unit[0]);

@@ -102,7 +102,9 @@ bool records(const Tensor& t) {
     if (t.is_leaf() && t.is_cuda()) {
         const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t.device().index());
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(now.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone) {
+        if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess) {
+            (void)hipGetLastError();                     // or the next launch would report it as its own
+        } else if (status != hipStreamCaptureStatusNone) {
             const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
             if (node && node->stream() && node->stream()->id() != now.id())
                 throw HipError("captured while a graph recorded on another stream over the same leaf tensor is alive: drop that graph first");
@@ -170,6 +172,7 @@ Tensor token_embedding(const Tensor& weight, const Tensor& tokens, double scale,
     row_dtype(weight, "weight");
     const Tensor tok = index_of(tokens, "tokens", weight);
     const int64_t C = weight.size(0);
+    if (!std::isfinite((float)scale)) throw py::value_error(say("token_embedding: scale must be finite in float32, got ", scale));
     EmbeddingArgs a{scale, -1};
     if (padding_idx) {
         if (*padding_idx < -C || *padding_idx >= C)
@@ -252,7 +255,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& gamma_, const st
     on_gpu(x, "x");
     for (Tensor& t : weights)
         if (t.defined()) t = t.contiguous();
-    if (records(x) || records(weights[0]) || records(weights[1])) {
+    if (records(x) | records(weights[0]) | records(weights[1])) {        // each of them is looked at
         auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
         return LayerNorm::apply(x, given(weights[0]), given(weights[1]), eps);
     }

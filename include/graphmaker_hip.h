@@ -364,8 +364,8 @@ int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N);
 int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ldg, const void* X, int64_t ldx, int dtype, const float* mean,
                       const float* rstd, const void* gamma, int weight_dtype, void* dX, int64_t lddx, void* dgamma, void* dbeta,
                       void* workspace, int64_t workspace_bytes, gm_stream_t stream);
-/* log_prob[i] = logits[i][classes[i]] - logsumexp(logits[i]); 0 where classes[i] == ignore_index (such a row is not read), NaN
- * for another class outside [0, V).  stats (gm_class_log_prob_stats_floats, 8-byte aligned, may be NULL): what the backward
+/* log_prob[i] = logits[i][classes[i]] - logsumexp(logits[i]); 0 where classes[i] == ignore_index, whatever the row holds, NaN
+ * for another class outside [0, V); V < 2^27.  stats (gm_class_log_prob_stats_floats, 8-byte aligned, may be NULL): what the backward
  * needs; rows of less than 16 bytes need none. */
 int64_t gm_class_log_prob_stats_floats(int64_t M, int64_t V, int dtype);
 int64_t gm_class_log_prob_workspace_bytes(int64_t M, int64_t V, int dtype);

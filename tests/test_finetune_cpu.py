@@ -30,6 +30,8 @@ def i(*shape, dtype=torch.int64):
     (lambda: ag.token_embedding(f(4, 8), f(3)), TypeError),
     (lambda: ag.token_embedding(f(4, 8), i(3), padding_idx=4), ValueError),
     (lambda: ag.token_embedding(f(4, 8), i(3), padding_idx=-5), ValueError),
+    (lambda: ag.token_embedding(f(4, 8), i(3), scale=float("inf")), ValueError),
+    (lambda: ag.token_embedding(f(4, 8), i(3), scale=1e39), ValueError),
     (lambda: ag.token_embedding(f(4, 8), i(3)), L.GraphMakerHipError),
     (lambda: ag.layer_norm(f(())), ValueError),
     (lambda: ag.layer_norm(f(3, 0)), ValueError),
@@ -171,6 +173,7 @@ def test_workspace_sizes():
     assert lib.gm_layer_norm_bwd_workspace_bytes(0, 8) >= 0
     assert lib.gm_layer_norm_bwd_workspace_bytes(8, 0) == -1 == lib.gm_layer_norm_bwd_workspace_bytes(8, 1 << 26)
     assert lib.gm_class_log_prob_stats_floats(8, 1 << 28, 1) == -1 == lib.gm_sequence_loss_workspace_bytes(1 << 34, 1)
+    assert lib.gm_class_log_prob_stats_floats(1, 1 << 27, 0) == -1 == lib.gm_class_log_prob_workspace_bytes(1, 1 << 27, 0)
     assert lib.gm_class_log_prob_workspace_bytes(8, 0, 0) == -1 == lib.gm_class_log_prob_workspace_bytes(8, 8, 3)
     assert lib.gm_class_log_prob_stats_floats(8, 3, 0) == 0 and lib.gm_class_log_prob_stats_floats(8, 4, 0) == 16
     assert lib.gm_class_log_prob_stats_floats(8, 7, 1) == 0 and lib.gm_class_log_prob_stats_floats(8, 8, 1) == 16

@@ -636,6 +636,18 @@ def test_preference_loss_extremes(dev):
     check_preference(big, ref, [0, 30, 64], dev, smoothing=0.2)                  # saturated, right and wrong way round
     check_preference(big, ref, [0, 0, 64], dev, smoothing=0.5)
     check_preference(-big, ref, [0, 30, 64], dev)
+    for at in (5, 40):                                                           # an impossible draw, preferred or rejected: z = -inf or inf
+        for smoothing in (0.0, 0.2):
+            off = torch.tensor([0, 30, 64], device=dev)
+            a = lp.clone()
+            a[at] = -math.inf
+            a = a.to(dev).requires_grad_(True)
+            loss, _ = ag.preference_loss(a, ref.to(dev), off, beta=0.5, label_smoothing=smoothing)
+            (dl,) = torch.autograd.grad(loss, [a])
+            z = -math.inf if at == 5 else math.inf
+            assert float(loss) == (math.inf if at == 5 or smoothing else 0.0)
+            dz = 0.5 * (1 / (1 + math.exp(-max(z, -700.0))) - (1 - smoothing))      # exp(700) is finite, its sigmoid below 1e-300
+            close(dl, torch.where(torch.arange(M) < 30, dz, -dz), 2 * U * abs(dz) + 1e-44, "gradient of an impossible draw")
     e = torch.empty(0, device=dev, requires_grad=True)
     loss, rewards = ag.preference_loss(e, e.detach(), torch.zeros(5, dtype=torch.int64, device=dev))
     assert abs(float(loss) - math.log(2)) <= 2 * U and torch.equal(rewards, torch.zeros(4, device=dev))
@@ -790,7 +802,9 @@ def test_capture_beside_a_living_eager_graph_is_refused(dev):
     alive = ag.layer_norm(x, w)                          # recorded eagerly on the default stream
     held = ag.token_embedding(emb, tok)
     torch.cuda.synchronize()
-    for call in (lambda: ag.layer_norm(x, w), lambda: ag.token_embedding(emb, tok)):
+    fresh = rnd(4, 30, 64).to(dev).requires_grad_(True)
+    for call in (lambda: ag.layer_norm(x, w), lambda: ag.token_embedding(emb, tok),
+                 lambda: ag.layer_norm(fresh * 2, w), lambda: ag.layer_norm(fresh, None, w)):
         with pytest.raises(RuntimeError, match="same leaf tensor is alive"):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 call()
