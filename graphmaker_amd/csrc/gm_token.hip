@@ -47,11 +47,12 @@ k_token_embedding_fwd(int64_t n, int64_t C, int w, int shift, IndexArray tok, co
 
 // ---- stable radix sort of n keys in [0, C] (C: tokens that add to no row, sorted behind the others), RADIX_BITS at a time
 constexpr int RADIX_BITS = 9, RADIX_BINS = 1 << RADIX_BITS;         // at most; the digits of a sort are as even as can be
-constexpr int SORT_STEP = 2048;                       // a workgroup's keys in steps of 4 waves x 8 rounds x 64 lanes
-// keys of a workgroup: enough that the counts of all workgroups stay a few steps of the scan, with two to four workgroups a CU
+constexpr int SORT_STEP = 1024;                       // a workgroup's keys in steps of 4 waves x 4 rounds x 64 lanes
+// keys of a workgroup: one step where that makes up to 256 workgroups, which all read each other's counts (512 KB at most).  A
+// digit takes 12 to 14 us up to 131,001 keys, 22 us of 524,001 (26 us in 128 workgroups) and 32 us of 1,048,001 (46 us).
 static inline int64_t sort_keys(int64_t n) {
     int64_t keys = SORT_STEP;
-    while (keys * 512 < n) keys *= 2;
+    while (keys * 256 < n) keys *= 2;
     return keys;
 }
 __device__ __forceinline__ uint32_t token_key(const IndexArray& tok, int64_t i, int64_t C, int64_t padding) {
@@ -78,7 +79,7 @@ __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, bool 
     return at;
 }
 
-// counts[digit][workgroup]
+// counts[workgroup][digit]
 __global__ void __launch_bounds__(256)
 k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys, int64_t each, int shift, int bits,
               uint32_t* __restrict__ counts) {
@@ -96,61 +97,21 @@ k_radix_count(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint3
         }
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)b * gridDim.x + blockIdx.x] = hist[b];
-}
-
-// exclusive prefix sum of m counts (a multiple of 4) by one workgroup, SCAN_EACH a thread and step
-constexpr int SCAN_EACH = 16;
-__global__ void __launch_bounds__(1024) k_radix_scan(int64_t m, uint32_t* __restrict__ counts) {
-    __shared__ uint32_t tot[16];
-    uint32_t carry = 0;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    for (int64_t b = 0; b < m; b += 1024 * SCAN_EACH) {
-        const int64_t i = b + threadIdx.x * SCAN_EACH;
-        uint32_t v[SCAN_EACH], sum = 0;
-#pragma unroll
-        for (int k = 0; k < SCAN_EACH; k += 4) {
-            const uint4 x = i + k < m ? *reinterpret_cast<const uint4*>(counts + i + k) : make_uint4(0, 0, 0, 0);
-            v[k] = x.x; v[k + 1] = x.y; v[k + 2] = x.z; v[k + 3] = x.w;
-        }
-#pragma unroll
-        for (int k = 0; k < SCAN_EACH; ++k) sum += v[k];
-        uint32_t s = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t t = __shfl_up(s, off);
-            if (lane >= off) s += t;
-        }
-        if (lane == 63) tot[wv] = s;
-        __syncthreads();
-        uint32_t at = carry + s - sum;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            if (k < wv) at += tot[k];
-            carry += tot[k];
-        }
-#pragma unroll
-        for (int k = 0; k < SCAN_EACH; k += 4) {
-            uint4 x;
-            x.x = at; at += v[k];
-            x.y = at; at += v[k + 1];
-            x.z = at; at += v[k + 2];
-            x.w = at; at += v[k + 3];
-            if (i + k < m) *reinterpret_cast<uint4*>(counts + i + k) = x;
-        }
-        __syncthreads();
-    }
+    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)blockIdx.x * bins + b] = hist[b];
 }
 
 // Each wave owns a quarter of the workgroup's `each` keys, consecutive ones, and keeps the next free place of every digit.
+// Where a digit's keys begin, every workgroup sums from all workgroups' counts; a scan by one workgroup between the two
+// launches took 5 to 30 us of its own and saved 1 to 3.
 template <int BITS>
 __global__ void __launch_bounds__(256)
 k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uint32_t* __restrict__ keys,
-                const uint32_t* __restrict__ pos, int64_t each, int shift, const uint32_t* __restrict__ starts, uint32_t* __restrict__ keys_out,
+                const uint32_t* __restrict__ pos, int64_t each, int shift, const uint32_t* __restrict__ counts, uint32_t* __restrict__ keys_out,
                 uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t next[4][RADIX_BINS];
+    __shared__ uint32_t tot[4];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    constexpr int bins = 1 << BITS;
+    constexpr int bins = 1 << BITS, OWN = bins > 256 ? bins / 256 : 1;       // digits of a thread, consecutive ones
     for (int b = threadIdx.x; b < 4 * RADIX_BINS; b += 256) (&next[0][0])[b] = 0;
     __syncthreads();
     constexpr int ROUNDS = SORT_STEP / 256;
@@ -169,16 +130,43 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
         for (int r = 0; r < ROUNDS; ++r)
             if (base + off + r * 64 + lane < n) atomicAdd(&next[wv][(key[r] >> shift) & (bins - 1)], 1u);
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256) {
-        uint32_t at = starts[(int64_t)b * gridDim.x + blockIdx.x];
+    uint32_t at[OWN] = {}, all[OWN] = {}, sum = 0;       // keys of the digit in the workgroups before this one, and in all
+    const bool owner = (int)threadIdx.x * OWN < bins;
+    if (owner)
+#pragma unroll 16
+        for (unsigned k = 0; k < gridDim.x; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t c = next[k][b];
-            next[k][b] = at;
-            at += c;
-        }
+            for (int j = 0; j < OWN; ++j) {
+                const uint32_t c = counts[k * bins + threadIdx.x * OWN + j];
+                all[j] += c;
+                at[j] += k < blockIdx.x ? c : 0;
+            }
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) sum += all[j];
+    uint32_t s = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t x = __shfl_up(s, off);
+        if (lane >= off) s += x;
     }
+    if (lane == 63) tot[wv] = s;
+    __syncthreads();
+    s -= sum;
+    for (int k = 0; k < wv; ++k) s += tot[k];
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) {
+        at[j] += s;
+        s += all[j];
+    }
+    if (owner)
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t c = next[k][threadIdx.x * OWN + j];
+                next[k][threadIdx.x * OWN + j] = at[j];
+                at[j] += c;
+            }
     __syncthreads();
     for (int64_t off = 0; off < each / 4; off += ROUNDS * 64) {
         if (each > SORT_STEP) fetch(base + off);         // a single step still has its keys
@@ -186,10 +174,10 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
         for (int r = 0; r < ROUNDS; ++r) {
             const int64_t i = base + off + r * 64 + lane;
             const bool in = i < n;
-            const uint32_t at = take_place<BITS>(next[wv], (key[r] >> shift) & (bins - 1), in, lane);
+            const uint32_t place = take_place<BITS>(next[wv], (key[r] >> shift) & (bins - 1), in, lane);
             if (in) {
-                keys_out[at] = key[r];
-                pos_out[at] = pos ? pos[i] : (uint32_t)i;
+                keys_out[place] = key[r];
+                pos_out[place] = pos ? pos[i] : (uint32_t)i;
             }
         }
     }
@@ -446,10 +434,44 @@ k_token_grad(int64_t n, int64_t C, int w, int lanes, uint32_t cut, unsigned piec
     }
 }
 
+// ---- up to DIRECT tokens: no sort.  The wave of a row holds all tokens, one a lane, and lists the positions of its own in
+// ascending order.  One launch where sort, borders and sums take three (82 x 559 bf16, forward and gradient: 44 us of 64 tokens,
+// 54 us of 65).
+constexpr int DIRECT = 64;
+template <class T, int V, bool TAIL>
+__global__ void __launch_bounds__(256)
+k_token_direct(int n, int64_t C, int w, int lanes, int64_t padding, IndexArray tok, const T* __restrict__ G, int64_t ldg, float scale,
+               T* __restrict__ dW, int64_t ldw) {
+    __shared__ uint32_t list[4][DIRECT];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const uint32_t key = token_key(tok, lane < n ? lane : n - 1, C, padding);
+    for (int64_t c = (int64_t)blockIdx.x * 4 + wv; c < C; c += (int64_t)gridDim.x * 4) {
+        const bool mine = lane < n && key == (uint32_t)c;
+        const uint64_t all = __ballot(mine);
+        wave_fence();                                    // the row before has read its list
+        if (mine) list[wv][__popcll(all & ((1ull << lane) - 1ull))] = lane;
+        wave_fence();
+        for (int col0 = blockIdx.y * 64 * V; col0 < w; col0 += gridDim.y * 64 * V) {
+            RowSum<T, V, TAIL> sum;
+            sum.clear();
+            if (all) {
+                sum.add(list[wv], 0, (uint32_t)__popcll(all), G, ldg, w, col0, lanes);
+                sum.join(lanes);
+            }
+            if (lane < lanes) {
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = sum.acc[v] * scale;
+                store_vec<T, V, TAIL>(dW + c * ldw, col0 + lane * V, w, y);
+            }
+        }
+    }
+}
+
 // ---- tables of at most FEW rows (class labels): no sort.  A wave walks `per_wave` tokens and keeps a sum of every row for its
 // 64 columns in LDS; its token is the same in all lanes, so each lane adds to its own word.  The four waves' sums are added
 // in order and go to part[workgroup][row][column], which k_token_few_join adds in order.  13,752 tokens of 10 labels x 64
-// float32: two launches and 11 us, where the sort's eight launches took 31 us.
+// float32: two launches and 11 us, where sort, borders, sums and join are five launches and 26 us.
 constexpr int FEW = 32;
 template <class T>
 __global__ void __launch_bounds__(256)
@@ -520,6 +542,8 @@ template <class Fn> static inline int with_digit(int bits, Fn&& fn) {
     }
 }
 
+static inline bool direct_rows(int64_t n) { return n > 0 && n <= DIRECT; }
+
 struct TokenLayout {
     int64_t nblk, keys[2], pos[2], counts, rowptr, part, bytes;
     uint32_t cut;
@@ -527,6 +551,10 @@ struct TokenLayout {
 };
 static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
     TokenLayout l{};
+    if (direct_rows(n)) {
+        l.bytes = 256;                                   // none is used; never 0, so that every call has a workspace
+        return l;
+    }
     if (few_rows(C, w)) {
         const int64_t per = 4 * few_per_wave(n, C);
         l.nblk = (n + per - 1) / per;
@@ -598,6 +626,26 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
                "gm_token_embedding_bwd needs %lld workspace bytes (gm_token_embedding_bwd_workspace_bytes)", (long long)l.bytes);
     hipStream_t s = as_stream(stream);
     char* ws = static_cast<char*>(workspace);
+    const int vec = w < 16 / dtype_size(dtype) ? 1 : 16 / dtype_size(dtype);        // with_row_form
+    const int64_t vecs = (w + vec - 1) / vec;
+    int lanes = 64;
+    while (lanes > 1 && lanes / 2 >= vecs) lanes /= 2;
+    // a wave walks the tiles of its row where the rows alone fill the chip eight times over
+    int64_t tiles = (vecs + 63) / 64;
+    if (tiles > 1 && C >= 65536 / tiles) tiles = C >= 65536 ? 1 : (65536 + C - 1) / C;
+    GM_REQUIRE(tiles < 65536, "w too large");
+    const unsigned rows = grid_for((C + 3) / 4, 512);
+    if (direct_rows(n))
+        return with_dtype(dtype, [&](auto t) -> int {
+            using T = decltype(t);
+            with_row_form<T>(w, [&](auto v, auto tail) {
+                hipLaunchKernelGGL((k_token_direct<T, decltype(v)::value, decltype(tail)::value>), dim3(rows, (unsigned)tiles), dim3(256), 0, s,
+                                   (int)n, C, (int)w, lanes, padding_idx, IndexArray{tokens, tokens_i64}, static_cast<const T*>(G), ldg, scale,
+                                   static_cast<T*>(dW), ldw);
+            });
+            GM_LAUNCH_CHECK();
+            return GM_OK;
+        });
     if (few_rows(C, w)) {
         float* few = static_cast<float*>(workspace);
         return with_dtype(dtype, [&](auto t) -> int {
@@ -632,8 +680,6 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
             hipLaunchKernelGGL(k_radix_count, dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr, sort_keys(n),
                                p * BITS, BITS, counts);
             GM_LAUNCH_CHECK();
-            hipLaunchKernelGGL(k_radix_scan, dim3(1), dim3(1024), 0, s, l.nblk << BITS, counts);
-            GM_LAUNCH_CHECK();
             hipLaunchKernelGGL((k_radix_scatter<BITS>), dim3((unsigned)l.nblk), dim3(256), 0, s, n, C, padding_idx, tok, p ? keys : nullptr,
                                p ? pos : nullptr, sort_keys(n), p * BITS, counts, ko, po);
             GM_LAUNCH_CHECK();
@@ -645,15 +691,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     if (rc != GM_OK) return rc;
     hipLaunchKernelGGL(k_token_rowptr, dim3((unsigned)((C + 1 + 255) / 256)), dim3(256), 0, s, n, C, keys, rowptr);
     GM_LAUNCH_CHECK();
-    const int vec = w < 16 / dtype_size(dtype) ? 1 : 16 / dtype_size(dtype);        // with_row_form
-    const int64_t vecs = (w + vec - 1) / vec;
-    int lanes = 64;
-    while (lanes > 1 && lanes / 2 >= vecs) lanes /= 2;
-    // a wave walks the tiles of its row where the rows alone fill the chip eight times over
-    int64_t tiles = (vecs + 63) / 64;
-    if (tiles > 1 && C >= 65536 / tiles) tiles = C >= 65536 ? 1 : (65536 + C - 1) / C;
     const unsigned chunks = (unsigned)((n + l.cut - 1) / l.cut);
-    GM_REQUIRE(tiles < 65536, "w too large");
     const int64_t ldp = (w + 3) / 4 * 4;
     int wide = 1;
     while (wide < 256 && wide * 4 < w) wide *= 2;
@@ -665,7 +703,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
             constexpr bool TAIL = decltype(tail)::value;
             status = [&]() -> int {
                 const unsigned pieces = n > l.cut ? (chunks + 3) / 4 : 0;
-                hipLaunchKernelGGL((k_token_grad<T, V, TAIL>), dim3(pieces + grid_for((C + 3) / 4, 512), (unsigned)tiles), dim3(256), 0, s, n, C, (int)w,
+                hipLaunchKernelGGL((k_token_grad<T, V, TAIL>), dim3(pieces + rows, (unsigned)tiles), dim3(256), 0, s, n, C, (int)w,
                                    lanes, l.cut, pieces, keys, rowptr, pos, static_cast<const T*>(G), ldg, part, ldp, scale,
                                    static_cast<T*>(dW), ldw);
                 GM_LAUNCH_CHECK();

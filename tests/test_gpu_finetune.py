@@ -125,6 +125,16 @@ def test_token_embedding_hot_rows(dev, n, C):
     check_embedding(rnd(6, C, 16), torch.full((n,), C // 2), 1.0, C // 2, dev)   # all padding
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n, C, w", [(2, 82, 559), (63, 40, 3), (64, 1000, 40), (64, 3, 1030), (65, 1000, 40), (16385, 5000, 5), (300001, 90000, 1)])
+def test_token_embedding_bad_tokens_and_padding(dev, dt, n, C, w):
+    """Around the borders of the gradient's forms: the same token often, tokens outside the table on either side, padding."""
+    t = torch.randint(-2, C + 2, (n,), generator=torch.Generator().manual_seed(n))
+    t[::3] = C // 3
+    check_embedding(rnd(9, C, w, dtype=DT[dt]), t, 0.7, C // 2, dev)
+    check_embedding(rnd(9, C, w, dtype=DT[dt]), t.to(torch.int32), 1.0, C // 3, dev)
+
+
 def test_token_embedding_is_reproducible_and_strided(dev):
     C, w, n = 5000, 40, 9001
     t = (torch.rand(n, generator=torch.Generator().manual_seed(1)) ** 4 * C).long().to(dev)
