@@ -360,10 +360,11 @@ static inline int64_t norm_blocks_fwd(int64_t M, int rows, int threads) {
     const int64_t want = (M + rows - 1) / rows, most = 256 * (1024 / threads);
     return want < most ? want : most;
 }
-// workgroups of the backward: two on every CU of up to 256 threads, else one (which is what their registers leave room for; a
-// second round of them writes the column sums twice: 4095 x 16384 bf16 121 instead of 99 us), with as many rows as it takes
-static inline int64_t norm_blocks(int64_t M, int rows, int threads) {
-    const int64_t most = threads >= 512 ? 256 : 512;
+// Workgroups of the backward, each with as many rows as it takes: two on every CU, or one of 512 and 1024 threads that hold their
+// row, whose registers leave no room for a second (a second round of them writes the column sums twice: 4095 x 16384 bf16 121
+// instead of 99 us).  Rows that are not held (tpr = 0) keep two (1023 x 32768 float32: 270 us, with one 334).
+static inline int64_t norm_blocks(int64_t M, int rows, int tpr) {
+    const int64_t most = tpr >= 512 ? 256 : 512;
     return M < most * rows ? (M + rows - 1) / rows : most;
 }
 
@@ -430,7 +431,7 @@ extern "C" int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ld
 
 extern "C" int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
     if (M < 0 || N <= 0 || M >= (1ll << 31) || N >= (1ll << 26)) return -1;
-    return norm_blocks(M, 1, 256) * 2 * N * 4;               // whatever the row type
+    return norm_blocks(M, 1, 0) * 2 * N * 4;                 // whatever the row type
 }
 
 extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ldg, const void* X, int64_t ldx, int dtype,
@@ -439,7 +440,7 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
     GM_NORM_CHECK();
     GM_REQUIRE(M == 0 || (G && X && mean && rstd && ldg >= N && ldx >= N && (!dX || lddx >= N)), "bad arguments");
     const bool cols = dgamma || dbeta;
-    int64_t nblk = norm_blocks(M, 1, 256);
+    int64_t nblk = norm_blocks(M, 1, 0);
     const int64_t need = nblk * 2 * N * 4;
     GM_REQUIRE(!cols || M == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
                "gm_layer_norm_bwd needs %lld workspace bytes (gm_layer_norm_bwd_workspace_bytes)", (long long)need);
@@ -453,7 +454,7 @@ extern "C" int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ld
             const RowShape r = row_shape(N, VEC<T>, 4);
 #define GM_LAUNCH_NORM(KERNEL, ROWS, THREADS)                                                                             \
     do {                                                                                                                  \
-        nblk = norm_blocks(M, ROWS, THREADS);                                                                                      \
+        nblk = norm_blocks(M, ROWS, r.tpr);                                                                                        \
         hipLaunchKernelGGL(KERNEL, dim3((unsigned)nblk), dim3(THREADS), 0, s, M, N, static_cast<const T*>(G), ldg,        \
                            static_cast<const T*>(X), ldx, mean, rstd, w, static_cast<T*>(dX), lddx, part);                \
     } while (0)
