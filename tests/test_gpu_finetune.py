@@ -848,6 +848,57 @@ def test_upstream_gradients_and_inplace_loss(dev):
     assert torch.equal(g1 / 4, g4)                       # a power of two
 
 
+@pytest.mark.parametrize("C", [5, 200])
+def test_token_embedding_without_tokens_and_of_one(dev, C):
+    W = rnd(1, C, 24).to(dev).requires_grad_(True)
+    for shape in ((0,), (3, 0)):
+        y = ag.token_embedding(W, torch.empty(shape, dtype=torch.int64, device=dev))
+        assert y.shape == shape + (24,)
+        (dW,) = torch.autograd.grad(y.sum(), [W])
+        assert not dW.any()
+    y = ag.token_embedding(W, torch.tensor(C - 1, device=dev), scale=2.0)        # no dimension
+    assert y.shape == (24,) and torch.equal(y, 2 * W.detach()[C - 1])
+    (dW,) = torch.autograd.grad(y.sum(), [W])                                    # the gradient of a sum: one element, expanded
+    assert (dW[C - 1] == 2).all() and not dW[:C - 1].any()
+    y = ag.token_embedding(W, torch.arange(C, device=dev)) + ag.token_embedding(W, torch.arange(C, device=dev).flip(0))
+    assert (torch.autograd.grad(y.sum(), [W])[0] == 2).all()                     # the same table twice
+
+
+def test_single_rows_and_inference_mode(dev):
+    x = rnd(1, 70).to(dev).requires_grad_(True)
+    gamma, beta = rnd(2, 70).to(dev).requires_grad_(True), rnd(3, 70).to(dev)
+    got = torch.autograd.grad(ag.layer_norm(x, gamma, beta).sum(), [x, gamma])
+    rows = ag.layer_norm(x[None], gamma, beta)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(rows.sum(), [x, gamma])))
+    lp = ag.class_log_prob(x, torch.tensor(9, device=dev))                       # one row, a class without a dimension
+    assert lp.shape == () and torch.equal(lp, ag.class_log_prob(x[None], torch.tensor([9], device=dev))[0])
+    (dx,) = torch.autograd.grad(lp, [x])
+    close(dx, torch.nn.functional.one_hot(torch.tensor(9), 70).double() - x.detach().cpu().double().softmax(0), (D(70) + 8) * U, "one row")
+    with torch.inference_mode():
+        y = ag.layer_norm(x, gamma, beta)
+        assert not y.requires_grad and torch.equal(y, rows[0])
+        assert torch.equal(ag.class_log_prob(x, torch.tensor(9, device=dev)), lp)
+        loss, _ = ag.policy_loss(y, y, y)
+        assert not loss.requires_grad
+    e = torch.empty(0, 70, device=dev, requires_grad=True)
+    got = torch.autograd.grad(ag.layer_norm(e, gamma, beta).sum(), [e, gamma])
+    assert got[0].shape == (0, 70) and not got[1].any()
+    assert ag.class_log_prob(e, torch.empty(0, dtype=torch.int32, device=dev)).shape == (0,)
+
+
+def test_losses_of_strided_and_many_dimensional_items(dev):
+    """Items in a transposed batch: the losses take them in the order of the tensor's indexes."""
+    lp = (-rnd(1, 12, 7).abs()).to(dev)
+    old, ref, adv = (lp + 0.1 * rnd(k, 12, 7).to(dev) for k in (2, 3, 4))
+    mask = rnd(5, 12, 7).to(dev) > 0
+    a, b = lp.t().detach().requires_grad_(True), lp.t().contiguous().requires_grad_(True)
+    for f in (lambda q: ag.policy_loss(q, old.t(), adv.t(), mask=mask.t(), ref_log_prob=ref.t(), kl_coef=0.1),
+              lambda q: ag.preference_loss(q, ref.t(), torch.tensor([0, 9, 9, 50, 84], device=dev), mask=mask.t())):
+        x, y = f(a), f(b)
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+        assert torch.equal(torch.autograd.grad(x[0], [a])[0], torch.autograd.grad(y[0], [b])[0])
+
+
 # ------------------------------------------------------------------ sizes past 32 bits
 def test_rows_past_2_31_elements(dev):
     M, N = 262_147, 8200                                 # 2.15e9 elements, 4.3 GB in 16 bits
