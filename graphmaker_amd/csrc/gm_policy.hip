@@ -20,6 +20,13 @@
 namespace gm {
 
 constexpr int SEQ_FUSED = 64;        // sequences up to which one workgroup both gathers the pieces and forms the loss
+// Sequences up to which one workgroup forms the loss and the weights (8000: 9 us, in two launches 12), and the most workgroups that
+// do beyond.
+constexpr int SEQ_ONE = 8192, FINISH_BLOCKS = 256;
+static inline unsigned finish_blocks(int64_t S) {
+    const int64_t want = S <= SEQ_ONE ? 1 : (S + 4095) / 4096;
+    return (unsigned)(want < FINISH_BLOCKS ? want : FINISH_BLOCKS);
+}
 
 struct Sequences {
     IndexArray offsets;              // p == NULL: all items are one sequence
@@ -279,33 +286,54 @@ template <int N> __device__ __forceinline__ void block_add(double (&v)[N], doubl
     }
 }
 
-// The losses and the sequences' weights, by one workgroup: 8 us for up to a few thousand sequences, latency of the pieces, the
-// sums and the weights one behind the other; 100,000 sequences 160 us.
+// what sequence s adds to a batch's totals: the sums, live items, sequences that have one
+__device__ __forceinline__ void add_sequence(const Sums<4>& w, int by_sequence, double (&tot)[5]) {
+    const double unit = w.v[3] > 0.0 && by_sequence ? 1.0 / w.v[3] : 1.0;
+    tot[4] += w.v[3] > 0.0 ? 1.0 : 0.0;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) tot[c] += w.v[c] * unit;
+    tot[3] += w.v[3];
+}
+// totals of a workgroup's share of many sequences
+__global__ void __launch_bounds__(1024)
+k_policy_totals(int64_t S, int by_sequence, const Sums<4>* __restrict__ whole, Sums<5>* __restrict__ totals) {
+    __shared__ double red[16][5];
+    double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+    for (int64_t s = (int64_t)blockIdx.x * 1024 + threadIdx.x; s < S; s += (int64_t)gridDim.x * 1024) add_sequence(whole[s], by_sequence, tot);
+    block_add(tot, red);
+    if (threadIdx.x == 0)
+#pragma unroll
+        for (int c = 0; c < 5; ++c) totals[blockIdx.x].v[c] = tot[c];
+}
+// The losses and the sequences' weights.  One workgroup up to SEQ_ONE sequences: 8 us, latency of the pieces, the sums and the
+// weights one behind the other.  Beyond, every workgroup adds all workgroups' totals in order and writes its share of the weights
+// (100,000 sequences 14 us with k_policy_totals, by one workgroup 160; 4 million 48 us, by one 3900).
 __global__ void __launch_bounds__(1024)
 k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, const Sums<4>* __restrict__ whole,
-                const Sums<4>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ weight) {
+                const Sums<4>* __restrict__ piece, const Sums<5>* __restrict__ totals, float* __restrict__ loss, float* __restrict__ stats,
+                float* __restrict__ weight) {
     __shared__ double red[16][5];
     __shared__ Sums<4> held[SEQ_FUSED];
     if (gather) gather_all<4>(q, chunk, whole, piece, held);
-    double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};           // the sums, live items, sequences that have one
-#pragma unroll 4
-    for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
-        const Sums<4> w = gather ? held[s] : whole[s];
-        const double unit = w.v[3] > 0.0 && by_sequence ? 1.0 / w.v[3] : 1.0;
-        tot[4] += w.v[3] > 0.0 ? 1.0 : 0.0;
+    double tot[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+    if (gridDim.x > 1) {
+        if (threadIdx.x < gridDim.x)
 #pragma unroll
-        for (int c = 0; c < 3; ++c) tot[c] += w.v[c] * unit;
-        tot[3] += w.v[3];
+            for (int c = 0; c < 5; ++c) tot[c] = totals[threadIdx.x].v[c];
+    } else {
+#pragma unroll 4
+        for (int64_t s = threadIdx.x; s < q.S; s += 1024) add_sequence(gather ? held[s] : whole[s], by_sequence, tot);
     }
     block_add(tot, red);
     const double over = by_sequence ? tot[4] : tot[3];
     const double norm = over > 0.0 ? 1.0 / over : 0.0;    // no live item: the loss and every gradient are 0
 #pragma unroll 4
-    for (int64_t s = threadIdx.x; s < q.S; s += 1024) {
+    for (int64_t s = (int64_t)blockIdx.x * 1024 + threadIdx.x; s < q.S; s += (int64_t)gridDim.x * 1024) {
         const double n = gather ? held[s].v[3] : whole[s].v[3];
         if (weight) weight[s] = n > 0.0 ? (float)(by_sequence ? norm / n : norm) : 0.0f;
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) {
         const double surrogate = tot[0] * norm, apart = tot[1] * norm;
         loss[0] = (float)(kl != 0.0f ? surrogate + (double)kl * apart : surrogate);
         stats[0] = (float)surrogate;
@@ -317,14 +345,15 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
 
 __global__ void __launch_bounds__(1024)
 k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double smoothing, int average, const Sums<2>* __restrict__ whole,
-                    const Sums<2>* __restrict__ piece, float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ weight) {
+                    const Sums<2>* __restrict__ piece, double* __restrict__ totals, float* __restrict__ loss, float* __restrict__ rewards,
+                    float* __restrict__ weight) {
     __shared__ double red[16][1];
     __shared__ Sums<2> held[SEQ_FUSED];
     if (gather) gather_all<2>(q, chunk, whole, piece, held);
     const int64_t P = q.S / 2;
     double tot[1] = {0.0};
 #pragma unroll 2
-    for (int64_t p = threadIdx.x; p < P; p += 1024) {
+    for (int64_t p = (int64_t)blockIdx.x * 1024 + threadIdx.x; p < P; p += (int64_t)gridDim.x * 1024) {
         double h[2], unit[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -342,6 +371,16 @@ k_preference_finish(Sequences q, int64_t chunk, int gather, double beta, double 
             weight[2 * p + 1] = (float)(-beta * dz * unit[1]);
         }
     }
+    block_add(tot, red);
+    if (threadIdx.x == 0) {
+        if (gridDim.x > 1) totals[blockIdx.x] = tot[0];
+        else loss[0] = (float)(tot[0] / (double)P);
+    }
+}
+// the loss from the workgroups' totals
+__global__ void __launch_bounds__(1024) k_preference_total(int parts, int64_t P, const double* __restrict__ totals, float* __restrict__ loss) {
+    __shared__ double red[16][1];
+    double tot[1] = {(int)threadIdx.x < parts ? totals[threadIdx.x] : 0.0};
     block_add(tot, red);
     if (threadIdx.x == 0) loss[0] = (float)(tot[0] / (double)P);
 }
@@ -398,14 +437,15 @@ static inline unsigned gather_blocks(int64_t S, int per) {
     return (unsigned)(want < 4096 ? want : 4096);
 }
 
-struct SequenceLayout { int64_t nchunk, whole, piece, bytes; };
+struct SequenceLayout { int64_t nchunk, whole, piece, totals, bytes; };
 static inline SequenceLayout sequence_layout(int64_t M, int64_t S) {
     SequenceLayout l;
     const int64_t chunk = chunk_items(M);
     l.nchunk = (M + chunk - 1) / chunk;
     l.whole = 0;
     l.piece = S * (int64_t)sizeof(Sums<4>);
-    l.bytes = l.piece + 2 * l.nchunk * (int64_t)sizeof(Sums<4>);
+    l.totals = l.piece + 2 * l.nchunk * (int64_t)sizeof(Sums<4>);
+    l.bytes = l.totals + (finish_blocks(S) > 1 ? FINISH_BLOCKS * (int64_t)sizeof(Sums<5>) : 0);
     return l;
 }
 
@@ -429,9 +469,7 @@ static int launch_sequence_loss(const Sequences& q, const F& f, void* workspace,
         hipLaunchKernelGGL((k_sequence_gather<Q>), dim3(gather_blocks(q.S, per)), dim3(256), 0, s, q, chunk, per, whole, piece);
         GM_LAUNCH_CHECK();
     }
-    finish(chunk, fused, whole, piece);
-    GM_LAUNCH_CHECK();
-    return GM_OK;
+    return finish(chunk, fused, whole, piece, static_cast<void*>(static_cast<char*>(workspace) + l.totals));
 }
 
 // fn(b0, b1, ...) with each flag as an integral constant
@@ -470,8 +508,17 @@ extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, c
     return with_flags(mask != nullptr, ref_log_prob != nullptr, offsets == nullptr, [&](auto m, auto r, auto item) {
         const PolicyTerm<decltype(m)::value, decltype(r)::value, decltype(item)::value> f{
             log_prob, old_log_prob, advantage, ref_log_prob, mask, 1.0f - clip_low, 1.0f + clip_high, kl_coef, slope};
-        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece) {
-            hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, loss, stats, weight);
+        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece, void* rest) {
+            const unsigned blocks = finish_blocks(S);
+            Sums<5>* totals = static_cast<Sums<5>*>(rest);
+            if (blocks > 1) {
+                hipLaunchKernelGGL(k_policy_totals, dim3(blocks), dim3(1024), 0, s, S, by_sequence, whole, totals);
+                GM_LAUNCH_CHECK();
+            }
+            hipLaunchKernelGGL(k_policy_finish, dim3(blocks), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, totals, loss,
+                               stats, weight);
+            GM_LAUNCH_CHECK();
+            return GM_OK;
         });
     });
 }
@@ -490,9 +537,17 @@ extern "C" int gm_preference_loss_fwd(int64_t M, int64_t P, const float* log_pro
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
     return with_flags(mask != nullptr, [&](auto m) {
         const PreferenceTerm<decltype(m)::value> f{log_prob, ref_log_prob, mask};
-        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<2>* whole, Sums<2>* piece) {
-            hipLaunchKernelGGL(k_preference_finish, dim3(1), dim3(1024), 0, s, q, chunk, fused, (double)beta, (double)label_smoothing, average,
-                               whole, piece, loss, rewards, weight);
+        return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<2>* whole, Sums<2>* piece, void* rest) {
+            const unsigned blocks = finish_blocks(S);
+            double* totals = static_cast<double*>(rest);
+            hipLaunchKernelGGL(k_preference_finish, dim3(blocks), dim3(1024), 0, s, q, chunk, fused, (double)beta, (double)label_smoothing,
+                               average, whole, piece, totals, loss, rewards, weight);
+            GM_LAUNCH_CHECK();
+            if (blocks > 1) {
+                hipLaunchKernelGGL(k_preference_total, dim3(1), dim3(1024), 0, s, (int)blocks, P, totals, loss);
+                GM_LAUNCH_CHECK();
+            }
+            return GM_OK;
         });
     });
 }

@@ -184,9 +184,8 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
     }
 }
 
-// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch (2048 tokens 10 us, latency).
-//  Each wave holds `rounds` x 64 keys that
-// are consecutive in the current order in registers; the keys change places through LDS.
+// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch (2048 tokens 10 us, latency).  Each
+// wave holds `rounds` x 64 keys that are consecutive in the current order in registers; the keys change places through LDS.
 constexpr int SMALL_WAVES = 16, SMALL_ROUNDS = 8, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64, SMALL_BITS = 8;
 template <int BITS>
 __global__ void __launch_bounds__(SMALL_WAVES * 64)

@@ -848,6 +848,17 @@ def test_upstream_gradients_and_inplace_loss(dev):
     assert torch.equal(g1 / 4, g4)                       # a power of two
 
 
+@pytest.mark.parametrize("S, M", [(8192, 9000), (8194, 9000), (300000, 400001), (1200000, 700000)])
+def test_losses_of_many_short_sequences(dev, S, M):
+    """More sequences than one workgroup takes: the totals and the weights come from several."""
+    lp, old, ref = ratios(S, M)
+    mask = torch.rand(M, generator=torch.Generator().manual_seed(S)) < 0.8
+    off = ragged(S + 1, S, M)
+    for reduction in ("token", "sequence"):
+        check_policy(lp, old, rnd(S, S), dev, ref=ref, mask=mask, offsets=off, kl=0.05, reduction=reduction)
+    check_preference(lp, ref, off, dev, mask=mask, beta=0.3, smoothing=0.1, average=True)
+
+
 @pytest.mark.parametrize("C", [5, 200])
 def test_token_embedding_without_tokens_and_of_one(dev, C):
     W = rnd(1, C, 24).to(dev).requires_grad_(True)
