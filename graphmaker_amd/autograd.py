@@ -20,7 +20,8 @@ float32, bfloat16 or float16 rows, sums in float32 or float64):
     policy_loss(log_prob, old_log_prob, advantage, ...)            clipped policy loss with a KL term
     preference_loss(log_prob, ref_log_prob, offsets, ...)          loss of preferred over rejected sequences
 They enqueue on the current stream of their tensors' device, keep their workspaces to one call, read nothing back to the
-host and can be captured in a HIP graph, forward and backward.  A captured call is refused while a graph that was recorded
+host and can be captured in a HIP graph, forward and backward.  They have no second and no forward-mode derivative: asking for
+one is an error.  A captured call is refused while a graph that was recorded
 eagerly on another stream over the same leaf tensor is alive (torch runs the leaf's gradient accumulation on that stream, and
 the process would end): drop such graphs, their losses and outputs, before capturing.
 """

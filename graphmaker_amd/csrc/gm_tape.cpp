@@ -64,6 +64,13 @@ void same_device(const Tensor& t, const char* what, const Tensor& like) {
     if (t.device() != like.device()) throw py::value_error(say(what, ": on ", t.device(), ", expected ", like.device()));
 }
 
+// A dual number (torch.autograd.forward_ad) is refused: these operators have no forward-mode derivative, and an output without a
+// tangent would count as a derivative of zero.
+void no_tangent(const Tensor& t, const char* what) {
+    if (t.defined() && t._fw_grad(0).defined())
+        C10_THROW_ERROR(NotImplementedError, say(what, " has a tangent: this graphmaker_amd operator has no forward-mode derivative"));
+}
+
 // an index argument, contiguous, int32 or int64
 Tensor index_of(const Tensor& t, const char* what, const Tensor& like) {
     if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
@@ -170,6 +177,7 @@ Tensor token_embedding(const Tensor& weight, const Tensor& tokens, double scale,
     if (weight.dim() != 2 || weight.numel() == 0)
         throw py::value_error(say("token_embedding: weight must be (C, w) with C, w > 0, got ", weight.sizes()));
     row_dtype(weight, "weight");
+    no_tangent(weight, "weight");
     const Tensor tok = index_of(tokens, "tokens", weight);
     const int64_t C = weight.size(0);
     if (!std::isfinite((float)scale)) throw py::value_error(say("token_embedding: scale must be finite in float32, got ", scale));
@@ -239,6 +247,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& gamma_, const st
     const int64_t N = x.dim() ? x.size(-1) : 0;
     if (N == 0) throw py::value_error(say("layer_norm: x must have a last dimension of at least 1, got ", x.sizes()));
     row_dtype(x, "x");
+    no_tangent(x, "x");
     Tensor weights[2] = {gamma_.value_or(Tensor()), beta_.value_or(Tensor())};
     for (int k = 0; k < 2; ++k) {
         const Tensor& t = weights[k];
@@ -248,6 +257,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& gamma_, const st
         if (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat)
             throw py::type_error(say("layer_norm: ", what, " is ", t.scalar_type(), ", expected ", x.scalar_type(), " or float32"));
         same_device(t, what, x);
+        no_tangent(t, what);
     }
     if (weights[0].defined() && weights[1].defined() && weights[0].scalar_type() != weights[1].scalar_type())
         throw py::type_error(say("layer_norm: gamma is ", weights[0].scalar_type(), " and beta is ", weights[1].scalar_type()));
@@ -309,6 +319,7 @@ Tensor class_log_prob(const Tensor& logits, const Tensor& classes, int64_t ignor
     if (classes.sizes() != logits.sizes().slice(0, logits.dim() - 1))
         throw py::value_error(say("class_log_prob: classes is ", classes.sizes(), ", logits is ", logits.sizes()));
     row_dtype(logits, "logits");
+    no_tangent(logits, "logits");
     const Tensor cls = index_of(classes, "classes", logits);
     on_gpu(logits, "logits");
     if (records(logits)) return ClassLogProb::apply(logits, cls, ignore_index);
@@ -319,6 +330,7 @@ Tensor class_log_prob(const Tensor& logits, const Tensor& classes, int64_t ignor
 // ------------------------------------------------------------------ losses over sequences
 void constant(const Tensor& t, const char* what) {
     if (t.requires_grad()) throw py::value_error(say(what, " is a constant of the loss and gets no gradient: pass ", what, ".detach()"));
+    no_tangent(t, what);
 }
 Tensor items(const Tensor& t, const char* what) {
     if (t.scalar_type() != at::kFloat) throw py::type_error(say(what, ": expected float32, got ", t.scalar_type()));
@@ -434,6 +446,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& log_prob, const Tensor& old_
     LossArgs a{};
     a.S = 1;
     items(log_prob, "log_prob");
+    no_tangent(log_prob, "log_prob");
     a.old = items_like(old_log_prob, "old_log_prob", log_prob);
     if (ref_log_prob && ref_log_prob->defined()) a.ref = items_like(*ref_log_prob, "ref_log_prob", log_prob);
     a.mask = mask_like(mask, log_prob);
@@ -469,6 +482,7 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& log_prob, const Tensor& 
                                           const std::optional<Tensor>& mask, double beta, double label_smoothing, bool average) {
     LossArgs a{};
     items(log_prob, "log_prob");
+    no_tangent(log_prob, "log_prob");
     a.ref = items_like(ref_log_prob, "ref_log_prob", log_prob);
     a.mask = mask_like(mask, log_prob);
     a.offsets = offsets_of(offsets, log_prob);

@@ -191,3 +191,30 @@ def test_signatures_match_the_header():
         args = re.search(r"\b" + name + r"\(([^)]*)\)", header, re.S).group(1).split(",")
         want = "".join("p" if "*" in a or "gm_stream_t" in a else "i" if "int64_t" in a else "f" if "float" in a else "d" for a in args)
         assert kinds == want, name
+
+
+def dual(t):
+    import torch.autograd.forward_ad as fwd
+    return fwd.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ag.token_embedding(dual(f(4, 8)), i(3)),
+    lambda: ag.layer_norm(dual(f(3, 4)), f(4), f(4)),
+    lambda: ag.layer_norm(f(3, 4), dual(f(4)), f(4)),
+    lambda: ag.layer_norm(f(3, 4), None, dual(f(4))),
+    lambda: ag.layer_norm(dual(f(3, 4)), f(4, grad=True), f(4)),
+    lambda: ag.class_log_prob(dual(f(3, 4)), i(3)),
+    lambda: ag.policy_loss(dual(f(6)), f(6), f(6)),
+    lambda: ag.policy_loss(f(6, grad=True), dual(f(6)), f(6)),
+    lambda: ag.policy_loss(f(6), f(6), dual(f(6))),
+    lambda: ag.policy_loss(f(6), f(6), dual(f(2)), offsets=i(3)),
+    lambda: ag.policy_loss(f(6), f(6), f(6), ref_log_prob=dual(f(6))),
+    lambda: ag.preference_loss(dual(f(6)), f(6), i(3)),
+    lambda: ag.preference_loss(f(6), dual(f(6)), i(3)),
+])
+def test_forward_mode_derivatives_are_refused(call):
+    """An output without a tangent would count as a derivative of zero; the package's other operators raise this error too."""
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        call()
