@@ -108,9 +108,10 @@ template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const bool live = !MASK || on.v[k] != 0;
-            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, r = exp_any(l.v[k] - o.v[k]);
+            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, d_k = l.v[k] - o.v[k], r = exp_any(d_k);
             const bool cut = (adv_k > 0.0f && r > high) || (adv_k < 0.0f && r < low);
-            const float gain = adv_k == 0.0f ? 0.0f : (cut ? (adv_k > 0.0f ? high : low) : r) * adv_k;
+            // no advantage: 0 for a ratio of any finite size, also one past float32; NaN for NaN and for an infinite ratio
+            const float gain = adv_k == 0.0f && d_k < INFINITY ? 0.0f : (cut ? (adv_k > 0.0f ? high : low) : r) * adv_k;
             float slope_k = cut ? 0.0f : -gain, apart = 0.0f;
             if constexpr (REF) {
                 const float x = q.v[k] - l.v[k];
