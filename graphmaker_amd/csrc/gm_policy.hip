@@ -74,27 +74,55 @@ static inline int64_t spread_items(int64_t M) { return M <= 1024 * 512 ? 512 : 2
 
 template <int Q> struct alignas(8) Sums { double v[Q]; };
 
-// exp(x) - 1 - x: the series where the difference would cancel (its first left-out term is below 2^-24 of the sum)
-__device__ __forceinline__ float exp_minus_1_x(float x) {
-    float p = 2.75573192e-7f;                           // 1/10!
-    p = __builtin_fmaf(p, x, 2.75573192e-6f);
-    p = __builtin_fmaf(p, x, 2.48015873e-5f);
-    p = __builtin_fmaf(p, x, 1.98412698e-4f);
-    p = __builtin_fmaf(p, x, 1.38888889e-3f);
-    p = __builtin_fmaf(p, x, 8.33333333e-3f);
-    p = __builtin_fmaf(p, x, 4.16666667e-2f);
-    p = __builtin_fmaf(p, x, 1.66666667e-1f);
-    p = __builtin_fmaf(p, x, 0.5f);
-    return __builtin_fabsf(x) < 1.0f ? p * x * x : exp_any(x) - 1.0f - x;
+// A batch's items are formed times `unit`, 2^-20 / M rounded down to a power of two: e^89 leaves float32, its share of the mean and
+// the KL coefficient's share of that do not.  What it takes from the small side, values below 2^-72, is nothing beside any other
+// item.  The sums take the unit back at the end, the weights of the gradient carry it the other way round.
+struct Unit { float u; int shift; };                     // u = 2^-shift
+static inline Unit item_unit(int64_t M) {
+    const int shift = 20 + (M > 0 ? 63 - __builtin_clzll((unsigned long long)M) : 0);
+    return {1.0f / (float)(1ull << shift), shift};
 }
+// exp(x) 2^-shift within about two units in the last place: exp_any with its power of two put on at the end
+__device__ __forceinline__ float exp_shifted(float x, int shift) {
+    x = x < -2000.0f ? -2000.0f : x > 2000.0f ? 2000.0f : x;   // 0 and infinity either way
+    const float t = x * 1.44269502f, n = __builtin_rintf(t);
+    const float lo = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f(t - n) * __builtin_fmaf(lo, 0.693147182f, 1.0f), (int)n - shift);
+}
+// exp(x) less 1, and less 1 + x, times the unit.  Below |x| = 1 from the series, where the differences would cancel (the first
+// term left out is below 1.2 x 2^-24 of the sum)
+struct LessOne {
+    float one, line;
+    __device__ __forceinline__ LessOne(float x, Unit unit) {
+        float p = 2.75573192e-7f;                       // 1/10!
+        p = __builtin_fmaf(p, x, 2.75573192e-6f);
+        p = __builtin_fmaf(p, x, 2.48015873e-5f);
+        p = __builtin_fmaf(p, x, 1.98412698e-4f);
+        p = __builtin_fmaf(p, x, 1.38888889e-3f);
+        p = __builtin_fmaf(p, x, 8.33333333e-3f);
+        p = __builtin_fmaf(p, x, 4.16666667e-2f);
+        p = __builtin_fmaf(p, x, 1.66666667e-1f);
+        p = __builtin_fmaf(p, x, 0.5f);
+        const float xu = x * unit.u;
+        line = p * x * xu;
+        one = xu + line;
+        if (__builtin_expect(!(__builtin_fabsf(x) < 1.0f), 0)) {       // a branch: a model is seldom so far from its reference
+            one = exp_shifted(x, unit.shift) - unit.u;
+            line = one - xu;
+        }
+    }
+};
 
-// What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.
+// What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.  An item's terms are
+// float32: they carry a few 2^-24, and |x| 2^-24 from the rounded difference x of two float32 log-probabilities, which carry as much
+// themselves.  (Of 10,547,784 items these take 41.5 us, float64 terms of float32 exponentials 47 and of float64 ones 54.)
 template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
     static constexpr int Q = 4;                          // sums: surrogate, KL, clipped items, live items
     struct Acc { double surrogate = 0.0, kl = 0.0; int cut = 0, live = 0; };
     const float *lp, *old, *adv, *ref;
     const uint8_t* mask;
-    float low, high, kl;                                 // 1 - clip_low, 1 + clip_high, KL coefficient
+    Unit unit;
+    float low, high, kl;                                 // 1 - clip_low and 1 + clip_high times the unit, KL coefficient
     float* slope;
     __device__ __forceinline__ float of_sequence(int64_t s) const { return ITEM_ADV ? 0.0f : adv[s]; }
     template <int W> __device__ __forceinline__ void add(int64_t i, float of_seq, Acc& a) const {
@@ -108,18 +136,17 @@ template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const bool live = !MASK || on.v[k] != 0;
-            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, d_k = l.v[k] - o.v[k], r = exp_any(d_k);
+            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, d_k = l.v[k] - o.v[k], r = exp_shifted(d_k, unit.shift);
             const bool cut = (adv_k > 0.0f && r > high) || (adv_k < 0.0f && r < low);
             // no advantage: 0 for a ratio of any finite size, also one past float32; NaN for NaN and for an infinite ratio
             const float gain = adv_k == 0.0f && d_k < INFINITY ? 0.0f : (cut ? (adv_k > 0.0f ? high : low) : r) * adv_k;
-            float slope_k = cut ? 0.0f : -gain, apart = 0.0f;
+            float slope_k = cut ? 0.0f : -gain;
             if constexpr (REF) {
-                const float x = q.v[k] - l.v[k];
-                apart = exp_minus_1_x(x);
-                if (kl != 0.0f) slope_k = slope_k - kl * (x + apart);
+                const LessOne e(q.v[k] - l.v[k], unit);
+                if (kl != 0.0f) slope_k = slope_k - kl * e.one;
+                a.kl += live ? (double)e.line : 0.0;
             }
             a.surrogate -= live ? (double)gain : 0.0;
-            if constexpr (REF) a.kl += live ? (double)apart : 0.0;
             a.cut += live && cut ? 1 : 0;
             a.live += live ? 1 : 0;
             d.v[k] = live ? slope_k : 0.0f;
@@ -311,7 +338,7 @@ k_policy_totals(int64_t S, int by_sequence, const Sums<4>* __restrict__ whole, S
 // weights one behind the other.  Beyond, every workgroup adds all workgroups' totals in order and writes its share of the weights
 // (100,000 sequences 14 us with k_policy_totals, by one workgroup 160; 4 million 48 us, by one 3900).
 __global__ void __launch_bounds__(1024)
-k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, const Sums<4>* __restrict__ whole,
+k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float kl, float unit, const Sums<4>* __restrict__ whole,
                 const Sums<4>* __restrict__ piece, const Sums<5>* __restrict__ totals, float* __restrict__ loss, float* __restrict__ stats,
                 float* __restrict__ weight) {
     __shared__ double red[16][5];
@@ -332,10 +359,10 @@ k_policy_finish(Sequences q, int64_t chunk, int gather, int by_sequence, float k
 #pragma unroll 4
     for (int64_t s = (int64_t)blockIdx.x * 1024 + threadIdx.x; s < q.S; s += (int64_t)gridDim.x * 1024) {
         const double n = gather ? held[s].v[3] : whole[s].v[3];
-        if (weight) weight[s] = n > 0.0 ? (float)(by_sequence ? norm / n : norm) : 0.0f;
+        if (weight) weight[s] = n > 0.0 ? (float)((by_sequence ? norm / n : norm) / (double)unit) : 0.0f;
     }
     if (threadIdx.x == 0 && blockIdx.x == 0) {
-        const double surrogate = tot[0] * norm, apart = tot[1] * norm;
+        const double surrogate = tot[0] * norm / (double)unit, apart = tot[1] * norm / (double)unit;
         loss[0] = (float)(kl != 0.0f ? surrogate + (double)kl * apart : surrogate);
         stats[0] = (float)surrogate;
         stats[1] = (float)apart;
@@ -506,9 +533,10 @@ extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, c
     GM_REQUIRE(kl_coef - kl_coef == 0.0f, "kl_coef is not finite");
     hipStream_t s = as_stream(stream);
     const Sequences q{IndexArray{offsets, offsets_i64}, S, M};
+    const Unit unit = item_unit(M);
     return with_flags(mask != nullptr, ref_log_prob != nullptr, offsets == nullptr, [&](auto m, auto r, auto item) {
         const PolicyTerm<decltype(m)::value, decltype(r)::value, decltype(item)::value> f{
-            log_prob, old_log_prob, advantage, ref_log_prob, mask, 1.0f - clip_low, 1.0f + clip_high, kl_coef, slope};
+            log_prob, old_log_prob, advantage, ref_log_prob, mask, unit, (1.0f - clip_low) * unit.u, (1.0f + clip_high) * unit.u, kl_coef, slope};
         return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece, void* rest) {
             const unsigned blocks = finish_blocks(S);
             Sums<5>* totals = static_cast<Sums<5>*>(rest);
@@ -516,7 +544,7 @@ extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, c
                 hipLaunchKernelGGL(k_policy_totals, dim3(blocks), dim3(1024), 0, s, S, by_sequence, whole, totals);
                 GM_LAUNCH_CHECK();
             }
-            hipLaunchKernelGGL(k_policy_finish, dim3(blocks), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, whole, piece, totals, loss,
+            hipLaunchKernelGGL(k_policy_finish, dim3(blocks), dim3(1024), 0, s, q, chunk, fused, by_sequence, kl_coef, unit.u, whole, piece, totals, loss,
                                stats, weight);
             GM_LAUNCH_CHECK();
             return GM_OK;

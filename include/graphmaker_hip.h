@@ -382,7 +382,8 @@ int gm_class_log_prob_bwd(int64_t M, int64_t V, const float* g, const void* logi
  *               -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1), averaged over the live items, or
  *               (by_sequence) per sequence and then over the sequences that have one.  A = advantage[s], or advantage[i] where
  *               offsets is NULL (S = 1: all items).  stats (4 floats): mean surrogate, mean KL, clipped share, live items.
- *               slope (M) and weight (S), may be NULL: what the backward needs.
+ *               slope (M) and weight (S), may be NULL: what the backward needs, whose
+ *               product is an item's gradient (each carries a power of two that the other takes back).
  *   preference  sequences 2p (chosen) and 2p + 1 (rejected) of P pairs: h = sum (average: mean) of log_prob - ref,
  *               z = beta (h_chosen - h_rejected), mean over pairs of -(1 - e) log sigmoid(z) - e log sigmoid(-z),
  *               e = label_smoothing.  rewards (2P) = beta h; weight (2P), may be NULL. */

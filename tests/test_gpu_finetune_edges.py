@@ -48,3 +48,69 @@ def test_policy_loss_shows_nan_at_advantage_zero(dev, offsets):
         fine[at], fine_old[at] = x, y
         for a, b in zip(run(fine, fine_old), want):
             assert torch.equal(a, b)
+
+
+def policy_formula(lp, old, adv, ref, kl, low=0.2, high=0.28):
+    """(loss, stats, gradient) of the mean over all items in float64, and what float32 terms may be off by.
+
+    The ratio and exp(q) are float32: 4 U of the exponential and |x| U of its argument's rounding; one U more of every product,
+    sum and border.  Below |q| = 1 exp(q) - 1 - q is a series: 1.2 U left out, 4 U of its own roundings."""
+    low, high, kl = (float(torch.tensor(v, dtype=torch.float32)) for v in (low, high, kl))
+    l, A, d = lp.double().requires_grad_(True), adv.double(), lp.double() - old.double()
+    r = (l - old.double()).exp()
+    t = -torch.minimum(r * A, r.clamp(1 - low, 1 + high) * A)
+    (dt,) = torch.autograd.grad(t.sum(), [l])
+    r, t = r.detach(), t.detach()
+    cut = ((A > 0) & (r > 1 + high)) | ((A < 0) & (r < 1 - low))
+    q = ref.double() - lp.double()
+    one = torch.special.expm1(q)
+    small = q.square() / 2 * (1 + q / 3 * (1 + q / 4 * (1 + q / 5)))             # its next term is below 1e-14 of it
+    line = torch.where(q.abs() < 1e-3, small, one - q)
+    e_t = torch.where(cut, 3.0, 7 + d.abs()) * t.abs() * U
+    far = q.exp() * (4 + q.abs().nan_to_num(posinf=0.0)) + one.abs()
+    e_one = torch.where(q.abs() < 1, q.abs() + 6 * line + one.abs(), far) * U
+    e_line = torch.where(q.abs() < 1, 6 * line + q.abs() * one.abs(), far + line) * U
+    sums = torch.stack([t.mean(), line.mean(), cut.double().mean(), torch.tensor(float(lp.numel()), dtype=torch.float64)])
+    tols = torch.stack([e_t.mean(), e_line.mean(), sums[2] * 0, sums[3] * 0]) + 1.01 * U * sums.abs()
+    e_dl = (torch.where(cut, 0.0, e_t) + kl * e_one + 4 * U * (dt.abs() + 2 * kl * one.abs())) / lp.numel()
+    loss = sums[0] + kl * sums[1]
+    return loss, sums, (dt - kl * one) / lp.numel(), (tols[0] + kl * tols[1] + 1.01 * U * loss.abs(), tols, e_dl)
+
+
+def check_terms(lp, old, adv, ref, kl, dev):
+    a = lp.to(dev).requires_grad_(True)
+    loss, stats = ag.policy_loss(a, old.to(dev), adv.to(dev), ref_log_prob=ref.to(dev), kl_coef=kl, clip_high=0.28)
+    (dl,) = torch.autograd.grad(loss, [a])
+    w_loss, w_stats, w_dl, tols = policy_formula(lp, old, adv, ref, kl)
+    w_stats[w_stats > torch.finfo(torch.float32).max] = math.inf
+    close(loss, w_loss, tols[0], "loss")
+    close(stats, w_stats, tols[1], "stats")
+    close(dl, w_dl, tols[2], "gradient")
+
+
+def test_policy_loss_terms(dev):
+    M = 4097
+    lp, old, ref = ratios(11, M)
+    check_terms(lp, old, 1.0 + rnd(12, M).abs(), ref, 0.05, dev)
+    check_terms(lp, old, rnd(13, M).sign(), lp + 2.0 * rnd(14, M), 0.5, dev)     # KL arguments of either side of 1
+
+
+@pytest.mark.parametrize("q", [1e-6, -1e-3, 95.0, 100.0, -17.3, -20000.3, -1e8, -math.inf])
+def test_policy_loss_of_a_far_reference(dev, q):
+    """exp(q) past float32, whose share of the mean is not, and q so low that exp(q) - 1 is -1 whatever q is."""
+    M = 100_003
+    lp, old, ref = ratios(5, M)
+    ref[70_000] = lp[70_000] + q
+    check_terms(lp, old, 1.0 + rnd(6, M).abs(), ref, 0.04, dev)
+    check_terms(lp[69_900:70_100], old[69_900:70_100], 1.0 + rnd(6, 200).abs(), ref[69_900:70_100], 1e-3, dev)
+
+
+@pytest.mark.parametrize("d", [88.0, 90.0, 95.0, -100.0])
+def test_policy_loss_of_a_far_old_model(dev, d):
+    """A ratio past float32 that the clip leaves as it is (a negative advantage)."""
+    M = 100_003
+    lp, old, ref = ratios(5, M)
+    adv = -1.0 - rnd(6, M).abs()
+    old[70_000] = lp[70_000] - d
+    check_terms(lp, old, adv, ref, 0.0, dev)
+    check_terms(lp, old, adv, ref, 0.04, dev)
