@@ -5,7 +5,7 @@
 //
 // A row whose class is `ignore_index` has log-probability 0 and a zero gradient, whatever its logits; the gradient of a row
 // whose g is 0 is 0 too.  Any other class outside [0, V) gives NaN in both.  Sums are float32 whatever the logits' type, of
-// exponentials about the row's largest logit.  stats[i] = (largest logit, log of that sum).
+// exponentials about the row's largest logit.  stats[i] = (largest logit, that sum).
 //
 // HBM-bound: the forward reads the logits once, the backward reads them and writes as much.  Three forms by the row's size:
 //   narrow   under 16 bytes: one thread a row, which forms the softmax again in the backward instead of keeping stats
@@ -16,7 +16,7 @@
 namespace gm {
 
 // exp(x), x <= 0, without exp_any's correction, off by 1.2 |x| 2^-24 relative: for the sums of long rows, where |x| weighted by exp(x) is
-// small against the number of additions
+// small against the number of additions, and for gradients of 16 bits, beside whose rounding it is nothing (2^-17 at x = -88)
 __device__ __forceinline__ float exp_quick(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
 // x inside the row, -inf outside (by masks, as in load_vec)
@@ -79,6 +79,9 @@ k_log_prob_narrow(int64_t M, const float* __restrict__ g, const T* __restrict__ 
 // ---- held: LANES lanes a row, K pieces of V elements a lane.  Rows of 64 lanes add enough terms for exp_quick; with exp_any
 // the forward of rows of 256 to 2000 bf16 logits is bound by its arithmetic (3.7 to 4.2 TB/s).
 template <int LANES> __device__ __forceinline__ float exp_row(float x) { return LANES == 64 ? exp_quick(x) : exp_any(x); }
+// an element of the gradient stands for itself: of float32 it has all its places.  It is exp(x - largest) over the row's sum, not
+// exp(x - largest - log of the sum), whose argument is rounded twice.
+template <class T> __device__ __forceinline__ float exp_grad(float x) { return sizeof(T) == 4 ? exp_any(x) : exp_quick(x); }
 template <class T, int V, bool TAIL, int K, int LANES>
 __global__ void __launch_bounds__(256)
 k_log_prob_held(int64_t M, int N, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore, float* __restrict__ lp,
@@ -109,7 +112,7 @@ k_log_prob_held(int64_t M, int N, const T* __restrict__ X, int64_t ldx, IndexArr
         if (t == 0) {
             const float ls = logf(s);
             lp[m] = c == ignore ? 0.0f : valid ? (xc - mx) - ls : __builtin_nanf("");
-            if (stats) stats[m] = make_float2(mx, ls);
+            if (stats) stats[m] = make_float2(mx, s);
         }
     }
 }
@@ -123,7 +126,7 @@ k_log_prob_held_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
         const int64_t c = cls.at(m);
         const float2 st = stats[m];
         const float gu = c == ignore ? 0.0f : g[m];
-        const float bad = gu == 0.0f || (c >= 0 && c < N) ? 0.0f : __builtin_nanf("");
+        const float bad = gu == 0.0f || (c >= 0 && c < N) ? 0.0f : __builtin_nanf(""), over = gu / st.y;
         Vec<T, V> r[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) r[k] = load_vec<T, V, TAIL>(X + m * ldx, (k * LANES + t) * V, N);
@@ -133,7 +136,7 @@ k_log_prob_held_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
             float y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float v = -gu * exp_row<LANES>((to_f32(r[k].v[i]) - st.x) - st.y);
+                const float v = -over * exp_grad<T>(to_f32(r[k].v[i]) - st.x);
                 y[i] = gu == 0.0f ? 0.0f : (col + i == c ? gu + v : v) + bad;
             }
             store_vec<T, V, TAIL>(dX + m * lddx, col, N, y);
@@ -235,7 +238,7 @@ k_log_prob_long(int64_t M, int N, int span, const T* __restrict__ X, int64_t ldx
             } else {
                 const float ls = logf(run.s);
                 lp[m] = c >= 0 && c < N ? (to_f32(row[c]) - run.m) - ls : __builtin_nanf("");
-                if (stats) stats[m] = make_float2(run.m, ls);
+                if (stats) stats[m] = make_float2(run.m, run.s);
             }
         }
     }
@@ -257,7 +260,7 @@ k_log_prob_join(int N, int parts, const float2* __restrict__ part, const T* __re
     if (threadIdx.x == 0) {
         const float ls = logf(run.s);
         lp[m] = c >= 0 && c < N ? (to_f32(X[m * ldx + c]) - run.m) - ls : __builtin_nanf("");
-        if (stats) stats[m] = make_float2(run.m, ls);
+        if (stats) stats[m] = make_float2(run.m, run.s);
     }
 }
 
@@ -299,7 +302,7 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
         const int64_t c = cls.at(m);
         const float2 st = stats[m];
         const float gu = c == ignore ? 0.0f : g[m];
-        const float scale = c >= 0 && c < N ? -gu : __builtin_nanf("");
+        const float scale = c >= 0 && c < N ? -gu / st.y : __builtin_nanf("");
         const T* row = X + m * ldx;
         T* out = dX + m * lddx;
         const int head = head_of(out), j = head + blockIdx.y * (LONG_PIECES * STEP) + threadIdx.x * V;
@@ -321,7 +324,7 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
             for (int u = 0; u < LONG_PIECES; ++u) r[u] = load_vec<T, V, true>(row, j + u * STEP, N);
         }
         if (first) {
-            const float p = scale * exp_quick((to_f32(row[threadIdx.x]) - st.x) - st.y);
+            const float p = scale * exp_grad<T>(to_f32(row[threadIdx.x]) - st.x);
             out[threadIdx.x] = from_f32<T>((int)threadIdx.x == c ? p + gu : p);
         }
 #pragma unroll
@@ -329,7 +332,7 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
             const int col = j + u * STEP;
             float y[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = scale * exp_quick((to_f32(r[u].v[i]) - st.x) - st.y);
+            for (int i = 0; i < V; ++i) y[i] = scale * exp_grad<T>(to_f32(r[u].v[i]) - st.x);
             if (c >= col && c < col + V)
 #pragma unroll
                 for (int i = 0; i < V; ++i) y[i] = col + i == c ? y[i] + gu : y[i];

@@ -114,3 +114,22 @@ def test_policy_loss_of_a_far_old_model(dev, d):
     old[70_000] = lp[70_000] - d
     check_terms(lp, old, adv, ref, 0.0, dev)
     check_terms(lp, old, adv, ref, 0.04, dev)
+
+
+@pytest.mark.parametrize("V", [70, 300, 1000, 5001, 40003])
+def test_log_prob_gradient_of_unlikely_classes(dev, V):
+    """Every element of a float32 gradient to its last places, not only those that weigh in the row's sum.  One logit is 0 and
+    the others are multiples of 1/8 from -60 to -20, so that differences from the largest are exact and the row's sum is 1 up to
+    two roundings: what is left are the exponential (4 U), the sum (2 U), g over the sum (1 U), the product (1 U) and the class's
+    own difference (1 U): 10 U with their products."""
+    M = 5
+    x = -(torch.randint(160, 481, (M, V), generator=torch.Generator().manual_seed(V)).float() / 8)
+    x[:, V // 3] = 0.0
+    x[M - 1] += 64.0                                     # about the largest logit, not about 0
+    g = 1.0 + rnd(1, M).abs()
+    c = torch.full((M,), V - 1)
+    a = x.to(dev).requires_grad_(True)
+    (dx,) = torch.autograd.grad(ag.class_log_prob(a, c.to(dev)), [a], g.to(dev))
+    p = x.double().softmax(1)
+    want = g.double()[:, None] * (torch.nn.functional.one_hot(c, V).double() - p)
+    close(dx, want, 10 * U * want.abs(), "gradient")
