@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -21,6 +22,7 @@
 #include <optional>
 #include <sstream>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "graphmaker_hip.h"
@@ -101,20 +103,33 @@ const uint8_t* bytes(const Tensor& t) { return static_cast<const uint8_t*>(at_of
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
 Tensor workspace(int64_t size, const Tensor& like) { return size > 0 ? empty({size}, at::kByte, like) : Tensor(); }
 
-// Whether a call on t is recorded.  A captured call on a leaf whose gradient is accumulated on another stream is refused:
-// torch ties a leaf's accumulation to the stream of the first graph that is alive, a backward pass inside the capture would
-// run it there, and that ends the process.
+// Whether a call on t is recorded.  A captured call over a leaf whose gradient is accumulated on another stream is refused, also
+// where casts, views or other operators lie between: torch ties a leaf's accumulation to the stream of the first graph that is
+// alive, a backward pass inside the capture would run it there, and that ends the process.
+void refuse_foreign(const c10::hip::HIPStream now, const std::shared_ptr<torch::autograd::Node>& accumulator) {
+    if (accumulator && accumulator->stream() && accumulator->stream()->id() != now.id())
+        throw HipError("captured while a graph recorded on another stream over the same leaf tensor is alive: drop that graph first");
+}
 bool records(const Tensor& t) {
     if (!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled()) return false;
-    if (t.is_leaf() && t.is_cuda()) {
-        const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t.device().index());
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess) {
-            (void)hipGetLastError();                     // or the next launch would report it as its own
-        } else if (status != hipStreamCaptureStatusNone) {
-            const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-            if (node && node->stream() && node->stream()->id() != now.id())
-                throw HipError("captured while a graph recorded on another stream over the same leaf tensor is alive: drop that graph first");
+    if (!t.is_cuda()) return true;
+    const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();                         // or the next launch would report it as its own
+    } else if (status != hipStreamCaptureStatusNone) {
+        if (t.is_leaf()) {
+            refuse_foreign(now, torch::autograd::impl::try_get_grad_accumulator(t));
+        } else {
+            std::vector<std::shared_ptr<torch::autograd::Node>> todo{t.grad_fn()};
+            std::unordered_set<torch::autograd::Node*> seen{todo[0].get()};
+            while (!todo.empty()) {
+                const auto node = std::move(todo.back());
+                todo.pop_back();
+                if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) refuse_foreign(now, node);
+                for (const auto& edge : node->next_edges())
+                    if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function);
+            }
         }
     }
     return true;

@@ -133,3 +133,44 @@ def test_log_prob_gradient_of_unlikely_classes(dev, V):
     p = x.double().softmax(1)
     want = g.double()[:, None] * (torch.nn.functional.one_hot(c, V).double() - p)
     close(dx, want, 10 * U * want.abs(), "gradient")
+
+
+def test_capture_looks_behind_casts_and_views(dev):
+    """The leaf whose eager graph is alive may be behind a cast, a view or a layout copy that is recorded inside the capture."""
+    x = rnd(1, 30, 64, dtype=torch.bfloat16).to(dev)
+    w = (1 + 0.1 * rnd(2, 64)).to(dev).requires_grad_(True)
+    emb = rnd(3, 40, 64).to(dev).requires_grad_(True)
+    wide = rnd(4, 128).to(dev).requires_grad_(True)
+    tok, off = torch.arange(30, device=dev), torch.tensor([0, 9, 64], device=dev)
+    alive = [ag.layer_norm(x, w.bfloat16()), ag.token_embedding(emb.bfloat16(), tok), wide * 2]
+    torch.cuda.synchronize()
+    for call in (lambda: ag.layer_norm(x, w.bfloat16()), lambda: ag.token_embedding(emb.bfloat16(), tok),
+                 lambda: ag.token_embedding(emb[:35], tok), lambda: ag.layer_norm(x.float(), wide[::2]),
+                 lambda: ag.class_log_prob((x.float() * w).relu().exp(), tok), lambda: ag.policy_loss(w * 2, w.detach(), w.detach()),
+                 lambda: ag.preference_loss(w * 2, w.detach(), off)):
+        with pytest.raises(RuntimeError, match="same leaf tensor is alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive
+
+    def step():
+        y = ag.token_embedding(emb.bfloat16(), tok)
+        y = ag.layer_norm(y + ag.token_embedding(emb[:35].bfloat16(), tok), w.bfloat16(), (wide[::2] * 1).bfloat16())
+        loss, _ = ag.policy_loss(w * 2, w.detach(), w.detach(), offsets=None)
+        pref, _ = ag.preference_loss(wide[::2] * 2, w.detach(), off)
+        return [y.detach(), *torch.autograd.grad(y.float().square().mean() + loss + pref, [emb, w, wide])]
+
+    g = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out = step()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
