@@ -380,24 +380,21 @@ struct LossArgs {
     int by_sequence, average;
 };
 
-// what a loss keeps for its backward (the S weights, then the slopes) and its workspace, in one allocation
-struct LossBuffer {
+// what a loss keeps for its backward: the S weights, then the slopes
+struct Kept {
     Tensor t;
     float *weight, *slope;
-    void* ws;
-    int64_t need;
 };
-LossBuffer loss_buffer(int64_t M, int64_t S, int64_t slopes, const Tensor& like) {
-    LossBuffer b;
-    b.need = gm_sequence_loss_workspace_bytes(M, S);
-    if (b.need < 0) throw HipError("gm_sequence_loss_workspace_bytes: too many items or sequences");
-    const int64_t head = (4 * (S + slopes) + 15) / 16 * 16;
-    b.t = empty({head + b.need}, at::kByte, like);
-    char* at = out_of<char>(b.t);
-    b.weight = reinterpret_cast<float*>(at);
-    b.slope = slopes ? b.weight + S : nullptr;
-    b.ws = at + head;
-    return b;
+Kept kept_floats(int64_t S, int64_t slopes, const Tensor& like) {
+    Kept k{empty({S + slopes}, at::kFloat, like), nullptr, nullptr};
+    k.weight = out_of<float>(k.t);
+    k.slope = slopes ? k.weight + S : nullptr;
+    return k;
+}
+int64_t loss_workspace(int64_t M, int64_t S) {
+    const int64_t need = gm_sequence_loss_workspace_bytes(M, S);
+    if (need < 0) throw HipError("gm_sequence_loss_workspace_bytes: too many items or sequences");
+    return need;
 }
 
 variable_list policy_fwd(const Tensor& lp, const LossArgs& a, bool grad, Tensor* kept) {
@@ -405,12 +402,14 @@ variable_list policy_fwd(const Tensor& lp, const LossArgs& a, bool grad, Tensor*
     const Tensor l = lp.contiguous();
     const int64_t M = l.numel();
     Tensor loss = empty({}, at::kFloat, lp), stats = empty({4}, at::kFloat, lp);
-    const LossBuffer b = loss_buffer(M, a.S, grad ? M : 0, lp);
+    const int64_t need = loss_workspace(M, a.S);
+    const Tensor ws = workspace(need, lp);
+    const Kept k = kept_floats(a.S, grad ? M : 0, lp);
     call(gm_policy_loss_fwd(M, a.S, floats(l), floats(a.old), floats(a.adv), floats(a.ref), bytes(a.mask), at_of(a.offsets),
                             a.offsets.defined() && is_i64(a.offsets), (float)a.clip_low, (float)a.clip_high, (float)a.kl_coef, a.by_sequence,
-                            out_of<float>(loss), out_of<float>(stats), b.slope, b.weight, b.ws, b.need, stream_of(lp)),
+                            out_of<float>(loss), out_of<float>(stats), k.slope, k.weight, out_of<void>(ws), need, stream_of(lp)),
          "gm_policy_loss_fwd");
-    if (kept) *kept = b.t;
+    if (kept) *kept = k.t;
     return {loss, stats};
 }
 variable_list preference_fwd(const Tensor& lp, const LossArgs& a, Tensor* kept) {
@@ -418,12 +417,14 @@ variable_list preference_fwd(const Tensor& lp, const LossArgs& a, Tensor* kept) 
     const Tensor l = lp.contiguous();
     const int64_t M = l.numel();
     Tensor loss = empty({}, at::kFloat, lp), rewards = empty({a.S}, at::kFloat, lp);
-    const LossBuffer b = loss_buffer(M, a.S, 0, lp);
+    const int64_t need = loss_workspace(M, a.S);
+    const Tensor ws = workspace(need, lp);
+    const Kept k = kept_floats(a.S, 0, lp);
     call(gm_preference_loss_fwd(M, a.S / 2, floats(l), floats(a.ref), bytes(a.mask), at_of(a.offsets), is_i64(a.offsets), (float)a.beta,
-                                (float)a.smoothing, a.average, out_of<float>(loss), out_of<float>(rewards), b.weight, b.ws, b.need,
+                                (float)a.smoothing, a.average, out_of<float>(loss), out_of<float>(rewards), k.weight, out_of<void>(ws), need,
                                 stream_of(lp)),
          "gm_preference_loss_fwd");
-    if (kept) *kept = b.t;
+    if (kept) *kept = k.t;
     return {loss, rewards};
 }
 

@@ -174,3 +174,21 @@ def test_capture_looks_behind_casts_and_views(dev):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+def test_losses_keep_no_workspace_for_the_backward(dev):
+    """Between the passes a loss keeps its weights (4 bytes a sequence) and slopes (4 bytes an item), not what its sums needed (32 bytes a sequence).  The
+    allocator leaves a rest of up to 1 MiB with a block of more than that; two are alive at most."""
+    S, M = 1_000_000, 1_100_000
+    off = (torch.arange(S + 1) * M // S).to(torch.int32).to(dev)
+    lp = rnd(1, M).to(dev).requires_grad_(True)
+    old, adv = rnd(2, M).to(dev), rnd(3, S).to(dev)
+    for call, need in ((lambda: ag.policy_loss(lp, old, adv, offsets=off), 4 * (S + M)),
+                       (lambda: ag.preference_loss(lp, old, off), 4 * S + 4 * S)):        # and the rewards
+        call()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(dev)
+        out = call()
+        assert torch.cuda.memory_allocated(dev) - before <= need + 2 * 2 ** 20 + 8192
+        torch.autograd.grad(out[0], [lp])
+        del out
