@@ -635,7 +635,7 @@ extern "C" int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const voi
     // a wave walks the tiles of its row where the rows alone fill the chip eight times over
     int64_t tiles = (vecs + 63) / 64;
     if (tiles > 1 && C >= 65536 / tiles) tiles = C >= 65536 ? 1 : (65536 + C - 1) / C;
-    GM_REQUIRE(tiles < 65536, "w too large");
+    if (tiles > 65535) tiles = 65535;                   // a launch's second dimension; its workgroups walk on
     const unsigned rows = grid_for((C + 3) / 4, 512);
     if (direct_rows(n))
         return with_dtype(dtype, [&](auto t) -> int {

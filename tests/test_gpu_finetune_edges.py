@@ -192,3 +192,18 @@ def test_losses_keep_no_workspace_for_the_backward(dev):
         assert torch.cuda.memory_allocated(dev) - before <= need + 2 * 2 ** 20 + 8192
         torch.autograd.grad(out[0], [lp])
         del out
+
+
+@pytest.mark.parametrize("n, C", [(2, 1), (65, 1), (65, 33)])
+def test_token_embedding_of_very_wide_rows(dev, n, C):
+    """Rows of more tiles than a launch has in its second dimension: a gradient wherever there is a forward."""
+    w = 65535 * 256 + 300
+    W = (torch.arange(C, device=dev)[:, None] + torch.arange(w, device=dev)[None] % 50).float().requires_grad_(True)
+    tok = torch.arange(n, device=dev) % C
+    y = ag.token_embedding(W, tok)
+    assert torch.equal(y[n - 1], W.detach()[tok[n - 1]])
+    up = (torch.arange(w, device=dev) % 7).float().expand(n, w)                  # small whole numbers: exact sums
+    (dW,) = torch.autograd.grad(y, [W], up)
+    count = torch.bincount(tok, minlength=C).float()
+    for c in range(C):
+        assert torch.equal(dW[c], up[0] * count[c])
