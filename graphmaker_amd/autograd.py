@@ -475,12 +475,13 @@ def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
     """scale * weight[tokens], shape tokens.shape + (w,), in weight's type (float32, bfloat16, float16).  tokens: int32 or int64
     of any shape.  The gradient sums each row's tokens in ascending position (no atomics: the same bits on every run) and
     leaves row padding_idx zero, as nn.Embedding does.  Tokens are not read on the host: one outside [0, C) gives a row of
-    NaN and adds to no gradient; ops.check_index_range(tokens, C, "tokens") is the check that raises."""
+    NaN and adds to no gradient; ops.check_index_range(tokens, C, "tokens") is the check that raises.  C and the number of
+    tokens are below 2^31, w below 2^30."""
     return L.tape().token_embedding(weight, tokens, scale, padding_idx)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5):
-    """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension, of any width, in x's type (float32, bfloat16,
+    """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension, of any width below 2^26, in x's type (float32, bfloat16,
     float16).  gamma and beta (N,): x's type or float32, both the same; None: 1 and 0.  Statistics are float32 about the mean,
     the variance that of the differences from it."""
     return L.tape().layer_norm(x, gamma, beta, eps)
@@ -490,7 +491,8 @@ def class_log_prob(logits, classes, ignore_index=-100):
     """log softmax(logits)[classes] over the last dimension: float32 of shape classes.shape = logits.shape[:-1]; logits float32,
     bfloat16 or float16, classes int32 or int64.  A row whose class is ignore_index has log-probability 0 and a zero gradient,
     whatever its logits hold; any other class outside [0, V) gives NaN in both (classes are not read on the host).  A row
-    whose upstream gradient is exactly 0 gets a zero gradient too."""
+    whose upstream gradient is exactly 0 gets a zero gradient too.  V is below 2^27.  Of a denoiser's logits this is the
+    log-probability of the clean class; sample() draws from BaseModel.posterior, whose logarithm is then what to pass."""
     return L.tape().class_log_prob(logits, classes, ignore_index)
 
 

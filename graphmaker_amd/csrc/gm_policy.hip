@@ -1,8 +1,8 @@
 // gm_policy.hip -- losses over the log-probabilities of a batch of ragged sequences (answers, or the draws of generated
-// graphs): the clipped policy loss with a KL term, and the preference loss of pairs.  Item i has log-probability l under
-// the trained model, `old` under the one that drew it and `ref` under a fixed reference; a sequence is a run of items
-// [offsets[s], offsets[s+1]).  An item is live if it is inside a sequence and its mask byte is set; the values of the
-// others are never used.
+// graphs, each under the distribution it was drawn from): the clipped policy loss with a KL term, and the preference loss of
+// pairs.  Item i has log-probability l under the trained model, `old` under the one that drew it and `ref` under a fixed
+// reference; a sequence is a run of items [offsets[s], offsets[s+1]).  An item is live if it is inside a sequence and its mask
+// byte is set; the values of the others are never used.
 //
 //   policy       r = exp(l - old),  t = -min(r A, clip(r, 1 - low, 1 + high) A) + k (exp(q) - q - 1),  q = ref - l
 //                loss = mean of t over the live items, or mean over sequences of each one's mean

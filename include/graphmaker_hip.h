@@ -350,12 +350,12 @@ enum { GM_DTYPE_F32 = 0, GM_DTYPE_BF16 = 1, GM_DTYPE_F16 = 2 };
 int gm_token_embedding_fwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, const void* weight, int64_t ldw,
                            int dtype, float scale, void* out, int64_t ldo, gm_stream_t stream);
 /* dW (C, w) = scale * (sum of the rows G[i] with tokens[i] == c, ascending i); zero where there is none, for row padding_idx
- * (negative: no such row) and from tokens outside [0, C).  The tokens are sorted in the workspace; n, C < 2^31. */
+ * (negative: no such row) and from tokens outside [0, C).  The tokens are sorted in the workspace; n, C < 2^31, w < 2^30. */
 int64_t gm_token_embedding_bwd_workspace_bytes(int64_t n, int64_t C, int64_t w);
 int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const void* tokens, int tokens_i64, int64_t padding_idx, const void* G,
                            int64_t ldg, int dtype, float scale, void* dW, int64_t ldw, void* workspace, int64_t workspace_bytes,
                            gm_stream_t stream);
-/* y = (x - mean) * rstd * gamma + beta over rows of any width N; gamma / beta may be NULL and have the rows' type or float32
+/* y = (x - mean) * rstd * gamma + beta over rows of any width N < 2^26; gamma / beta may be NULL and have the rows' type or float32
  * (weight_dtype); mean, rstd (M floats each, both or neither): what the backward needs */
 int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ldx, int dtype, const void* gamma, const void* beta,
                       int weight_dtype, float eps, void* Y, int64_t ldy, float* mean, float* rstd, gm_stream_t stream);

@@ -207,3 +207,34 @@ def test_token_embedding_of_very_wide_rows(dev, n, C):
     count = torch.bincount(tok, minlength=C).float()
     for c in range(C):
         assert torch.equal(dW[c], up[0] * count[c])
+
+
+def test_log_prob_of_the_samplers_own_draws(dev):
+    """class_log_prob of the log of BaseModel.posterior is the log-probability of an attribute as the sampler draws it: its own
+    two posterior values (float32 products and sums of positive numbers, a few roundings each) normalised."""
+    import numpy as np
+    import graphmaker_amd as gm
+    from graphmaker_amd import diffusion, ops
+    n, F = 70, 9
+    g = torch.Generator().manual_seed(3)
+    marginal = torch.rand(F, generator=g) * 0.8 + 0.1
+    marginal = torch.stack([1 - marginal, marginal], 1)
+    trans = diffusion.MarginalTransition(dev, marginal.to(dev), torch.tensor([0.9, 0.1], device=dev), 2)
+    alpha, abar_s, abar_t = np.float32(0.8), np.float32(0.5), np.float32(0.4)
+    tab = torch.from_numpy(trans.table_X(alpha, abar_s, abar_t)).to(dev)
+    logits = (2 * torch.randn(n, F, 2, generator=g)).to(dev).requires_grad_(True)
+    x_t = torch.randint(0, 2, (n, F), generator=g, dtype=torch.uint8).to(dev)
+    drawn, _, values = ops.attr_posterior_sample(logits.detach().reshape(n, 2 * F), x_t, tab, seed=4, step=1, want_debug=True)
+    Z = torch.nn.functional.one_hot(x_t.t().long(), 2).float()                   # (F, n, 2)
+    Q, Qs, Qt = (trans.get_Q_bar_X(float(a)) for a in (alpha, abar_s, abar_t))
+    post = gm.ModelSync.posterior(None, Z, Q, Qs, Qt, logits.softmax(-1).transpose(0, 1)).transpose(0, 1)
+    lp = ag.class_log_prob(post.log(), drawn.long())
+    p = values.double().cpu()
+    p = (p / p.sum(-1, keepdim=True)).gather(-1, drawn.long().cpu()[..., None])[..., 0]
+    # float32: softmax, two tables, two products, a sum, the logarithm's argument: 32 U relative of a probability, and of the
+    # logarithms as much of their size
+    close(lp, p.log(), 32 * U * (1 + p.log().abs()), "log-probability of a draw")
+    plain = ag.class_log_prob(logits, drawn.long())
+    assert (plain.detach() - lp.detach()).abs().max() > 0.1                      # softmax(logits) is another distribution
+    (dl,) = torch.autograd.grad(lp.sum(), [logits])
+    assert dl.isfinite().all() and dl.any()
