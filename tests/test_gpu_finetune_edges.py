@@ -238,3 +238,71 @@ def test_log_prob_of_the_samplers_own_draws(dev):
     assert (plain.detach() - lp.detach()).abs().max() > 0.1                      # softmax(logits) is another distribution
     (dl,) = torch.autograd.grad(lp.sum(), [logits])
     assert dl.isfinite().all() and dl.any()
+
+
+@pytest.mark.parametrize("M, N", [(1100, 16388), (600, 32772)])
+def test_layer_norm_long_rows_in_turn(dev, M, N):
+    """Rows that no workgroup holds, more of them than workgroups: the column sums go on from row to row."""
+    check_norm((rnd(N, M, N) * (1 + torch.arange(M)[:, None] % 3) + 0.7), 1 + 0.3 * rnd(1, N), rnd(2, N), rnd(3, M, N), dev)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_have_the_same_bits_at_any_alignment(dev, dt):
+    t = DT[dt]
+    for N in (3, 40, 512, 1000, 5001):
+        M = 50
+        base, gb = rnd(1, M, N + 9, dtype=t).to(dev), rnd(2, M, N + 9, dtype=t).to(dev)
+        ga, be = (1 + 0.2 * rnd(3, N)).to(t).to(dev).requires_grad_(True), rnd(4, N, dtype=t).to(dev).requires_grad_(True)
+        c = torch.randint(0, N, (M,), generator=torch.Generator().manual_seed(3)).to(dev)
+        g = rnd(4, M).to(dev)
+        for at in (0, 1, 3, 8, 9):
+            got = []
+            for make in (lambda v: v, lambda v: v.contiguous()):
+                x = make(base[:, at:at + N]).detach().requires_grad_(True)
+                y = ag.layer_norm(x, ga, be)
+                out = [y, *torch.autograd.grad(y, [x, ga, be], make(gb[:, at:at + N]))]
+                lp = ag.class_log_prob(x, c)
+                got.append(out + [lp, *torch.autograd.grad(lp, [x], g)])
+            for k, (a, b) in enumerate(zip(*got)):
+                assert torch.equal(a, b), (N, at, k)
+
+
+def test_fine_tuning_gradients_against_differences_along_themselves(dev):
+    """Every parameter's gradient of the whole chain, along its own direction (where the slope is its norm) and along a random
+    one at right angles to it (where the slope is 0), against central differences of steps h and h/2 joined to fourth order.
+    Their difference is 3/4 of what truncation leaves at h, and a fourth of it is allowed for what the joining leaves; the float32
+    losses of about 1 are given 64 U of rounding each.  The tolerance has to be below a thousandth of the gradient's norm, so that
+    the check has force.  The clip is opened: no ratio may cross a
+    border of its range."""
+    from test_gpu_finetune import fine_tuning_setup
+    p, batch = fine_tuning_setup(dev, torch.float32)
+    mask = batch["classes"] != -100
+
+    def f(q):
+        h = ag.layer_norm(ag.token_embedding(q["emb"], batch["tokens"], scale=4.0, padding_idx=0), q["gamma"], q["beta"])
+        lp = ag.class_log_prob(ag.linear(h, q["W"], q["b"]), batch["classes"])
+        a, _ = ag.policy_loss(lp, batch["old"], batch["adv"], offsets=batch["offsets"], mask=mask, ref_log_prob=batch["ref"], clip_low=1.0,
+                              clip_high=100.0, kl_coef=0.05, reduction="sequence")
+        b, _ = ag.preference_loss(lp, batch["ref"], batch["offsets"], mask=mask, beta=0.3)
+        return a + b
+
+    grads = dict(zip(p, torch.autograd.grad(f(p), list(p.values()))))
+    for name, t in p.items():
+        g = grads[name].double()
+        along = g / g.norm()
+        across = torch.randn(t.shape, generator=torch.Generator().manual_seed(5), dtype=torch.float64).to(dev)
+        if name == "emb":
+            across[0] = 0.0                              # the padding row: used, and without a gradient by definition
+        across -= (across * along).sum() * along
+        across /= across.norm()
+        for v in (along, across):
+            def quotient(step):
+                with torch.no_grad():
+                    up, down = (float(f({**p, name: (t.double() + s * v).float()}).double()) for s in (step, -step))
+                return (up - down) / (2 * step)
+            h = 1e-2
+            wide, near = quotient(h), quotient(h / 2)
+            got, want = (4 * near - wide) / 3, float((g * v).sum())
+            # (4 (2 E) / h + (2 E) / (2 h)) / 3 with E = 64 U
+            tol = abs(wide - near) / 4 + 3 * 64 * U / h
+            assert tol < 1e-3 * float(g.norm()) and abs(got - want) <= tol, (name, got, want, tol)
