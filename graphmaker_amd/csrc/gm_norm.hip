@@ -354,7 +354,7 @@ static inline RowShape row_shape(int64_t N, int vec, int most) {
     if (v <= 16) return {16, 1};
     if (v <= 32) return {32, 1};
     for (const int tpr : {64, 256, 512, 1024})
-        if (v <= 4 * tpr && !(tpr == 1024 && v > most * 1024)) return {tpr, (int)((v + tpr - 1) / tpr)};
+        if (v <= 4 * tpr) return {tpr, (int)((v + tpr - 1) / tpr)};
     return v <= 8 * 1024 && most >= 8 ? RowShape{1024, 8} : RowShape{0, 0};
 }
 // workgroups of the forward: what the CUs hold at once

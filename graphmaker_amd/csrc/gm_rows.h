@@ -84,11 +84,6 @@ template <class T> __device__ __forceinline__ T wave_add(T v) {
     for (int off = 32; off >= 1; off >>= 1) v = v + __shfl_xor(v, off);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off));
-    return v;
-}
 
 // exp(x) within about two units in the last place: 2^(x log2 e), with the product's rounding error (|x| 2^-24 relative, were it
 // left) put back as a factor.  exp(-inf) = 0, overflow gives infinity, NaN stays NaN.
