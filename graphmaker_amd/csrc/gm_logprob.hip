@@ -175,7 +175,7 @@ struct Running {
 };
 
 // part[row][blockIdx.y] of columns [blockIdx.y * span, + span); with one part a row (gridDim.y = 1) lp and stats at once.
-// 4095 x 50,021 bf16: 97 us, 4.2 TB/s (odd rows straddle lines: 4096 x 50,016 take 84 us)
+// 4095 x 50,021 bf16: 98 us, 4.2 TB/s (odd rows straddle lines: 4096 x 50,016 take 84 us)
 template <class T>
 __global__ void __launch_bounds__(256)
 k_log_prob_long(int64_t M, int N, int span, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore, float* __restrict__ lp,
@@ -292,7 +292,7 @@ template <bool PAST, class T, int V> __device__ __forceinline__ Vec<T, V> get_ve
 }
 
 // columns head + [blockIdx.y * span, + span) of a row, span = LONG_PIECES steps, the head with the first (4095 x 50,021 bf16:
-// 138 us, 5.9 TB/s)
+// 140 us, 5.9 TB/s)
 template <class T, bool PAST>
 __global__ void __launch_bounds__(256)
 k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __restrict__ X, int64_t ldx, IndexArray cls, int64_t ignore,

@@ -72,7 +72,7 @@ template <int TPR> __device__ __forceinline__ void row_add(float& a, float& b, f
 
 // A row stays in registers: TPR threads hold K x 16 bytes each, so HBM sees every element once.  A workgroup walks several
 // rows with gamma and beta in registers too, and loads the next row before it reduces the one it has: what a row waits for
-// is HBM alone (8191 x 8192 bf16: 53 us, the card's copy rate; reading gamma and beta and waiting for the row took 92).  Rows of
+// is HBM alone (8191 x 8192 bf16: 55 us, the card's copy rate; reading gamma and beta and waiting for the row took 92).  Rows of
 // 1024 threads are LEAN, without either: half the registers, so that a second workgroup fits a CU.
 template <class T, int V, bool TAIL, int K, int TPR>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
@@ -142,7 +142,7 @@ k_layer_norm_fwd(int64_t M, int N, const T* __restrict__ X, int64_t ldx, Weights
 }
 
 // dx of a workgroup's rows, and the column sums of g xh and g over them, held in registers until the last row:
-// part[workgroup][0][c], part[workgroup][1][c].  HBM-bound: 8191 x 8192 bf16 97 us, 4.2 TB/s of which 32 MB are the column sums.
+// part[workgroup][0][c], part[workgroup][1][c].  HBM-bound: 8191 x 8192 bf16 100 us, 4.0 TB/s and the 32 MB of column sums besides.
 template <class T, int V, bool TAIL, int K, int TPR>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 k_layer_norm_bwd(int64_t M, int N, const T* __restrict__ G, int64_t ldg, const T* __restrict__ X, int64_t ldx,

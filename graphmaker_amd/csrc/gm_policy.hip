@@ -115,7 +115,8 @@ struct LessOne {
 
 // What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.  An item's terms are
 // float32: they carry a few 2^-24, and |x| 2^-24 from the rounded difference x of two float32 log-probabilities, which carry as much
-// themselves.  (Of 10,547,784 items these take 41.5 us, float64 terms of float32 exponentials 47 and of float64 ones 54.)
+// themselves.  (Of 10,547,784 items these take 41.5 us, 2 to 3 more where every wave has an item past |q| = 1; float64 terms of
+// float32 exponentials take 47 and of float64 ones 54.)
 template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
     static constexpr int Q = 4;                          // sums: surrogate, KL, clipped items, live items
     struct Acc { double surrogate = 0.0, kl = 0.0; int cut = 0, live = 0; };
@@ -178,7 +179,7 @@ template <bool MASK> struct PreferenceTerm {
 };
 
 // pieces of the sequences: `whole`[s] of one inside this chunk; `piece`[2k] of one that began before chunk k,
-// `piece`[2k+1] of one that begins in it and goes on.  HBM-bound: 10,547,784 items with KL and slopes 40 us, 4.2 TB/s
+// `piece`[2k+1] of one that begins in it and goes on.  HBM-bound: 10,547,784 items with KL and slopes 41.5 us, 4.1 TB/s
 template <class F>
 __global__ void __launch_bounds__(256)
 k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whole, Sums<F::Q>* __restrict__ piece) {
@@ -413,7 +414,8 @@ __global__ void __launch_bounds__(1024) k_preference_total(int parts, int64_t P,
     if (threadIdx.x == 0) loss[0] = (float)(tot[0] / (double)P);
 }
 
-// dl[i] = g weight[s] slope[i] for the live items of sequence s, 0 for every other item (10,547,784 items 17 us, 4.9 TB/s)
+// dl[i] = g weight[s] slope[i] for the live items of sequence s, 0 for every other item (10,547,784 items 17 us, 4.9 TB/s).  Slope
+// and weight are float32, as the gradient is: the first halves what a pass reads, and the three roundings are half a step each.
 template <bool SLOPE, bool MASK>
 __global__ void __launch_bounds__(256)
 k_sequence_spread(Sequences q, int64_t chunk, const float* __restrict__ slope, const uint8_t* __restrict__ mask,

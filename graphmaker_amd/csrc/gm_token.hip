@@ -12,7 +12,7 @@ namespace gm {
 
 // A row is `tpr` threads wide (a power of two up to the workgroup), V elements a thread and step; a workgroup takes
 // FWD_ROWS rows per thread so that their loads are in flight together (the address of each waits for its token).  HBM-bound: 130,941
-// rows of 1024 bf16 71 us, 5.5 TB/s of the rows written and the different ones read.
+// rows of 1024 bf16 71 us, 4.4 TB/s of the rows written and the 22,000 different ones read.
 constexpr int FWD_ROWS = 4;
 template <class T, int V, bool TAIL>
 __global__ void __launch_bounds__(256)
@@ -184,7 +184,8 @@ k_radix_scatter(int64_t n, int64_t C, int64_t padding, IndexArray tok, const uin
     }
 }
 
-// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch (2048 tokens 10 us, latency).  Each
+// The same sort of up to SMALL_KEYS keys by one workgroup, all digits in one launch (2048 tokens 10 us, latency; the whole
+// gradient of 8192 tokens, 1000 x 256 bf16, takes 25 us and of 8193, sorted by several, 30).  Each
 // wave holds `rounds` x 64 keys that are consecutive in the current order in registers; the keys change places through LDS.
 constexpr int SMALL_WAVES = 16, SMALL_ROUNDS = 8, SMALL_KEYS = SMALL_WAVES * SMALL_ROUNDS * 64, SMALL_BITS = 8;
 template <int BITS>
@@ -359,7 +360,7 @@ __device__ __forceinline__ void token_piece(int64_t n, int64_t C, int w, int lan
 
 // The row that begins in chunk blockIdx.x and goes on behind it, if it is one of more than `cut` tokens.  `wide` threads (a
 // power of two) take four columns each, 1024 / wide lanes of them every so-manieth piece; the lanes are added as a tree.  The
-// hottest row's 165 pieces bound the launch: 16 us, not less with more columns or loads a launch.
+// hottest row's 115 pieces (130,941 tokens of 50,021) bound the launch: 16 us, not less with more columns or loads a launch.
 template <class T>
 __global__ void __launch_bounds__(1024)
 k_token_join(int64_t n, int64_t C, int w, int64_t ldp, int wide, uint32_t cut, const uint32_t* __restrict__ keys,
@@ -472,8 +473,11 @@ k_token_direct(int n, int64_t C, int w, int lanes, int64_t padding, IndexArray t
 
 // ---- tables of at most FEW rows (class labels): no sort.  A wave walks `per_wave` tokens and keeps a sum of every row for its
 // 64 columns in LDS; its token is the same in all lanes, so each lane adds to its own word.  The four waves' sums are added
-// in order and go to part[workgroup][row][column], which k_token_few_join adds in order.  13,752 tokens of 10 labels x 64
-// float32: two launches and 11 us, where sort, borders, sums and join are five launches and 26 us.
+// in order and go to part[workgroup][row][column], which k_token_few_join adds in order.  Its time grows with the rows, which
+// every wave adds up at its end; us against the sorted form's at 10, 32 and 48 rows:
+//   13,752 x 64 float32     10 : 24    19 : 24    26 : 24         1,000 x 64 float32      9 : 16    18 : 13    25 : 13
+//   130,000 x 512 float32   71 : 85    65 : 81    80 : 80         130,000 x 512 bf16     62 : 57    58 : 52    75 : 51
+//   1,000,000 x 64 float32  76 : 97    64 : 98    81 : 99         1,000,000 x 64 bf16    63 : 66    59 : 67    75 : 68
 constexpr int FEW = 32;
 template <class T>
 __global__ void __launch_bounds__(256)
@@ -570,6 +574,9 @@ static inline TokenLayout token_layout(int64_t n, int64_t C, int64_t w) {
     l.digit = (bits + l.passes - 1) / l.passes;
     if (l.digit < 5) l.digit = 5;                      // with_digit
     l.nblk = (n + sort_keys(n) - 1) / sort_keys(n);
+    // Tokens from which a row is summed in pieces.  32, 64, 128 and 256 take 157, 143, 135 and 142 us of 130,941 tokens of 50,021 x
+    // 1024 bf16 (few rows with thousands each), and 89, 95, 111 and 142 us of 16,000 such of float32: longer pieces are fewer to
+    // join, and each is one wave that the others wait for.
     l.cut = 64;
     while ((int64_t)l.cut * 4096 < n) l.cut *= 2;      // at most 4096 pieces of one row
     int64_t at = 0;

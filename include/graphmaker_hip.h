@@ -359,7 +359,8 @@ int gm_token_embedding_bwd(int64_t n, int64_t C, int64_t w, const void* tokens, 
  * (weight_dtype); mean, rstd (M floats each, both or neither): what the backward needs */
 int gm_layer_norm_fwd(int64_t M, int64_t N, const void* X, int64_t ldx, int dtype, const void* gamma, const void* beta,
                       int weight_dtype, float eps, void* Y, int64_t ldy, float* mean, float* rstd, gm_stream_t stream);
-/* gradients of the above for dY = G; dX, dgamma, dbeta may each be NULL (workspace needed only for dgamma / dbeta) */
+/* gradients of the above for dY = G; dX, dgamma, dbeta may each be NULL.  dgamma / dbeta need the
+ * workspace: 8 N bytes for each of min(M, 512) workgroups, which sum their rows' share each. */
 int64_t gm_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N);
 int gm_layer_norm_bwd(int64_t M, int64_t N, const void* G, int64_t ldg, const void* X, int64_t ldx, int dtype, const float* mean,
                       const float* rstd, const void* gamma, int weight_dtype, void* dX, int64_t lddx, void* dgamma, void* dbeta,
