@@ -144,6 +144,20 @@ variable_list once(variable_list grads) {
     return (*error)(std::move(grads));
 }
 
+// A saved tensor as the backward pass may use it.  Hooks on saved tensors (torch.autograd.graph) can hand it back with other
+// strides, or as something else altogether, so nothing is taken over from the forward but what it has to be.
+void saved_is(const Tensor& t, const char* what, at::ScalarType type, int64_t numel, const Tensor& like) {
+    if (t.scalar_type() != type || t.numel() != numel || t.device() != like.device())
+        throw HipError(say("the saved ", what, " came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", saved were ", numel, " of ", type,
+                           " on ", like.device()));
+}
+Tensor saved_packed(const Tensor& t, const char* what, at::ScalarType type, int64_t numel, const Tensor& like) {
+    if (!t.defined()) return t;
+    saved_is(t, what, type, numel, like);
+    return t.contiguous();
+}
+int64_t type_code(const Tensor& t) { return t.defined() ? (int64_t)t.scalar_type() : (int64_t)at::kByte; }
+
 // ------------------------------------------------------------------ token_embedding
 struct EmbeddingArgs {
     double scale;
@@ -167,15 +181,16 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
     static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, const EmbeddingArgs& a) {
         ctx->save_for_backward({tokens});
         ctx->saved_data["C"] = weight.size(0);
+        ctx->saved_data["type"] = type_code(tokens);
         ctx->saved_data["scale"] = a.scale;
         ctx->saved_data["padding"] = a.padding;
         return embedding_fwd(weight, tokens, a);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const Tensor& g = grads[0];
-        const Tensor tokens = ctx->get_saved_variables()[0];
         const c10::DeviceGuard guard(g.device());
-        const int64_t n = tokens.numel(), C = ctx->saved_data["C"].toInt(), w = g.size(-1);
+        const int64_t C = ctx->saved_data["C"].toInt(), w = g.size(-1), n = g.numel() / w;
+        const Tensor tokens = saved_packed(ctx->get_saved_variables()[0], "tokens", (at::ScalarType)ctx->saved_data["type"].toInt(), n, g);
         const Rows r = rows_of(g, w);
         Tensor dW = empty({C, w}, g.scalar_type(), g);
         const int64_t need = gm_token_embedding_bwd_workspace_bytes(n, C, w);
@@ -231,16 +246,19 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Rows r = rows_of(x, N);
         const Tensor stats = empty({2 * (x.numel() / N)}, at::kFloat, x);
         ctx->save_for_backward({r.t, stats, gamma});
-        ctx->saved_data["ld"] = r.ld;
+        ctx->saved_data["gamma"] = type_code(gamma);
         ctx->saved_data["beta"] = beta.defined() ? (int64_t)beta.scalar_type() : -1;
         return norm_fwd(x, r, gamma, beta, eps, stats);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const Tensor& g = grads[0];
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &stats = saved[1], &gamma = saved[2];
         const c10::DeviceGuard guard(g.device());
-        const int64_t N = g.size(-1), M = g.numel() / N, ld = ctx->saved_data["ld"].toInt();
+        const int64_t N = g.size(-1), M = g.numel() / N;
+        saved_is(saved[0], "x", g.scalar_type(), M * N, g);
+        const Rows x = rows_of(saved[0], N);
+        const Tensor stats = saved_packed(saved[1], "statistics", at::kFloat, 2 * M, g);
+        const Tensor gamma = saved_packed(saved[2], "gamma", (at::ScalarType)ctx->saved_data["gamma"].toInt(), N, g);
         const int64_t beta_type = ctx->saved_data["beta"].toInt();
         const bool has_gamma = gamma.defined(), has_beta = beta_type >= 0;      // edges are numbered over the present inputs
         const Rows r = rows_of(g, N);
@@ -250,7 +268,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const int64_t need = dgamma.defined() || dbeta.defined() ? gm_layer_norm_bwd_workspace_bytes(M, N) : 0;
         const Tensor ws = workspace(need, g);
         const Tensor& wt = gamma.defined() ? gamma : dbeta;
-        call(gm_layer_norm_bwd(M, N, at_of(r.t), r.ld, at_of(x), ld, row_dtype(g, "gradient"), floats(stats), M ? floats(stats) + M : nullptr,
+        call(gm_layer_norm_bwd(M, N, at_of(r.t), r.ld, at_of(x.t), x.ld, row_dtype(g, "gradient"), floats(stats), M ? floats(stats) + M : nullptr,
                                at_of(gamma), row_dtype(wt.defined() ? wt : g, "gamma"), out_of<void>(dx), N, out_of<void>(dgamma),
                                out_of<void>(dbeta), out_of<void>(ws), need, stream_of(g)),
              "gm_layer_norm_bwd");
@@ -308,7 +326,8 @@ struct ClassLogProb : torch::autograd::Function<ClassLogProb> {
         const int64_t need = gm_class_log_prob_stats_floats(classes.numel(), logits.size(-1), row_dtype(logits, "logits"));
         const Tensor stats = need > 0 ? empty({need}, at::kFloat, logits) : Tensor();
         ctx->save_for_backward({r.t, classes, stats});
-        ctx->saved_data["ld"] = r.ld;
+        ctx->saved_data["type"] = type_code(logits);
+        ctx->saved_data["classes"] = type_code(classes);
         ctx->saved_data["shape"] = logits.sizes().vec();
         ctx->saved_data["ignore"] = ignore_index;
         return log_prob_fwd(logits, r, classes, ignore_index, stats);
@@ -316,12 +335,17 @@ struct ClassLogProb : torch::autograd::Function<ClassLogProb> {
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const Tensor g = grads[0].contiguous();
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &classes = saved[1], &stats = saved[2];
         const c10::DeviceGuard guard(g.device());
         const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-        const int64_t V = shape.back();
-        Tensor dx = empty(shape, x.scalar_type(), g);
-        call(gm_class_log_prob_bwd(classes.numel(), V, floats(g), at_of(x), ctx->saved_data["ld"].toInt(), row_dtype(x, "logits"), at_of(classes),
+        const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const int64_t V = shape.back(), M = g.numel();
+        Tensor dx = empty(shape, type, g);
+        const int code = row_dtype(dx, "logits");
+        saved_is(saved[0], "logits", type, M * V, g);
+        const Rows x = rows_of(saved[0], V);
+        const Tensor classes = saved_packed(saved[1], "classes", (at::ScalarType)ctx->saved_data["classes"].toInt(), M, g);
+        const Tensor stats = saved_packed(saved[2], "statistics", at::kFloat, gm_class_log_prob_stats_floats(M, V, code), g);
+        call(gm_class_log_prob_bwd(M, V, floats(g), at_of(x.t), x.ld, code, at_of(classes),
                                    is_i64(classes), ctx->saved_data["ignore"].toInt(), floats(stats), out_of<void>(dx), V, stream_of(g)),
              "gm_class_log_prob_bwd");
         return once({dx, Tensor(), Tensor()});
@@ -435,6 +459,8 @@ template <bool POLICY> struct SequenceLoss : torch::autograd::Function<SequenceL
         ctx->save_for_backward({kept, a.mask, a.offsets});
         ctx->saved_data["S"] = a.S;
         ctx->saved_data["shape"] = lp.sizes().vec();
+        ctx->saved_data["mask"] = type_code(a.mask);
+        ctx->saved_data["offsets"] = type_code(a.offsets);
         ctx->mark_non_differentiable({out[1]});
         ctx->set_materialize_grads(false);
         return out;
@@ -443,12 +469,15 @@ template <bool POLICY> struct SequenceLoss : torch::autograd::Function<SequenceL
         if (!grads[0].defined()) return {Tensor(), Tensor()};
         const Tensor& g = grads[0];
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &kept = saved[0], &mask = saved[1], &offsets = saved[2];
         const c10::DeviceGuard guard(g.device());
         const int64_t S = ctx->saved_data["S"].toInt();
         Tensor dl = empty(ctx->saved_data["shape"].toIntVector(), at::kFloat, g);
+        const int64_t M = dl.numel();
+        const Tensor kept = saved_packed(saved[0], "weights", at::kFloat, POLICY ? S + M : S, g);
+        const Tensor mask = saved_packed(saved[1], "mask", (at::ScalarType)ctx->saved_data["mask"].toInt(), M, g);
+        const Tensor offsets = saved_packed(saved[2], "offsets", (at::ScalarType)ctx->saved_data["offsets"].toInt(), S + 1, g);
         const float* weight = floats(kept);
-        call(gm_sequence_loss_bwd(dl.numel(), S, POLICY ? weight + S : nullptr, bytes(mask), at_of(offsets), offsets.defined() && is_i64(offsets),
+        call(gm_sequence_loss_bwd(M, S, POLICY ? weight + S : nullptr, bytes(mask), at_of(offsets), offsets.defined() && is_i64(offsets),
                                   weight, floats(g), out_of<float>(dl), stream_of(g)),
              "gm_sequence_loss_bwd");
         return once({dl, Tensor()});

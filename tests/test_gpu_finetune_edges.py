@@ -306,3 +306,52 @@ def test_fine_tuning_gradients_against_differences_along_themselves(dev):
             # (4 (2 E) / h + (2 E) / (2 h)) / 3 with E = 64 U
             tol = abs(wide - near) / 4 + 3 * 64 * U / h
             assert tol < 1e-3 * float(g.norm()) and abs(got - want) <= tol, (name, got, want, tol)
+
+
+def hooked_step(dev, dtype, strided):
+    """Every operator's gradient, of inputs that are rows of wider tensors or packed."""
+    def put(seed, *shape, dtype=torch.float32):
+        t = rnd(seed, *shape[:-1], 2 * shape[-1] + 3, dtype=dtype).to(dev)[..., 3:3 + shape[-1]]
+        return (t if strided else t.contiguous()).detach().requires_grad_(True)
+    n, C, w = 90, 30, 72
+    x, emb, logits, narrow, lp = put(1, n, w, dtype=dtype), put(2, C, w, dtype=dtype), put(3, n, 5003, dtype=dtype), put(4, n, 2), put(5, 12, 9)
+    gamma, beta = put(6, w), put(7, w)
+    tok, cls = (torch.arange(n, device=dev) * 7 % C).int(), torch.arange(n, device=dev) % 2
+    mask, off = rnd(8, 12, 9).to(dev) > 0, torch.tensor([0, 30, 100], device=dev, dtype=torch.int32)
+    old, adv = lp.detach() + 0.1, rnd(9, 2).to(dev)
+    out = ag.layer_norm(x, gamma, beta).float().square().sum() + ag.token_embedding(emb, tok).float().square().sum()
+    out = out + ag.class_log_prob(logits, cls).square().sum() + ag.class_log_prob(narrow, cls).sum()
+    out = out + ag.policy_loss(lp, old, adv, offsets=off, mask=mask)[0] + ag.preference_loss(lp, old, off, mask=mask)[0]
+    return out, [x, gamma, beta, emb, logits, narrow, lp]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("strided", [False, True])
+def test_saved_tensors_may_be_moved(dev, dt, strided):
+    """Hooks on saved tensors hand them back with strides of their own: kept in host memory, or cloned."""
+    out, leaves = hooked_step(dev, DT[dt], strided)
+    want = torch.autograd.grad(out, leaves)
+    packed = torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t)
+    other = torch.autograd.graph.saved_tensors_hooks(lambda t: t.expand(2, *t.shape).movedim(0, -1).contiguous()[..., 0], lambda t: t)
+    for hooks in (packed, other, torch.autograd.graph.save_on_cpu(pin_memory=False), torch.autograd.graph.save_on_cpu(pin_memory=True)):
+        with hooks:
+            out, leaves = hooked_step(dev, DT[dt], strided)
+        for a, b in zip(torch.autograd.grad(out, leaves), want):
+            assert torch.equal(a, b)
+    y = torch.utils.checkpoint.checkpoint(lambda: hooked_step(dev, DT[dt], strided)[0], use_reentrant=False)
+    assert torch.isfinite(y)
+
+
+def test_saved_tensors_of_another_kind_are_refused(dev):
+    """What comes back with another type, size or place would be read as what it is not."""
+    x, w = rnd(1, 40, 64).to(dev).requires_grad_(True), rnd(2, 64).to(dev).requires_grad_(True)
+    tok, off = torch.arange(40, device=dev), torch.tensor([0, 9, 40], device=dev)
+    flat = rnd(3, 40).to(dev).requires_grad_(True)
+    ref = rnd(4, 40).to(dev)
+    for change in (lambda t: t.bfloat16() if t.is_floating_point() else t.int(), lambda t: t[:-1], lambda t: t.cpu()):
+        for call, leaf in ((lambda: ag.layer_norm(x, w), x), (lambda: ag.token_embedding(x, tok), x), (lambda: ag.class_log_prob(x, tok), x),
+                           (lambda: ag.policy_loss(flat, ref, ref)[0], flat), (lambda: ag.preference_loss(flat, ref, off)[0], flat)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                y = call()
+            with pytest.raises(RuntimeError, match="came back as"):
+                torch.autograd.grad(y.sum(), [leaf])
