@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -135,13 +136,18 @@ bool records(const Tensor& t) {
     return true;
 }
 
-// Gradients of an operator without a second derivative: who differentiates them (create_graph) gets an error, not zeros.
-variable_list once(variable_list grads) {
+// Gradients of an operator without a second derivative: who differentiates them (create_graph) gets an error, not zeros.  They
+// depend on the operator's inputs and on the upstream gradient, so that every way from them to either meets the error.
+variable_list once(variable_list grads, const Tensor& upstream) {
     if (!at::GradMode::is_enabled()) return grads;
+    torch::autograd::edge_list edges;
+    for (const torch::autograd::Edge& edge : torch::autograd::get_current_node()->next_edges())
+        if (edge.is_valid()) edges.push_back(edge);
+    if (upstream.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(upstream));
+    const auto error = std::make_shared<torch::autograd::Error>("this graphmaker_amd operator has no second derivative", std::move(edges));
     for (Tensor& t : grads)
-        if (t.defined()) t.requires_grad_(true);
-    auto error = std::make_shared<torch::autograd::DelayedError>("this graphmaker_amd operator has no second derivative", (int64_t)grads.size());
-    return (*error)(std::move(grads));
+        if (t.defined()) torch::autograd::set_history(t, error);
+    return grads;
 }
 
 // A saved tensor as the backward pass may use it.  Hooks on saved tensors (torch.autograd.graph) can hand it back with other
@@ -199,7 +205,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
                                     row_dtype(g, "gradient"), (float)ctx->saved_data["scale"].toDouble(), out_of<void>(dW), w,
                                     out_of<void>(ws), need, stream_of(g)),
              "gm_token_embedding_bwd");
-        return once({dW, Tensor(), Tensor()});
+        return once({dW, Tensor(), Tensor()}, g);
     }
 };
 
@@ -272,7 +278,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                at_of(gamma), row_dtype(wt.defined() ? wt : g, "gamma"), out_of<void>(dx), N, out_of<void>(dgamma),
                                out_of<void>(dbeta), out_of<void>(ws), need, stream_of(g)),
              "gm_layer_norm_bwd");
-        return once({dx, dgamma, dbeta, Tensor()});
+        return once({dx, dgamma, dbeta, Tensor()}, g);
     }
 };
 
@@ -348,7 +354,7 @@ struct ClassLogProb : torch::autograd::Function<ClassLogProb> {
         call(gm_class_log_prob_bwd(M, V, floats(g), at_of(x.t), x.ld, code, at_of(classes),
                                    is_i64(classes), ctx->saved_data["ignore"].toInt(), floats(stats), out_of<void>(dx), V, stream_of(g)),
              "gm_class_log_prob_bwd");
-        return once({dx, Tensor(), Tensor()});
+        return once({dx, Tensor(), Tensor()}, g);
     }
 };
 
@@ -480,7 +486,7 @@ template <bool POLICY> struct SequenceLoss : torch::autograd::Function<SequenceL
         call(gm_sequence_loss_bwd(M, S, POLICY ? weight + S : nullptr, bytes(mask), at_of(offsets), offsets.defined() && is_i64(offsets),
                                   weight, floats(g), out_of<float>(dl), stream_of(g)),
              "gm_sequence_loss_bwd");
-        return once({dl, Tensor()});
+        return once({dl, Tensor()}, g);
     }
 };
 

@@ -355,3 +355,27 @@ def test_saved_tensors_of_another_kind_are_refused(dev):
                 y = call()
             with pytest.raises(RuntimeError, match="came back as"):
                 torch.autograd.grad(y.sum(), [leaf])
+
+
+def test_second_derivatives_are_refused_however_they_are_asked_for(dev):
+    """Also where only one path is differentiated and a missing one would count as zero: a Hessian, a Jacobian-vector product by
+    two backward passes, a gradient's derivative after the upstream gradient."""
+    x, w = rnd(1, 6, 40).to(dev), rnd(2, 40).to(dev)
+    flat, ref = rnd(3, 6).to(dev), rnd(4, 6).to(dev)
+    tok, off = torch.arange(6, device=dev), torch.tensor([0, 2, 6], device=dev)
+    calls = [(lambda a: ag.layer_norm(a, w).square().sum(), x), (lambda a: ag.layer_norm(a[:, ::2]).sum(), x), (lambda a: ag.layer_norm(x, a).square().sum(), w),
+             (lambda a: ag.token_embedding(a, tok).square().sum(), x), (lambda a: ag.class_log_prob(a, tok).sum(), x),
+             (lambda a: ag.class_log_prob(a[:, :2], tok % 2).sum(), x), (lambda a: ag.policy_loss(a, ref, ref)[0], flat),
+             (lambda a: ag.preference_loss(a, ref, off)[0], flat)]
+    F = torch.autograd.functional
+    for f, at in calls:
+        for ask in (lambda: F.hessian(f, at), lambda: F.jvp(f, at, torch.ones_like(at)), lambda: F.hvp(f, at, torch.ones_like(at)), lambda: F.vhp(f, at, torch.ones_like(at))):
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                ask()
+        a, up = at.clone().requires_grad_(True), torch.ones((), device=dev, requires_grad=True)
+        (da,) = torch.autograd.grad(f(a), [a], up, create_graph=True)
+        for of in (a, up):
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                torch.autograd.grad(da.sum(), [of], allow_unused=True, retain_graph=True)
+        del da
+    assert torch.equal(F.vjp(calls[0][0], x)[1], F.jacobian(calls[0][0], x))     # one backward pass is fine
