@@ -379,3 +379,33 @@ def test_second_derivatives_are_refused_however_they_are_asked_for(dev):
                 torch.autograd.grad(da.sum(), [of], allow_unused=True, retain_graph=True)
         del da
     assert torch.equal(F.vjp(calls[0][0], x)[1], F.jacobian(calls[0][0], x))     # one backward pass is fine
+
+
+@pytest.mark.parametrize("dt, V", [("f32", 2), ("f32", 3), ("bf16", 2), ("bf16", 7), ("f16", 3), ("f16", 7)])
+def test_log_prob_of_a_nearly_certain_class(dev, dt, V):
+    """A draw of a sparse graph is nearly certain: log-probabilities of -1e-3 to -1e-20, and the gradient 1 - p of the class itself,
+    keep their own last places, not those of 1.  The logits are multiples of 1/8 below 48 (the largest of them exact in any type), so that differences are exact: 4 U of an exponential,
+    U of each of up to 6 sums and of 1 + the rest, 3 U of the logarithm and its correction, 2 U of a quotient and a product."""
+    M = 2000
+    gen = torch.Generator().manual_seed(V)
+    x = -(torch.randint(8, 360, (M, V), generator=gen).float() / 8)
+    top = torch.randint(0, V, (M,), generator=gen)
+    x[torch.arange(M), top] = 0.0
+    x += (torch.arange(M) % 5 - 2)[:, None]
+    x = x.to(DT[dt])
+    c = torch.where(torch.arange(M) % 4 > 0, top, (top + 1) % V)
+    g = 1.0 + rnd(1, M).abs()
+    a = x.to(dev).requires_grad_(True)
+    lp = ag.class_log_prob(a, c.to(dev))
+    (dx,) = torch.autograd.grad(lp, [a], g.to(dev))
+    t = x.double() - x.double().gather(1, top[:, None])
+    others = torch.nn.functional.one_hot(top, V).double()
+    rest = (t.exp() * (1 - others)).sum(1)
+    want = t.gather(1, c[:, None])[:, 0] - rest.log1p()
+    assert float(want.abs().min()) < 1e-12
+    close(lp, want, 16 * U * want.abs(), "log-probability")
+    own = torch.nn.functional.one_hot(c, V).double()
+    e = t.exp()
+    grad = g.double()[:, None] / (1 + rest)[:, None] * (own * ((1 - own) * e).sum(1, keepdim=True) - (1 - own) * e)
+    close(dx, grad, 16 * U * grad.abs() + torch.finfo(DT[dt]).eps / 2 * 1.01 * grad.abs()
+          + torch.finfo(DT[dt]).smallest_normal * torch.finfo(DT[dt]).eps, "gradient")
