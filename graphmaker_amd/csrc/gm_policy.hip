@@ -89,41 +89,33 @@ __device__ __forceinline__ float exp_shifted(float x, int shift) {
     const float lo = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
     return __builtin_ldexpf(__builtin_amdgcn_exp2f(t - n) * __builtin_fmaf(lo, 0.693147182f, 1.0f), (int)n - shift);
 }
-// exp(x) less 1, and less 1 + x, times the unit.  Below |x| = 1 from the series, where the differences would cancel (the first
-// term left out is below 1.2 x 2^-24 of the sum)
-struct LessOne {
-    float one, line;
-    __device__ __forceinline__ LessOne(float x, Unit unit) {
-        float p = 2.75573192e-7f;                       // 1/10!
-        p = __builtin_fmaf(p, x, 2.75573192e-6f);
-        p = __builtin_fmaf(p, x, 2.48015873e-5f);
-        p = __builtin_fmaf(p, x, 1.98412698e-4f);
-        p = __builtin_fmaf(p, x, 1.38888889e-3f);
-        p = __builtin_fmaf(p, x, 8.33333333e-3f);
-        p = __builtin_fmaf(p, x, 4.16666667e-2f);
-        p = __builtin_fmaf(p, x, 1.66666667e-1f);
-        p = __builtin_fmaf(p, x, 0.5f);
-        const float xu = x * unit.u;
-        line = p * x * xu;
-        one = xu + line;
-        if (__builtin_expect(!(__builtin_fabsf(x) < 1.0f), 0)) {       // a branch: a model is seldom so far from its reference
-            one = exp_shifted(x, unit.shift) - unit.u;
-            line = one - xu;
-        }
-    }
-};
+// (exp(x) - 1 - x) / x^2 for |x| < 1 (the first term left out is below 1.2 x 2^-24 of the sum)
+__device__ __forceinline__ float exp_series(float x) {
+    float p = 2.75573192e-7f;                           // 1/10!
+    p = __builtin_fmaf(p, x, 2.75573192e-6f);
+    p = __builtin_fmaf(p, x, 2.48015873e-5f);
+    p = __builtin_fmaf(p, x, 1.98412698e-4f);
+    p = __builtin_fmaf(p, x, 1.38888889e-3f);
+    p = __builtin_fmaf(p, x, 8.33333333e-3f);
+    p = __builtin_fmaf(p, x, 4.16666667e-2f);
+    p = __builtin_fmaf(p, x, 1.66666667e-1f);
+    return __builtin_fmaf(p, x, 0.5f);
+}
 
-// What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.  An item's terms are
-// float32: they carry a few 2^-24, and |x| 2^-24 from the rounded difference x of two float32 log-probabilities, which carry as much
-// themselves.  (Of 10,547,784 items these take 41.5 us, 2 to 3 more where every wave has an item past |q| = 1; float64 terms of
-// float32 exponentials take 47 and of float64 ones 54.)
+// What an item adds to its sequence's sums: `add` takes W consecutive items of one sequence, loads first.  An item's exponentials
+// are float32, and carry |x| 2^-24 from the rounded difference x of two float32 log-probabilities, which carry as much themselves.
+// Below |x| = 1, where a model and its near past lie, they are 1 and a small part from the series, off by a few 2^-24 of the part:
+// nothing cancels, and the gain, formed of both in float64 as the clip borders are, keeps its places where advantages cancel.
+// Beyond they are exp_shifted, behind a branch.  (10,547,784 items take 42 us, and 5 more where every wave has items beyond;
+// two float32 exponentials without the branch take 43.6, float64 made of them 47, float64 exponentials 54.)
 template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
     static constexpr int Q = 4;                          // sums: surrogate, KL, clipped items, live items
     struct Acc { double surrogate = 0.0, kl = 0.0; int cut = 0, live = 0; };
     const float *lp, *old, *adv, *ref;
     const uint8_t* mask;
     Unit unit;
-    float low, high, kl;                                 // 1 - clip_low and 1 + clip_high times the unit, KL coefficient
+    double low, high;                                    // 1 - clip_low and 1 + clip_high, times the unit
+    float low_f, high_f, kl;                             // the same, KL coefficient
     float* slope;
     __device__ __forceinline__ float of_sequence(int64_t s) const { return ITEM_ADV ? 0.0f : adv[s]; }
     template <int W> __device__ __forceinline__ void add(int64_t i, float of_seq, Acc& a) const {
@@ -137,17 +129,30 @@ template <bool MASK, bool REF, bool ITEM_ADV> struct PolicyTerm {
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const bool live = !MASK || on.v[k] != 0;
-            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, d_k = l.v[k] - o.v[k], r = exp_shifted(d_k, unit.shift);
-            const bool cut = (adv_k > 0.0f && r > high) || (adv_k < 0.0f && r < low);
-            // no advantage: 0 for a ratio of any finite size, also one past float32; NaN for NaN and for an infinite ratio
-            const float gain = adv_k == 0.0f && d_k < INFINITY ? 0.0f : (cut ? (adv_k > 0.0f ? high : low) : r) * adv_k;
-            float slope_k = cut ? 0.0f : -gain;
-            if constexpr (REF) {
-                const LessOne e(q.v[k] - l.v[k], unit);
-                if (kl != 0.0f) slope_k = slope_k - kl * e.one;
-                a.kl += live ? (double)e.line : 0.0;
+            const float adv_k = ITEM_ADV ? A.v[k] : of_seq, d_k = l.v[k] - o.v[k];
+            // the ratio is base + part, the KL argument's exponential less 1 and less a line are `one` and `line`; all times the unit
+            const float u = unit.u, x = REF ? q.v[k] - l.v[k] : 0.0f, du = d_k * u, xu = x * u;
+            float base = u, part = __builtin_fmaf(exp_series(d_k) * d_k, du, du);
+            float line = REF ? exp_series(x) * x * xu : 0.0f, one = xu + line;
+            if (__builtin_expect(!(__builtin_fabsf(d_k) < 1.0f && __builtin_fabsf(x) < 1.0f), 0)) {
+                if (!(__builtin_fabsf(d_k) < 1.0f)) {    // no advantage: 0 for any finite ratio, also one past float32; NaN for an infinite one
+                    base = 0.0f;
+                    part = adv_k == 0.0f && d_k < INFINITY ? 0.0f : exp_shifted(d_k, unit.shift);
+                }
+                if (!(__builtin_fabsf(x) < 1.0f)) {
+                    one = exp_shifted(x, unit.shift) - u;
+                    line = one - xu;
+                }
             }
-            a.surrogate -= live ? (double)gain : 0.0;
+            const float r = base + part;
+            const bool cut = (adv_k > 0.0f && r > high_f) || (adv_k < 0.0f && r < low_f);
+            const double gain = (cut ? (adv_k > 0.0f ? high : low) : (double)base + (double)part) * (double)adv_k;
+            float slope_k = cut ? 0.0f : -(r * adv_k);
+            if constexpr (REF) {
+                if (kl != 0.0f) slope_k = slope_k - kl * one;
+                a.kl += live ? (double)line : 0.0;
+            }
+            a.surrogate -= live ? gain : 0.0;
             a.cut += live && cut ? 1 : 0;
             a.live += live ? 1 : 0;
             d.v[k] = live ? slope_k : 0.0f;
@@ -179,7 +184,7 @@ template <bool MASK> struct PreferenceTerm {
 };
 
 // pieces of the sequences: `whole`[s] of one inside this chunk; `piece`[2k] of one that began before chunk k,
-// `piece`[2k+1] of one that begins in it and goes on.  HBM-bound: 10,547,784 items with KL and slopes 41.5 us, 4.1 TB/s
+// `piece`[2k+1] of one that begins in it and goes on.  HBM-bound: 10,547,784 items with KL and slopes 42 us, 4.0 TB/s
 template <class F>
 __global__ void __launch_bounds__(256)
 k_sequence_pieces(Sequences q, int64_t chunk, F f, Sums<F::Q>* __restrict__ whole, Sums<F::Q>* __restrict__ piece) {
@@ -538,7 +543,8 @@ extern "C" int gm_policy_loss_fwd(int64_t M, int64_t S, const float* log_prob, c
     const Unit unit = item_unit(M);
     return with_flags(mask != nullptr, ref_log_prob != nullptr, offsets == nullptr, [&](auto m, auto r, auto item) {
         const PolicyTerm<decltype(m)::value, decltype(r)::value, decltype(item)::value> f{
-            log_prob, old_log_prob, advantage, ref_log_prob, mask, unit, (1.0f - clip_low) * unit.u, (1.0f + clip_high) * unit.u, kl_coef, slope};
+            log_prob, old_log_prob, advantage, ref_log_prob, mask, unit, (1.0 - (double)clip_low) * (double)unit.u,
+            (1.0 + (double)clip_high) * (double)unit.u, (1.0f - clip_low) * unit.u, (1.0f + clip_high) * unit.u, kl_coef, slope};
         return launch_sequence_loss(q, f, workspace, workspace_bytes, s, [&](int64_t chunk, int fused, Sums<4>* whole, Sums<4>* piece, void* rest) {
             const unsigned blocks = finish_blocks(S);
             Sums<5>* totals = static_cast<Sums<5>*>(rest);

@@ -409,3 +409,22 @@ def test_log_prob_of_a_nearly_certain_class(dev, dt, V):
     grad = g.double()[:, None] / (1 + rest)[:, None] * (own * ((1 - own) * e).sum(1, keepdim=True) - (1 - own) * e)
     close(dx, grad, 16 * U * grad.abs() + torch.finfo(DT[dt]).eps / 2 * 1.01 * grad.abs()
           + torch.finfo(DT[dt]).smallest_normal * torch.finfo(DT[dt]).eps, "gradient")
+
+
+@pytest.mark.parametrize("share", [0.5, 0.25])
+def test_policy_loss_where_gains_cancel(dev, share):
+    """Clipped items against items of ratio 1 whose advantages make up for them, up to the places that float32 does not have: the
+    borders are 1 - clip_low and 1 + clip_high of the float32 arguments, and what is left is right to one rounding."""
+    M = 4000
+    n = int(M * share)
+    low, high = (float(torch.tensor(v)) for v in (0.2, 0.28))
+    for sign, border in ((1.0, 1 + high), (-1.0, 1 - low)):
+        old, adv = torch.zeros(M), torch.full((M,), sign)
+        old[:n] = -sign                                  # ratio e with an advantage, 1 / e with a disadvantage: clipped
+        adv[n:] = -sign * border * n / (M - n)           # ratio 1
+        a = torch.zeros(M, device=dev, requires_grad=True)
+        loss, stats = ag.policy_loss(a, old.to(dev), adv.to(dev), clip_high=0.28)
+        want = -(n * sign * border + adv[n:].double().sum()) / M
+        assert 0 < abs(float(want)) < 4 * U
+        close(loss, want, 1.01 * U * abs(float(want)) + 2.0 ** -50, "loss")
+        assert float(stats[2]) == share
