@@ -355,7 +355,8 @@ k_log_prob_long_bwd(int64_t M, int N, const float* __restrict__ g, const T* __re
     }
 }
 
-// pieces a row, and lanes and pieces a lane of the held form; lanes = 0: long
+// Pieces a row, and lanes and pieces a lane of the held form; lanes = 0: long.  Up to five pieces: 20,000 x 1280 float32 are held
+// in 17 us forward, 20,000 x 1284 take 34 by a workgroup each.
 struct LogProbShape { int lanes, K; };
 static inline LogProbShape log_prob_shape(int64_t N, int vec) {
     const int64_t v = (N + vec - 1) / vec;

@@ -270,7 +270,8 @@ template <int Q>
 __global__ void __launch_bounds__(256)
 k_sequence_gather(Sequences q, int64_t chunk, int per, Sums<Q>* __restrict__ whole, const Sums<Q>* __restrict__ piece) {
     // a lane looks at each of a wave's `per` sequences, the wave sums those that cross chunks: all of a few thousand may, of
-    // more only as many as there are chunks
+    // more only as many as there are chunks (whole loss with one and with 64 a wave: 8000 sequences 29 and 50 us, 16,384 32 and
+    // 30, a million 200 and 58)
     const int lane = threadIdx.x & 63;
     const int64_t step = (int64_t)gridDim.x * 4 * per;
     for (int64_t base = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per; base < q.S; base += step) {
